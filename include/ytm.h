@@ -353,6 +353,108 @@ ytm_status ytm_infer_noalloc(const ytm_config *cfg, const uint32_t *state, const
  * reference counterpart. */
 ytm_status ytm_match_counters(uint64_t *out, void *stream);
 
+/* ---- From clause outputs to an answer ------------------------------------
+ * Operators beside ytm_infer's class sums for models with many classes: the
+ * vote of clause weights held in 4 bits, the adjustment of class sums with the
+ * choice of a class, and the cross entropy of adjusted class sums with its
+ * gradients.  No counterpart in the reference, whose predict is the argmax of
+ * the class sums (src/cutm/multiclass.py:54-59).  They take plain arrays (no
+ * ytm_config); rows are strided (strides in elements), the elements of a row
+ * contiguous, and a stride of 0 repeats one row.  Indices and sizes are 64-bit
+ * inside.  Calls keep nothing between them and may overlap on different
+ * streams. */
+#define YTM_I32 0
+#define YTM_F32 1
+#define YTM_F16 2
+#define YTM_BF16 3
+#define YTM_BITS 4 /* u32 words, bit j of word w = clause 32*w+j */
+
+/* Quantise clause weights [C][K] (i32 or f32, finite, row stride w_stride) to
+ * 4 bits: per class and `group` (32, 64 or 128) consecutive clauses, with a =
+ * max |w|, scale = a / 7 (rounded to scale_type) and q = round-half-even(7 w /
+ * a) in [-7, 7].  packed u8 [K][16 * ceil(C / 32)]: q + 8, clause c in byte c /
+ * 2, low half when c is even, 8 behind the last clause.  scales [K][ceil(C /
+ * group)]. */
+ytm_status ytm_q4_pack(const void *weights, int32_t w_type, int64_t w_stride, int32_t C, int32_t K, int32_t group,
+                       uint8_t *packed, void *scales, int32_t scale_type, void *stream);
+
+/* Votes y[n][k] = bias[k] + sum_g scale[k][g] * sum_{c in g} (packed[k][c] - 8)
+ * * x[n][c], sums in fp32, rounded once to y_type.  x [N][C] (f32, f16, bf16)
+ * or clause bits (YTM_BITS, x_stride in words); packed on a 16-byte boundary,
+ * halves 0..15; bias f32 [K] or NULL; y [N][K]. */
+ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t N, int32_t C, const uint8_t *packed,
+                        const void *scales, int32_t scale_type, int32_t group, int32_t K, const float *bias, void *y,
+                        int32_t y_type, void *stream);
+
+/* Fired clauses of inference as bits u32 [N][ceil(C / 32)] (bits behind the
+ * last clause 0): the clauses ytm_infer counts, i.e. without those that
+ * include nothing unless cfg->count_empty.  workspace:
+ * ytm_workspace_bytes(cfg, YTM_OP_INFER, N). */
+ytm_status ytm_infer_fired(const ytm_config *cfg, const uint32_t *state, const uint32_t *lits, int64_t N,
+                           uint32_t *fired, void *workspace, void *stream);
+
+/* Adjusted class sums and the choice.  With v = cs[n][k] and c the number of
+ * times k occurs in the first lengths[n] entries of history[n]:
+ *   if c > 0: v = (v > 0 ? v / repetition : v * repetition) - frequency * c - presence
+ *   z = allowed ? (v + bias) / temperature : -inf
+ * in 64 bits, rounded once to fp32.  choice = the lowest class of the largest
+ * z (NaN above all numbers), -1 if no class is allowed; logprob =
+ * log softmax(z)[choice], -inf if no class is allowed. */
+typedef struct ytm_answer_args {
+    const void *cs;          /* [n][k], cs_type i32, f32, f16 or bf16          */
+    int64_t cs_stride;
+    int64_t n;
+    int32_t k;
+    int32_t cs_type;
+    const float *bias;       /* [n][k], or NULL                                */
+    int64_t bias_stride;
+    const uint32_t *allowed; /* bits [n][ceil(k / 32)], or NULL: all classes   */
+    int64_t allowed_stride;
+    const void *history;     /* [n][history_len] class indices, or NULL;
+                                entries outside [0, k) count for nothing       */
+    int64_t history_stride;
+    int32_t history_len;
+    int32_t history_64;      /* indices are i64 (else i32)                     */
+    const int32_t *lengths;  /* [n], clamped to 0..history_len; NULL: all      */
+    const float *repetition, *frequency, *presence, *temperature; /* [n] or
+                                NULL: the value for all rows below             */
+    float repetition_all, frequency_all, presence_all, temperature_all;
+    int64_t *choice;         /* [n], or NULL                                   */
+    float *logprob;          /* [n], or NULL                                   */
+    float *adjusted;         /* z [n][k], or NULL                              */
+} ytm_answer_args;
+
+ytm_status ytm_answer(const ytm_answer_args *args, void *stream);
+
+/* Cross entropy with z as above (no penalties): loss[n] = weight[n] *
+ * (log sum exp z - z[target[n]]), and with d = weight (softmax z - onehot) the
+ * gradients dcs = d / temperature, dbias = sum_n d / temperature and
+ * dtemperature = -sum d z / temperature, summed in a fixed order.  Rows whose
+ * target lies outside [0, k) or whose weight is 0 count for nothing; a target
+ * that the mask forbids gives a loss of weight * inf and no gradient. */
+typedef struct ytm_loss_args {
+    const void *cs;           /* [n][k], cs_type i32, f32, f16 or bf16         */
+    int64_t cs_stride;
+    int64_t n;
+    int32_t k;
+    int32_t cs_type;
+    const float *bias;        /* [k], or NULL                                  */
+    const uint32_t *allowed;  /* bits [n][ceil(k / 32)], or NULL               */
+    int64_t allowed_stride;
+    const void *target;       /* [n] class indices                             */
+    const float *weight;      /* [n], or NULL: 1                               */
+    const float *temperature; /* one value, or NULL: temperature_all           */
+    float temperature_all;
+    int32_t target_64;        /* targets are i64 (else i32)                    */
+    float *loss;              /* [n]                                           */
+    void *dcs;                /* [n][k] of cs_type (not i32), or NULL          */
+    float *dbias;             /* [k], or NULL                                  */
+    float *dtemperature;      /* one value, or NULL                            */
+} ytm_loss_args;
+
+uint64_t ytm_class_loss_workspace_bytes(int64_t n, int32_t k);
+ytm_status ytm_class_loss(const ytm_loss_args *args, void *workspace, void *stream);
+
 /* Message of the last failing call on this thread ("" if none). */
 const char *ytm_last_error(void);
 

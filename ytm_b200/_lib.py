@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(HERE, "libytm.so")
 YTM_OK = 0
 YTM_OP_ENCODE, YTM_OP_INFER, YTM_OP_TRANSFORM, YTM_OP_TRAIN, YTM_OP_TRAIN_B1, YTM_OP_ENCODE_THERMO = 1, 2, 3, 4, 5, 6
 YTM_OP_TRAIN_LOOP = 7
+YTM_I32, YTM_F32, YTM_F16, YTM_BF16, YTM_BITS = 0, 1, 2, 3, 4
 
 # Every function include/ytm.h declares; tests check the library exports them.
 EXPORTS = (
@@ -26,6 +27,7 @@ EXPORTS = (
     "ytm_encode_thermometer", "ytm_nccl_unique_id", "ytm_nccl_comm_init", "ytm_nccl_comm_destroy",
     "ytm_train_fit_batches", "ytm_peer_ar_create", "ytm_peer_ar_open", "ytm_peer_allreduce_i32",
     "ytm_peer_ar_status", "ytm_peer_ar_destroy", "ytm_config_size", "ytm_match_counters",
+    "ytm_q4_pack", "ytm_q4_votes", "ytm_infer_fired", "ytm_answer", "ytm_class_loss", "ytm_class_loss_workspace_bytes",
 )
 
 
@@ -54,6 +56,31 @@ class Config(ct.Structure):
         ("one_negative", ct.c_int32), ("count_empty", ct.c_int32),
         ("input_images", ct.c_int32), ("image_words", ct.c_int32),
         ("run_range", ct.c_uint32 * 8),
+    ]
+
+
+class AnswerArgs(ct.Structure):
+    """Mirror of struct ytm_answer_args."""
+    _fields_ = [
+        ("cs", ct.c_void_p), ("cs_stride", ct.c_int64), ("n", ct.c_int64), ("k", ct.c_int32), ("cs_type", ct.c_int32),
+        ("bias", ct.c_void_p), ("bias_stride", ct.c_int64), ("allowed", ct.c_void_p), ("allowed_stride", ct.c_int64),
+        ("history", ct.c_void_p), ("history_stride", ct.c_int64), ("history_len", ct.c_int32),
+        ("history_64", ct.c_int32), ("lengths", ct.c_void_p),
+        ("repetition", ct.c_void_p), ("frequency", ct.c_void_p), ("presence", ct.c_void_p),
+        ("temperature", ct.c_void_p), ("repetition_all", ct.c_float), ("frequency_all", ct.c_float),
+        ("presence_all", ct.c_float), ("temperature_all", ct.c_float),
+        ("choice", ct.c_void_p), ("logprob", ct.c_void_p), ("adjusted", ct.c_void_p),
+    ]
+
+
+class LossArgs(ct.Structure):
+    """Mirror of struct ytm_loss_args."""
+    _fields_ = [
+        ("cs", ct.c_void_p), ("cs_stride", ct.c_int64), ("n", ct.c_int64), ("k", ct.c_int32), ("cs_type", ct.c_int32),
+        ("bias", ct.c_void_p), ("allowed", ct.c_void_p), ("allowed_stride", ct.c_int64),
+        ("target", ct.c_void_p), ("weight", ct.c_void_p), ("temperature", ct.c_void_p),
+        ("temperature_all", ct.c_float), ("target_64", ct.c_int32),
+        ("loss", ct.c_void_p), ("dcs", ct.c_void_p), ("dbias", ct.c_void_p), ("dtemperature", ct.c_void_p),
     ]
 
 
@@ -95,6 +122,12 @@ _SIGS = {
     "ytm_peer_allreduce_i32": ([_P, _P, _I64, _I64, _P], ct.c_int),
     "ytm_peer_ar_status": ([_P, ct.POINTER(ct.c_int32)], ct.c_int),
     "ytm_peer_ar_destroy": ([_P], ct.c_int),
+    "ytm_q4_pack": ([_P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I32, _P], ct.c_int),
+    "ytm_q4_votes": ([_P, _I32, _I64, _I64, _I32, _P, _P, _I32, _I32, _I32, _P, _P, _I32, _P], ct.c_int),
+    "ytm_infer_fired": ([_CFG, _P, _P, _I64, _P, _P, _P], ct.c_int),
+    "ytm_answer": ([ct.POINTER(AnswerArgs), _P], ct.c_int),
+    "ytm_class_loss": ([ct.POINTER(LossArgs), _P, _P], ct.c_int),
+    "ytm_class_loss_workspace_bytes": ([_I64, _I32], _U64),
     "ytm_last_error": ([], ct.c_char_p),
     "ytm_version": ([], ct.c_char_p),
     "ytm_config_size": ([], ct.c_int32),

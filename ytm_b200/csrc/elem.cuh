@@ -1,0 +1,51 @@
+// elem.cuh — element types of the answer operators.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace ytm {
+
+inline bool is_float_type(int t) { return t == YTM_F32 || t == YTM_F16 || t == YTM_BF16; }
+inline int64_t type_bytes(int t) { return t == YTM_F16 || t == YTM_BF16 ? 2 : 4; }
+
+__host__ __device__ inline int64_t q4_row_bytes(int C) { return ((int64_t)C + 31) / 32 * 16; }
+
+__device__ __forceinline__ float to_f32(int32_t v) { return (float)v; }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+__device__ __forceinline__ double to_f64(int32_t v) { return (double)v; }
+__device__ __forceinline__ double to_f64(float v) { return (double)v; }
+__device__ __forceinline__ double to_f64(__half v) { return (double)__half2float(v); }
+__device__ __forceinline__ double to_f64(__nv_bfloat16 v) { return (double)__bfloat162float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Element c of the row of x that starts at element `row` (packed bits: word).
+template <int X>
+__device__ __forceinline__ float load_x(const void *x, int64_t row, int c) {
+    if (X == YTM_BITS) return (float)((((const uint32_t *)x)[row + c / 32] >> (c % 32)) & 1u);
+    if (X == YTM_F32) return ((const float *)x)[row + c];
+    if (X == YTM_F16) return __half2float(((const __half *)x)[row + c]);
+    return __bfloat162float(((const __nv_bfloat16 *)x)[row + c]);
+}
+
+// Bit k of a row of allowed-class words (NULL: every class is allowed).
+__device__ __forceinline__ bool is_allowed(const uint32_t *row, int64_t k) {
+    return !row || ((row[k >> 5] >> (k & 31)) & 1u);
+}
+
+}  // namespace ytm

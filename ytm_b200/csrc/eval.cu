@@ -669,6 +669,20 @@ __global__ void k_expand(const uint32_t *__restrict__ fired, int64_t N, int C, u
     }
 }
 
+// fired &= clauses that include something (kernel.cu:328): a warp makes the
+// keep word of 32 clauses by ballot and clears the others in its samples.
+__global__ void __launch_bounds__(256) k_drop_empty(const int32_t *__restrict__ ninc, int C, int64_t N,
+                                                    uint32_t *__restrict__ fired) {
+    const int CWn = (C + 31) / 32, lane = threadIdx.x & 31;
+    for (int w = blockIdx.x * 8 + (threadIdx.x >> 5); w < CWn; w += gridDim.x * 8) {
+        const int c = w * 32 + lane;
+        const uint32_t keep = __ballot_sync(0xFFFFFFFFu, c < C && ninc[c] != 0);
+        if (keep == 0xFFFFFFFFu) continue;
+        for (int64_t n = (int64_t)blockIdx.y * 32 + lane; n < N; n += (int64_t)gridDim.y * 32)
+            fired[n * CWn + w] &= keep;
+    }
+}
+
 // One thread per (sample, clause): pick a matching patch uniformly
 // (reference select_active, kernel.cu:285-316, reservoir sampling; here the
 // TAG_PATCH draw r gives index floor(r * count / 2^32) among the matches in
@@ -759,6 +773,28 @@ ytm_status ytm_infer_include(const ytm_config *cfg, const uint32_t *inc, const i
     if ((rc = launch_match_any(cfg, inc, lits, N, ws + l.total + cs_planes_bytes(cfg), fired, st))) return rc;
     return launch_cs_planes(fired, cfg->count_empty ? nullptr : ninc, weights, bias, cfg, N, 0, cs, ws + l.total,
                             st);
+}
+
+ytm_status ytm_infer_fired(const ytm_config *cfg, const uint32_t *state, const uint32_t *lits, int64_t N,
+                           uint32_t *fired, void *workspace, void *stream) {
+    ytm_status rc = check_cfg(cfg);
+    if (rc) return rc;
+    if (N < 0) return fail(YTM_ERR_ARG, "N < 0");
+    if (N == 0) return YTM_OK;
+    if (!state || !lits || !fired || !workspace) return fail(YTM_ERR_ARG, "null pointer");
+    cudaStream_t st = as_stream(stream);
+    const int C = cfg->clause_count, W = cfg->words;
+    InferWs l = infer_ws_layout(cfg, N);
+    char *ws = (char *)workspace;
+    int32_t *ninc = (int32_t *)(ws + l.ninc);
+    const uint32_t *inc = state + (int64_t)(cfg->planes - 1) * C * W;
+    if ((rc = cuda_check(cudaMemsetAsync(fired, 0, (size_t)N * cdiv(C, 32) * 4, st), "memset"))) return rc;
+    if ((rc = launch_match_any(cfg, inc, lits, N, ws + l.total + cs_planes_bytes(cfg), fired, st))) return rc;
+    if (cfg->count_empty) return YTM_OK;
+    if ((rc = launch_ninc(cfg, state, ninc, st))) return rc;
+    const dim3 grid((unsigned)cdiv(cdiv(C, 32), 8), (unsigned)std::min<uint64_t>(cdiv(N, 32), 1024));
+    k_drop_empty<<<grid, 256, 0, st>>>(ninc, C, N, fired);
+    return launch_check("empty clauses");
 }
 
 ytm_status ytm_transform(const ytm_config *cfg, const uint32_t *state, const uint32_t *lits, int64_t N,

@@ -490,8 +490,10 @@ class BaseTM:
         dist.all_gather(parts, cs, group=self._pg)
         return torch.cat(parts)[:N]
 
-    def _score_device(self, lits: torch.Tensor, chunk: int | None = None) -> torch.Tensor:
+    def _score_device(self, lits: torch.Tensor, chunk: int | None = None, votes=None) -> torch.Tensor:
         N = lits.shape[0]
+        if votes is not None and self.world > 1:
+            raise NotImplementedError("packed votes are for models held by one process")
         if self.world > 1 and self.inference_sharding == "samples":
             return self._score_samples_sharded(lits)
         if chunk is None:
@@ -501,10 +503,22 @@ class BaseTM:
             chunk = max(1, min(N, (1 << 31) // per))
         outs = []
         for i in range(0, N, chunk):
+            if votes is not None:
+                outs.append(self.engine.infer_packed(lits[i:i + chunk], votes))
+                continue
             cs = self.engine.infer(lits[i:i + chunk], add_bias=self.rank == 0)
             outs.append(self._allreduce(cs))
-        return torch.cat(outs) if outs else torch.empty((0, self.number_of_outputs), dtype=torch.int32,
-                                                       device=self.device)
+        return torch.cat(outs) if outs else torch.empty((0, self.number_of_outputs), device=self.device,
+                                                       dtype=torch.int32 if votes is None else torch.float32)
+
+    def pack_votes(self, group: int = 64, scale_dtype: torch.dtype = torch.float32):
+        """The clause weights as they are now in 4 bits, with a scale for every
+        `group` (32, 64, 128) clauses of a class: pass the result as `votes` to
+        score, predict or answer, which then read an eighth of the weights'
+        bytes and give class sums of the rounded weights.  One process only."""
+        if self.world > 1:
+            raise NotImplementedError("packed votes are for models held by one process")
+        return self.engine.pack_votes(group, scale_dtype)
 
     def _score_batch(self, encoded_X, block_size: int | None = None) -> np.ndarray:
         lits = self._literals_device(encoded_X, True)

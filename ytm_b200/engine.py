@@ -11,16 +11,29 @@ u32 data live in int32 tensors (same bytes); numpy views reinterpret them.
 from __future__ import annotations
 
 import ctypes as ct
+from dataclasses import dataclass
 
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, answers
 from ._lib import check
 
 
 def _p(t):
     return None if t is None else ct.c_void_p(t.data_ptr())
+
+
+@dataclass(frozen=True)
+class PackedVotes:
+    """Clause weights in 4 bits (answers.q4_pack): what inference reads of them
+    is an eighth of the int32 weights plus the scales.  A copy: later training
+    does not change it."""
+    packed: torch.Tensor
+    scales: torch.Tensor
+    group: int
+    clauses: int
+    bias: torch.Tensor
 
 
 class CudaEngine:
@@ -191,6 +204,31 @@ class CudaEngine:
             check(self.lib.ytm_infer_include(ct.byref(cfg_full), _p(inc), _p(weights), _p(bias), _p(lits), N, _p(cs),
                                              _p(ws), self._stream()), "ytm_infer_include")
         return cs
+
+    def infer_fired(self, lits: torch.Tensor) -> torch.Tensor:
+        """The clauses that infer counts, as bits int32 [N, ceil(C / 32)]."""
+        c = self._cfg_for(lits)
+        N = lits.shape[0]
+        out = torch.empty((N, (self.C + 31) // 32), dtype=torch.int32, device=self.device)
+        if N == 0:
+            return out
+        ws = self.workspace(_lib.YTM_OP_INFER, N, c)
+        with torch.cuda.device(self.device):
+            check(self.lib.ytm_infer_fired(c, _p(self.state), _p(lits), N, _p(out), _p(ws), self._stream()),
+                  "ytm_infer_fired")
+        return out
+
+    def pack_votes(self, group: int = 64, scale_dtype: torch.dtype = torch.float32) -> "PackedVotes":
+        """The clause weights as they are now, in 4 bits with group scales."""
+        packed, scales = answers.q4_pack(self.weights, group, scale_dtype)
+        return PackedVotes(packed, scales, group, self.C, self.bias.to(torch.float32))
+
+    def infer_packed(self, lits: torch.Tensor, votes: "PackedVotes") -> torch.Tensor:
+        """Class sums float32 [N, K] under packed weights."""
+        if votes.clauses != self.C or votes.packed.shape[0] != self.K:
+            raise ValueError("the packed votes are another model's")
+        return answers.q4_votes(self.infer_fired(lits), votes.packed, votes.scales, votes.group, bias=votes.bias,
+                                clauses=self.C)
 
     def transform(self, lits: torch.Tensor) -> torch.Tensor:
         c = self._cfg_for(lits)
