@@ -60,7 +60,9 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
     for kw in (dict(k=0), dict(n=-1), dict(cs_type=4), dict(cs=None), dict(dcs=16), dict(target=None), dict(loss=None),
                dict(cs_stride=-1), dict(allowed_stride=-1)):
         assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, **kw})), one, None) == 1, kw
-    assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**good)), None, None) == 1
+    assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "n": 100000})), None, None) == 1
+    assert lib.ytm_class_loss_workspace_bytes(100000, 4) > 0
+    assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "k": 262145})), one, None) == 3
     assert lib.ytm_class_loss(None, one, None) == 1
     assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "n": 0})), None, None) == 0
     assert lib.ytm_class_loss_workspace_bytes(-1, 4) == 0

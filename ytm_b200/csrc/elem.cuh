@@ -11,6 +11,7 @@
 namespace ytm {
 
 inline bool is_float_type(int t) { return t == YTM_F32 || t == YTM_F16 || t == YTM_BF16; }
+inline bool is_sum_type(int t) { return is_float_type(t) || t == YTM_I32; }
 inline int64_t type_bytes(int t) { return t == YTM_F16 || t == YTM_BF16 ? 2 : 4; }
 
 __host__ __device__ inline int64_t q4_row_bytes(int C) { return ((int64_t)C + 31) / 32 * 16; }
@@ -46,6 +47,10 @@ __device__ __forceinline__ float load_x(const void *x, int64_t row, int c) {
 // Bit k of a row of allowed-class words (NULL: every class is allowed).
 __device__ __forceinline__ bool is_allowed(const uint32_t *row, int64_t k) {
     return !row || ((row[k >> 5] >> (k & 31)) & 1u);
+}
+
+__device__ __forceinline__ int64_t index_at(const void *p, int is64, int64_t i) {
+    return is64 ? ((const int64_t *)p)[i] : (int64_t)((const int32_t *)p)[i];
 }
 
 }  // namespace ytm
