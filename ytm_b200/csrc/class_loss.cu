@@ -1,17 +1,19 @@
 // class_loss.cu — cross entropy of biased, masked, tempered class sums with
-// its gradients, in one pass over the class sums.
+// its gradients.
 //
 // In units of log2 e: with c = log2(e) / t and z = (v + b) c (allowed classes),
 //   e_k = 2^(z_k - m), s = sum e, h = sum e (z - m)         (m = max z)
 //   loss = w (ln s - (z_y - m) ln 2)
 //   dcs_k = (w / t) (e_k / s - 1[k = y]),  dbias = sum_n dcs
 //   dt = -(ln 2 / t) sum_n w (h / s - (z_y - m))
-// so the row's exponentials are kept in registers between the sum and the
-// gradient, h needs no second look at z, and the class sums are read once.
-// A thread keeps the same classes from row to row, so that dbias is summed in
-// its registers; what the blocks have summed is added by a second small
-// kernel in a fixed order.
-#include <cooperative_groups.h>
+// so that h gives the temperature's gradient without another look at z.
+//
+// Rows of up to 1024 classes stay in the registers of 4 to 32 threads between
+// the sum and the gradient (k_loss_small).  Longer rows take two streams over
+// the class sums, which need no barrier: k_loss_stat for (m, s, h), then
+// k_loss_grad, whose threads keep their classes over a chunk of rows.  Both
+// kernels sum dbias in registers and leave one part per team or chunk, which
+// k_loss_join adds in a fixed order.
 #include <limits.h>
 #include <math.h>
 
@@ -21,8 +23,6 @@
 #include "elem.cuh"
 
 namespace ytm {
-
-namespace cg = cooperative_groups;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -36,22 +36,20 @@ __device__ __forceinline__ float ex2(float x) {
 // largest class's exponent off 0.
 __device__ __forceinline__ float loss_z(float v, float b, float c) { return __fmul_rn(__fadd_rn(v, b), c); }
 
-// What a row needs besides its class sums.
-struct LossRow {
-    float w, zy;
+// A row's label, weight and label's mask bit.  y < 0: the row counts for
+// nothing; open: it has a gradient.
+struct LossLabel {
     int y;
-    bool use, open;
+    float w;
+    bool open;
 };
 
-template <typename T>
-__device__ __forceinline__ LossRow loss_row(const ytm_loss_args &a, int64_t n, float c) {
-    LossRow r;
+__device__ __forceinline__ LossLabel loss_label(const ytm_loss_args &a, int64_t n) {
+    LossLabel r;
     const int64_t y = index_at(a.target, a.target_64, n);
     r.w = a.weight ? a.weight[n] : 1.f;
-    r.use = y >= 0 && y < a.k && r.w != 0.f;
-    r.y = r.use ? (int)y : 0;
-    r.open = r.use && is_allowed(a.allowed ? a.allowed + n * a.allowed_stride : nullptr, r.y);
-    r.zy = loss_z(to_f32(((const T *)a.cs)[n * a.cs_stride + r.y]), a.bias ? a.bias[r.y] : 0.f, c);
+    r.y = y >= 0 && y < a.k && r.w != 0.f ? (int)y : -1;
+    r.open = r.y >= 0 && is_allowed(a.allowed ? a.allowed + n * a.allowed_stride : nullptr, r.y);
     return r;
 }
 
@@ -59,7 +57,7 @@ __device__ __forceinline__ float loss_rt(const ytm_loss_args &a) {
     return 1.f / (a.temperature ? *a.temperature : a.temperature_all);
 }
 
-// Partial sums of a block (or cluster): dbias [G][k], then dt / (-ln 2 / t) [G].
+// Partial sums of the teams or chunks: dbias [G][k], dt / (-ln 2 / t) [G].
 struct LossPart {
     float *db;
     double *dt;
@@ -129,37 +127,73 @@ __global__ void __launch_bounds__(LS_THREADS, NV >= 4 ? 2 : NV == 2 ? 3 : 4) k_l
             acc[j][i] = 0.f;
         }
     }
-    double dt = 0.0;
-    for (int64_t n0 = (int64_t)blockIdx.x * ROWS; n0 < a.n; n0 += (int64_t)gridDim.x * ROWS) {
-        const bool live = n0 + team < a.n;
-        const int64_t n = live ? n0 + team : a.n - 1;
+    // A row's loads are issued a round ahead, and its label's two rounds ahead,
+    // so that the label's class sum, which waits for the label, comes in time.
+    const auto clamped = [&](int64_t n) { return n < a.n ? n : a.n - 1; };
+    struct Row {
+        Vec4<T> v[NV];
+        uint32_t open;
+        T vy;
+        float by;
+        LossLabel label;
+    };
+    const auto fetch = [&](int64_t n0, const LossLabel &label) {
+        Row r;
+        const int64_t n = clamped(n0 + team);
         const T *cs = (const T *)a.cs + n * a.cs_stride;
-        const LossRow row = loss_row<T>(a, n, c);
-        float z[NV][4], m = -INFINITY;
+        r.open = shared_open;
+        r.label = label;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            uint32_t open = shared_open >> (4 * j);
-            if (a.allowed_stride) open &= small_open<TPR, NV, VEC>(a.allowed + n * a.allowed_stride, lane, j, K);
-            Vec4<T> v;
             if (VEC) {
                 const int k = small_class<TPR, NV, VEC>(lane, j, 0);
                 if (k + 4 <= K) {
-                    if constexpr (sizeof(T) == 4) *(uint4 *)&v = *(const uint4 *)(cs + k);
-                    else *(uint2 *)&v = *(const uint2 *)(cs + k);
+                    if constexpr (sizeof(T) == 4) *(uint4 *)&r.v[j] = *(const uint4 *)(cs + k);
+                    else *(uint2 *)&r.v[j] = *(const uint2 *)(cs + k);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v.v[i] = cs[min(k + i, K - 1)];
+                    for (int i = 0; i < 4; ++i) r.v[j].v[i] = cs[min(k + i, K - 1)];
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v.v[i] = cs[min(small_class<TPR, NV, VEC>(lane, j, i), K - 1)];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                z[j][i] = (open >> i) & 1u ? loss_z(to_f32(v.v[i]), KEEP ? b[KEEP ? j : 0][i] : bias_of(j, i), c) : -INFINITY;
-                m = fmaxf(m, z[j][i]);
+                for (int i = 0; i < 4; ++i) r.v[j].v[i] = cs[min(small_class<TPR, NV, VEC>(lane, j, i), K - 1)];
             }
         }
+        if (a.allowed_stride) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                bits |= small_open<TPR, NV, VEC>(a.allowed + n * a.allowed_stride, lane, j, K) << (4 * j);
+            r.open &= bits;
+        }
+        const int y = max(label.y, 0);
+        r.vy = cs[y];
+        r.by = a.bias ? a.bias[y] : 0.f;
+        return r;
+    };
+    double dt = 0.0;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t n0 = (int64_t)blockIdx.x * ROWS;
+    LossLabel label1 = loss_label(a, clamped(n0 + step + team));
+    Row next = fetch(n0, loss_label(a, clamped(n0 + team)));
+    for (; n0 < a.n; n0 += step) {
+        const Row row = next;
+        if (n0 + step < a.n) {
+            next = fetch(n0 + step, label1);
+            label1 = loss_label(a, clamped(n0 + 2 * step + team));
+        }
+        const bool live = n0 + team < a.n;
+        const int64_t n = clamped(n0 + team);
+        float z[NV][4], m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                z[j][i] = (row.open >> (4 * j + i)) & 1u
+                              ? loss_z(to_f32(row.v[j].v[i]), KEEP ? b[KEEP ? j : 0][i] : bias_of(j, i), c)
+                              : -INFINITY;
+                m = fmaxf(m, z[j][i]);
+            }
 #pragma unroll
         for (int d = TPR / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
         float s = 0.f, h = 0.f;
@@ -177,15 +211,15 @@ __global__ void __launch_bounds__(LS_THREADS, NV >= 4 ? 2 : NV == 2 ? 3 : 4) k_l
             s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
             h += __shfl_xor_sync(0xFFFFFFFFu, h, d);
         }
-        const bool use = live && row.open;
-        const float wt = row.w * rt, f = wt / s;
+        const bool use = live && row.label.open;
+        const float wt = row.label.w * rt, f = wt / s;
         T *dcs = (T *)a.dcs + n * (int64_t)K;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float d = z[j][i] * f;
-                if (small_class<TPR, NV, VEC>(lane, j, i) == row.y) d -= wt;
+                if (small_class<TPR, NV, VEC>(lane, j, i) == row.label.y) d -= wt;
                 z[j][i] = use ? d : 0.f;
                 acc[j][i] += z[j][i];
             }
@@ -209,9 +243,9 @@ __global__ void __launch_bounds__(LS_THREADS, NV >= 4 ? 2 : NV == 2 ? 3 : 4) k_l
             }
         }
         if (lane == 0 && live) {
-            const float gap = row.zy - m;
-            a.loss[n] = use ? row.w * (logf(s) - gap * LN2) : row.use ? row.w * INFINITY : 0.f;
-            if (use) dt += (double)row.w * (double)(h / s - gap);
+            const float w = row.label.w, gap = loss_z(to_f32(row.vy), row.by, c) - m;
+            a.loss[n] = use ? w * (logf(s) - gap * LN2) : row.label.y >= 0 ? w * INFINITY : 0.f;
+            if (use) dt += (double)w * (double)(h / s - gap);
         }
     }
     // the block's sums, teams in order
@@ -240,10 +274,6 @@ __global__ void __launch_bounds__(LS_THREADS, NV >= 4 ? 2 : NV == 2 ? 3 : 4) k_l
 }
 
 // -------------------------------------------------- rows of many classes
-// A block, or a cluster of up to 16 blocks, holds a row, E classes a thread:
-// vectors of 16 bytes where the rows are 16-byte aligned, else neighbouring
-// lanes take neighbouring classes.  Blocks of a cluster exchange (m, s, h) by
-// writing into each other's shared memory.
 
 struct LossStat {
     float m, s, h;
@@ -261,182 +291,216 @@ __device__ __forceinline__ LossStat merge(const LossStat &a, const LossStat &b) 
                       __fmul_rn(fb, fmaf(b.s, fmaxf(db, -1024.f), b.h)))};
 }
 
-// Blocks an SM holds: 128 registers a thread at 32 classes, 80 at 16, 64 at 8.
-constexpr int big_blocks(int threads, int e) { return e == 32 ? 512 / threads : e == 16 ? 3 : 4; }
+constexpr int LB_THREADS = 256;
+constexpr int LB_PART = LB_THREADS * 16;  // classes that a block of k_loss_stat takes in one round
 
-template <typename T, int THREADS, int E, bool VEC>
-__global__ void __launch_bounds__(THREADS, big_blocks(THREADS, E)) k_loss_big(const ytm_loss_args a, const LossPart part, int cluster) {
-    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = E / V, WARPS = THREADS / 32;
-    __shared__ LossStat warp_stat[2][WARPS], block_stat[2][16];
-    const int tid = threadIdx.x, K = a.k;
-    const int rank = cluster > 1 ? (int)cg::this_cluster().block_rank() : 0;
-    const int team = blockIdx.x / cluster, teams = gridDim.x / cluster;
-    const int k0 = rank * THREADS * E + tid * V;  // class (j, i): k0 + j * THREADS * V + i
-    const float rt = loss_rt(a), c = rt * LOG2E;
-    float b[E], acc[E];
+// E classes of a row from k0 on, as z (-inf where closed or behind the row):
+// vectors of 16 bytes THREADS apart (VEC: rows, bias and gradients on 16-byte
+// boundaries), else single classes THREADS apart, so that a warp's loads are
+// neighbours and its mask bits those of one word.
+template <typename T, int E, bool VEC>
+struct Classes {
+    static constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = E / V;
+    __device__ static __forceinline__ int first(int tid) { return tid * V; }
+    __device__ static __forceinline__ int at(int e) { return e / V * LB_THREADS * V + e % V; }
+
+    __device__ static __forceinline__ void load_bias(const float *bias, int k0, int K, float (&b)[E]) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int k = k0 + e / V * THREADS * V + e % V;
-        b[e] = a.bias && k < K ? a.bias[k] : 0.f;
-        acc[e] = 0.f;
+        for (int j = 0; j < NV; ++j) {
+            const int k = k0 + at(j * V);
+            if (VEC && bias && k + V <= K) {
+#pragma unroll
+                for (int i = 0; i < V / 4; ++i) *(float4 *)&b[j * V + 4 * i] = *(const float4 *)(bias + k + 4 * i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) b[j * V + i] = bias && k + i < K ? bias[k + i] : 0.f;
+            }
+        }
     }
+
+    __device__ static __forceinline__ void load(const T *cs, int k0, int K, T (&raw)[E]) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int k = k0 + at(j * V);
+            if (VEC && k + V <= K) *(uint4 *)&raw[j * V] = *(const uint4 *)(cs + k);
+            else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) raw[j * V + i] = k + i < K ? cs[k + i] : T(0.f);
+            }
+        }
+    }
+
+    // Bit e: class e is there and allowed.
+    __device__ static __forceinline__ uint32_t open(const uint32_t *allowed, int k0, int K) {
+        uint32_t o = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int k = k0 + at(j * V);
+            if (k < K) o |= ((allowed ? allowed[k >> 5] >> (k & 31) : ~0u) & (k + V <= K ? (1u << V) - 1u : (1u << (K - k)) - 1u)) << (j * V);
+        }
+        return o;
+    }
+};
+
+// (m, s, h) of `rounds` rounds of LB_PART classes of one row: block (part, row).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args a, LossStat *__restrict__ stats, int rounds) {
+    using C = Classes<T, 16, VEC>;
+    __shared__ LossStat warp_stat[LB_THREADS / 32];
+    const int K = a.k;
+    const int64_t n = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+    if (n >= a.n) return;
+    const float c = loss_rt(a) * LOG2E;
+    const T *cs = (const T *)a.cs + n * a.cs_stride;
+    const uint32_t *allowed = a.allowed ? a.allowed + n * a.allowed_stride : nullptr;
+    LossStat st = {-INFINITY, 0.f, 0.f};
+    int k0 = (int)blockIdx.x * rounds * LB_PART + C::first(threadIdx.x);
+    const int end = min(K, (int)min((int64_t)K, (int64_t)(blockIdx.x + 1) * rounds * LB_PART));
+    for (; k0 < end; k0 += LB_PART) {
+        T raw[16];
+        float b[16], z[16], m = st.m;
+        C::load(cs, k0, K, raw);
+        C::load_bias(a.bias, k0, K, b);
+        const uint32_t open = C::open(allowed, k0, K);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            z[e] = (open >> e) & 1u ? loss_z(to_f32(raw[e]), b[e], c) : -INFINITY;
+            m = fmaxf(m, z[e]);
+        }
+        const float base = m == -INFINITY ? 0.f : m;  // nothing yet: every e is 0
+        const float d = st.m == m ? 0.f : st.m - m, f = ex2(d);
+        st.h = f * fmaf(st.s, fmaxf(d, -1024.f), st.h);
+        st.s *= f;
+        st.m = m;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float x = z[e] - base, p = ex2(x);
+            st.s += p;
+            st.h = fmaf(p, fmaxf(x, -1024.f), st.h);  // 0 * -inf counts for nothing
+        }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1)
+        st = merge(st, {__shfl_xor_sync(0xFFFFFFFFu, st.m, d), __shfl_xor_sync(0xFFFFFFFFu, st.s, d),
+                        __shfl_xor_sync(0xFFFFFFFFu, st.h, d)});
+    if ((threadIdx.x & 31) == 0) warp_stat[threadIdx.x >> 5] = st;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < LB_THREADS / 32; ++i) st = merge(st, warp_stat[i]);
+        stats[n * gridDim.x + blockIdx.x] = st;
+    }
+}
+
+// Gradients of a tile: block (tile of LB_THREADS * E classes, chunk of rows).
+// Tile 0 writes the losses and the chunk's part of the temperature's gradient.
+constexpr int LB_ROWS = 128;  // rows of a chunk at most
+
+struct GradRow {
+    float m, f, wt;  // z of the largest class, w / (t s), w / t
+    int y;           // -1: no gradient
+};
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args a, const LossStat *__restrict__ stats,
+                                                             int parts, int chunk, const LossPart part) {
+    constexpr int E = 16 / (int)sizeof(T), U = 4;
+    using C = Classes<T, E, VEC>;
+    __shared__ GradRow rows[LB_ROWS];
+    __shared__ double red_dt[LB_THREADS / 32];
+    cudaGridDependencySynchronize();
+    const int K = a.k, chunks = gridDim.y;
+    const int64_t n0 = (int64_t)blockIdx.y * chunk;
+    const int count = (int)min((int64_t)chunk, a.n - n0);
+    const float rt = loss_rt(a), c = rt * LOG2E;
     double dt = 0.0;
-    int turn = 0;  // changes with every row that is summed
-    if (cluster > 1) cg::this_cluster().sync();  // all blocks are there to be written to
-    for (int64_t n = team; n < a.n; n += teams) {
-        const T *cs = (const T *)a.cs + n * a.cs_stride;
-        T *dcs = (T *)a.dcs + n * (int64_t)K;
-        const LossRow row = loss_row<T>(a, n, c);
-        if (!row.open) {
-            if (a.dcs) {
+    for (int i = threadIdx.x; i < count; i += LB_THREADS) {
+        const int64_t n = n0 + i;
+        const LossLabel label = loss_label(a, n);
+        GradRow r = {0.f, 0.f, 0.f, -1};
+        float loss = label.y >= 0 ? label.w * INFINITY : 0.f;
+        if (label.open) {
+            LossStat st = stats[n * parts];
+            for (int j = 1; j < parts; ++j) st = merge(st, stats[n * parts + j]);
+            r = {st.m, label.w * rt / st.s, label.w * rt, label.y};
+            if (blockIdx.x == 0) {
+                const float gap = loss_z(to_f32(((const T *)a.cs)[n * a.cs_stride + label.y]),
+                                         a.bias ? a.bias[label.y] : 0.f, c) - st.m;
+                loss = label.w * (logf(st.s) - gap * LN2);
+                dt += (double)label.w * (double)(st.h / st.s - gap);
+            }
+        }
+        rows[i] = r;
+        if (blockIdx.x == 0) a.loss[n] = loss;
+    }
+    if (blockIdx.x == 0) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) dt += __shfl_xor_sync(0xFFFFFFFFu, dt, d);
+        if ((threadIdx.x & 31) == 0) red_dt[threadIdx.x >> 5] = dt;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        for (int i = 1; i < LB_THREADS / 32; ++i) dt += red_dt[i];
+        if (chunks > 1) part.dt[blockIdx.y] = dt;
+        else if (a.dtemperature) *a.dtemperature = (float)(-dt * (double)LN2 * (double)rt);
+    }
+    if (!a.dcs && !a.dbias) return;
+    const int k0 = (int)blockIdx.x * LB_THREADS * E + C::first(threadIdx.x);
+    float b[E], acc[E];
+    C::load_bias(a.bias, k0, K, b);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    const uint32_t shared_open = C::open(a.allowed_stride ? nullptr : a.allowed, k0, K);
+    for (int i0 = 0; i0 < count; i0 += U) {
+        T raw[U][E];
+        uint32_t open[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t n = n0 + min(i0 + u, count - 1);
+            C::load((const T *)a.cs + n * a.cs_stride, k0, K, raw[u]);
+            open[u] = shared_open;
+            if (a.allowed_stride) open[u] &= C::open(a.allowed + n * a.allowed_stride, k0, K);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u >= count) break;
+            const GradRow r = rows[i0 + u];
+            float d[E];
+            if (r.y >= 0) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const int k = k0 + e / V * THREADS * V + e % V;
-                    if (k < K) dcs[k] = T(0.f);
+                    d[e] = (open[u] >> e) & 1u ? ex2(loss_z(to_f32(raw[u][e]), b[e], c) - r.m) * r.f : 0.f;
+                    if (k0 + C::at(e) == r.y) d[e] -= r.wt;
+                    acc[e] += d[e];
                 }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) d[e] = 0.f;
             }
-            if (tid == 0 && rank == 0) a.loss[n] = row.use ? row.w * INFINITY : 0.f;
-            continue;  // the same for every block of the cluster
-        }
-        const uint32_t *allowed = a.allowed ? a.allowed + n * a.allowed_stride : nullptr;
-        float z[E];
-        LossStat st = {-INFINITY, 0.f, 0.f};
-        uint32_t open = 0;  // bit e: class e of this thread is there and allowed
-        if (VEC) {
-            uint4 raw[NV];
+            if constexpr (!std::is_integral<T>::value) {
+                if (a.dcs) {
+                    T *dcs = (T *)a.dcs + (n0 + i0 + u) * (int64_t)K;
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int k = k0 + j * THREADS * V;
-                raw[j] = make_uint4(0, 0, 0, 0);
-                if (k + V <= K) {
-                    raw[j] = *(const uint4 *)(cs + k);
-                    open |= ((1u << V) - 1u) << (j * V);
-                } else if (k < K) {
-                    for (int i = 0; i < K - k; ++i) ((T *)&raw[j])[i] = cs[k + i];
-                    open |= ((1u << (K - k)) - 1u) << (j * V);
-                }
-            }
-            if (allowed) {
-                uint32_t bits = 0;
+                    for (int j = 0; j < C::NV; ++j) {
+                        const int k = k0 + C::at(j * C::V);
+                        alignas(16) T out[C::V];
 #pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int k = k0 + j * THREADS * V;
-                    if (k < K) bits |= (allowed[k >> 5] >> (k & 31) & ((1u << V) - 1u)) << (j * V);
-                }
-                open &= bits;
-            }
+                        for (int i = 0; i < C::V; ++i) out[i] = from_f32<T>(d[j * C::V + i]);
+                        if (VEC && k + C::V <= K) *(uint4 *)(dcs + k) = *(const uint4 *)out;
+                        else {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const T *v = (const T *)&raw[j];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const int e = j * V + i;
-                    z[e] = (open >> e) & 1u ? loss_z(to_f32(v[i]), b[e], c) : -INFINITY;
-                    st.m = fmaxf(st.m, z[e]);
-                }
-            }
-        } else {
-            const T *c0 = cs + k0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const bool there = k0 + e * THREADS < K;
-                z[e] = there ? to_f32(c0[e * THREADS]) : 0.f;
-                if (there) open |= 1u << e;
-            }
-            if (allowed) {  // a warp's classes are the bits of one word
-                const uint32_t *w0 = allowed + (k0 >> 5);
-                uint32_t bits = 0;
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (k0 + e * THREADS < K) bits |= (w0[e * (THREADS / 32)] >> (k0 & 31) & 1u) << e;
-                open &= bits;
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                z[e] = (open >> e) & 1u ? loss_z(z[e], b[e], c) : -INFINITY;
-                st.m = fmaxf(st.m, z[e]);
-            }
-        }
-        const float base = st.m == -INFINITY ? 0.f : st.m;  // nothing here: every e is 0
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float x = z[e] - base;
-            z[e] = ex2(x);
-            st.s += z[e];
-            st.h = fmaf(z[e], fmaxf(x, -1024.f), st.h);
-        }
-        const float mine = st.m;
-#pragma unroll
-        for (int d = 16; d; d >>= 1)
-            st = merge(st, {__shfl_xor_sync(0xFFFFFFFFu, st.m, d), __shfl_xor_sync(0xFFFFFFFFu, st.s, d),
-                            __shfl_xor_sync(0xFFFFFFFFu, st.h, d)});
-        if ((tid & 31) == 0) warp_stat[turn][tid >> 5] = st;
-        __syncthreads();
-        st = warp_stat[turn][tid & (WARPS - 1)];
-#pragma unroll
-        for (int d = WARPS / 2; d; d >>= 1)
-            st = merge(st, {__shfl_xor_sync(0xFFFFFFFFu, st.m, d), __shfl_xor_sync(0xFFFFFFFFu, st.s, d),
-                            __shfl_xor_sync(0xFFFFFFFFu, st.h, d)});
-        if (cluster > 1) {
-            // slots of the other turn may still be read by a slower block;
-            // these were last read before the barrier of the turn between
-            cg::cluster_group cl = cg::this_cluster();
-            if (tid < cluster) *cl.map_shared_rank(&block_stat[turn][rank], tid) = st;
-            cl.sync();
-            st = block_stat[turn][0];
-            for (int i = 1; i < cluster; ++i) st = merge(st, block_stat[turn][i]);
-        }
-        const float wt = row.w * rt;
-        const float f = ex2(mine == st.m ? 0.f : mine - st.m) * (wt / st.s);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            z[e] *= f;
-            acc[e] += z[e];
-        }
-        // the label's class: its owner takes w / t off
-        const int o = row.y - k0, oj = o / (THREADS * V), oi = o - oj * THREADS * V;
-        if (o >= 0 && oj < NV && oi < V) {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (e == oj * V + oi) {
-                    z[e] -= wt;
-                    acc[e] -= wt;
-                }
-        }
-        if constexpr (!std::is_integral<T>::value) {
-            if (a.dcs) {
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int k = k0 + j * THREADS * V;
-                    T out[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) out[i] = from_f32<T>(z[j * V + i]);
-                    if (VEC && k + V <= K) *(uint4 *)(dcs + k) = *(const uint4 *)out;
-                    else
-#pragma unroll
-                        for (int i = 0; i < V; ++i)
-                            if (k + i < K) dcs[k + i] = out[i];
+                            for (int i = 0; i < C::V; ++i)
+                                if (k + i < K) dcs[k + i] = out[i];
+                        }
+                    }
                 }
             }
         }
-        if (tid == 0 && rank == 0) {
-            const float gap = row.zy - st.m;
-            a.loss[n] = row.w * (logf(st.s) - gap * LN2);
-            dt += (double)row.w * (double)(st.h / st.s - gap);
-        }
-        turn ^= 1;
     }
-    float *db = teams == 1 ? a.dbias : part.db + (int64_t)team * K;
     if (a.dbias) {
+        float *db = chunks == 1 ? a.dbias : part.db + (int64_t)blockIdx.y * K;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int k = k0 + e / V * THREADS * V + e % V;
-            if (k < K) db[k] = acc[e];
-        }
-    }
-    if (tid == 0 && rank == 0) {
-        if (teams > 1) part.dt[team] = dt;
-        else if (a.dtemperature) *a.dtemperature = (float)(-dt * (double)LN2 * (double)rt);
+        for (int e = 0; e < E; ++e)
+            if (k0 + C::at(e) < K) db[k0 + C::at(e)] = acc[e];
     }
 }
 
@@ -475,57 +539,79 @@ __global__ void __launch_bounds__(1024) k_loss_join(const ytm_loss_args a, const
 
 // ------------------------------------------------------------- launching
 
-// How a call is cut: which kernel, how many teams of how many blocks.
+// How a call is cut: which kernels, and how many teams' parts there are to join.
 struct LossPlan {
     bool big;
-    int threads, e, cluster;  // big
-    int tpr, nv;              // small
-    int64_t teams;            // blocks (small) or clusters (big): parts to join
+    int tpr, nv;               // small
+    int parts, rounds, chunk;  // big: parts of a row, rounds of a part, rows of a chunk
+    int64_t teams;             // blocks (small) or chunks (big)
 };
 
-constexpr int LOSS_CHAIN = 256;  // rows that one team adds up in fp32 at most
+constexpr int LOSS_CHAIN = 256;  // rows that one thread adds up in fp32 at most
 
-static ytm_status loss_plan(int64_t n, int64_t k, LossPlan &p) {
-    p = LossPlan{};
-    const int sms = sm_count();
+static LossPlan loss_plan(int64_t n, int64_t k, int64_t elem) {
+    LossPlan p = {};
+    const int64_t sms = sm_count();
     if (k <= 1024) {
         p.tpr = k <= 16 ? 4 : k <= 128 ? 8 : k <= 256 ? 16 : 32;
         p.nv = k <= 32 ? 1 : k <= 64 ? 2 : k <= 512 ? 4 : 8;
         const int64_t rows = LS_THREADS / p.tpr;
         // up to four rounds of one block cost less than joining blocks
-        p.teams = n <= 4 * rows ? 1 : std::min<int64_t>(cdiv(n, rows), (int64_t)sms * 4);
+        p.teams = n <= 4 * rows ? 1 : std::min<int64_t>(cdiv(n, rows), sms * (p.nv >= 4 ? 2 : 4));
         p.teams = std::max<int64_t>(p.teams, cdiv(n, rows * LOSS_CHAIN));
-        return YTM_OK;
+        return p;
     }
     p.big = true;
-    p.threads = k <= 131072 ? 256 : 512;
-    p.e = k <= 2048 ? 8 : k <= 4096 ? 16 : 32;
-    p.cluster = 1;
-    while ((int64_t)p.cluster * p.threads * p.e < k) p.cluster *= 2;
-    if (p.cluster > 16) return fail(YTM_ERR_UNSUPPORTED, "class loss: more than 262,144 classes");
-    p.teams = std::min<int64_t>(n, std::max<int64_t>(1, (int64_t)sms * big_blocks(p.threads, p.e) / p.cluster));
-    p.teams = std::max<int64_t>(p.teams, cdiv(n, LOSS_CHAIN));
-    return YTM_OK;
+    // parts of a row until every SM has about eight blocks
+    const int64_t rounds = cdiv(k, LB_PART), want = std::max<int64_t>(1, std::min<int64_t>(32, cdiv(sms * 8, n)));
+    p.rounds = (int)cdiv(rounds, std::min(want, rounds));
+    p.parts = (int)cdiv(rounds, p.rounds);
+    // chunks of rows until there are about two rounds of blocks (four an SM)
+    const int64_t tiles = cdiv(k, LB_THREADS * 16 / elem);
+    p.chunk = (int)std::min<int64_t>(LB_ROWS, std::max<int64_t>(4, cdiv(n * tiles, sms * 8)));
+    p.teams = cdiv(n, p.chunk);
+    return p;
 }
 
-template <typename T, int THREADS, int E>
-static ytm_status launch_big(const ytm_loss_args &a, const LossPlan &p, const LossPart &part, bool vec, cudaStream_t st) {
+// A launch that may start while the kernel before it ends (it waits for that
+// kernel's results itself).
+template <typename... P, typename... A>
+static ytm_status launch_after(void (*f)(P...), dim3 grid, unsigned block, cudaStream_t st, const char *what, A... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.teams * p.cluster));
-    cfg.blockDim = dim3(THREADS);
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)p.cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-    auto *f = vec ? k_loss_big<T, THREADS, E, true> : k_loss_big<T, THREADS, E, false>;
-    ytm_status rc;
-    if (p.cluster > 8 && (rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
-                                          "class loss cluster")))
-        return rc;
-    return cuda_check(cudaLaunchKernelEx(&cfg, f, a, part, p.cluster), "class loss");
+    cfg.numAttrs = 1;
+    return cuda_check(cudaLaunchKernelEx(&cfg, f, P(args)...), what);
+}
+
+// Workspace: dt parts, dbias parts, row statistics.
+struct LossWs {
+    uint64_t db, stats, total;
+};
+
+static LossWs loss_ws(const LossPlan &p, int64_t n, int64_t k) {
+    LossWs w;
+    const bool join = p.teams > 1;
+    w.db = join ? align_up((uint64_t)p.teams * 8, 256) : 0;
+    w.stats = w.db + (join ? align_up((uint64_t)p.teams * k * 4, 256) : 0);
+    w.total = w.stats + (p.big ? (uint64_t)n * p.parts * sizeof(LossStat) : 0);
+    return w;
+}
+
+template <typename T, bool VEC>
+static ytm_status launch_big(const ytm_loss_args &a, const LossPlan &p, const LossPart &part, LossStat *stats, cudaStream_t st) {
+    const unsigned gz = (unsigned)cdiv(a.n, 65535), gy = (unsigned)cdiv(a.n, gz);
+    k_loss_stat<T, VEC><<<dim3(p.parts, gy, gz), LB_THREADS, 0, st>>>(a, stats, p.rounds);
+    ytm_status rc = launch_check("class loss statistics");
+    if (rc) return rc;
+    const unsigned tiles = a.dcs || a.dbias ? (unsigned)cdiv(a.k, LB_THREADS * 16 / sizeof(T)) : 1;
+    return launch_after(k_loss_grad<T, VEC>, dim3(tiles, (unsigned)p.teams), LB_THREADS, st, "class loss", a, stats, p.parts,
+                        p.chunk, part);
 }
 
 template <typename T, int TPR, int NV>
@@ -537,17 +623,13 @@ static ytm_status launch_small(const ytm_loss_args &a, const LossPlan &p, const 
 }
 
 template <typename T>
-static ytm_status launch_loss(const ytm_loss_args &a, const LossPlan &p, const LossPart &part, cudaStream_t st) {
-    // vectors: 16 bytes in the big kernel, four classes in the small one
+static ytm_status launch_loss(const ytm_loss_args &a, const LossPlan &p, const LossPart &part, LossStat *stats, cudaStream_t st) {
+    // vectors: 16 bytes of long rows, four classes of short ones
     const uint64_t step = p.big ? 16 : 4 * sizeof(T);
     const bool vec = (uintptr_t)a.cs % step == 0 && a.cs_stride * sizeof(T) % step == 0 &&
-                     (!a.dcs || ((uintptr_t)a.dcs % step == 0 && (uint64_t)a.k * sizeof(T) % step == 0));
-    if (p.big) {
-        if (p.threads == 512) return launch_big<T, 512, 32>(a, p, part, vec, st);
-        if (p.e == 8) return launch_big<T, 256, 8>(a, p, part, vec, st);
-        if (p.e == 16) return launch_big<T, 256, 16>(a, p, part, vec, st);
-        return launch_big<T, 256, 32>(a, p, part, vec, st);
-    }
+                     (!a.dcs || ((uintptr_t)a.dcs % step == 0 && (uint64_t)a.k * sizeof(T) % step == 0)) &&
+                     (!p.big || (uintptr_t)a.bias % 16 == 0);
+    if (p.big) return vec ? launch_big<T, true>(a, p, part, stats, st) : launch_big<T, false>(a, p, part, stats, st);
     if (p.tpr == 4) return launch_small<T, 4, 1>(a, p, part, vec, st);
     if (p.tpr == 8 && p.nv == 1) return launch_small<T, 8, 1>(a, p, part, vec, st);
     if (p.tpr == 8 && p.nv == 2) return launch_small<T, 8, 2>(a, p, part, vec, st);
@@ -563,10 +645,9 @@ using namespace ytm;
 
 extern "C" {
 
-uint64_t ytm_class_loss_workspace_bytes(int64_t n, int32_t k) {
-    LossPlan p;
-    if (n <= 0 || k <= 0 || loss_plan(n, k, p) || p.teams == 1) return 0;
-    return align_up((uint64_t)p.teams * 8, 256) + (uint64_t)p.teams * k * 4;
+uint64_t ytm_class_loss_workspace_bytes(int64_t n, int32_t k, int32_t cs_type) {
+    if (n <= 0 || k <= 0 || !is_sum_type(cs_type)) return 0;
+    return loss_ws(loss_plan(n, k, type_bytes(cs_type)), n, k).total;
 }
 
 ytm_status ytm_class_loss(const ytm_loss_args *args, void *workspace, void *stream) {
@@ -584,28 +665,21 @@ ytm_status ytm_class_loss(const ytm_loss_args *args, void *workspace, void *stre
         if (a.dtemperature && (rc = cuda_check(cudaMemsetAsync(a.dtemperature, 0, 4, st), "memset"))) return rc;
         return YTM_OK;
     }
-    LossPlan p;
-    if ((rc = loss_plan(a.n, a.k, p))) return rc;
-    if (!a.cs || !a.target || !a.loss || (p.teams > 1 && !workspace)) return fail(YTM_ERR_ARG, "null pointer");
-    LossPart part = {nullptr, nullptr};
-    if (p.teams > 1) part = {(float *)((char *)workspace + align_up((uint64_t)p.teams * 8, 256)), (double *)workspace};
+    const LossPlan p = loss_plan(a.n, a.k, type_bytes(a.cs_type));
+    const LossWs ws = loss_ws(p, a.n, a.k);
+    if (p.teams > (p.big ? 65535 : INT_MAX)) return fail(YTM_ERR_UNSUPPORTED, "class loss: too many rows for one call");
+    if (!a.cs || !a.target || !a.loss || (ws.total && !workspace)) return fail(YTM_ERR_ARG, "null pointer");
+    const LossPart part = {(float *)((char *)workspace + ws.db), (double *)workspace};
+    LossStat *stats = (LossStat *)((char *)workspace + ws.stats);
     switch (a.cs_type) {
-        case YTM_I32: rc = launch_loss<int32_t>(a, p, part, st); break;
-        case YTM_F32: rc = launch_loss<float>(a, p, part, st); break;
-        case YTM_F16: rc = launch_loss<__half>(a, p, part, st); break;
-        default: rc = launch_loss<__nv_bfloat16>(a, p, part, st); break;
+        case YTM_I32: rc = launch_loss<int32_t>(a, p, part, stats, st); break;
+        case YTM_F32: rc = launch_loss<float>(a, p, part, stats, st); break;
+        case YTM_F16: rc = launch_loss<__half>(a, p, part, stats, st); break;
+        default: rc = launch_loss<__nv_bfloat16>(a, p, part, stats, st); break;
     }
     if (rc || p.teams == 1 || (!a.dbias && !a.dtemperature)) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.dbias ? cdiv(a.k, 32) : 0) + 1);
-    cfg.blockDim = dim3(1024);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cuda_check(cudaLaunchKernelEx(&cfg, k_loss_join, a, part, (int)p.teams), "class loss sums");
+    return launch_after(k_loss_join, dim3((unsigned)(a.dbias ? cdiv(a.k, 32) : 0) + 1), 1024, st, "class loss sums", a, part,
+                        (int)p.teams);
 }
 
 }  // extern "C"
