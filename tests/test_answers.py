@@ -61,11 +61,11 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
                dict(cs_stride=-1), dict(allowed_stride=-1)):
         assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, **kw})), one, None) == 1, kw
     assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "n": 100000})), None, None) == 1
-    assert lib.ytm_class_loss_workspace_bytes(100000, 4, 1) > 0
+    assert lib.ytm_class_loss_workspace_bytes(100000, 4, 1, 4) > 0
     assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "k": 5000, "n": 1 << 27})), one, None) == 3
     assert lib.ytm_class_loss(None, one, None) == 1
     assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "n": 0})), None, None) == 0
-    assert lib.ytm_class_loss_workspace_bytes(-1, 4, 1) == 0
+    assert lib.ytm_class_loss_workspace_bytes(-1, 4, 1, 4) == 0
     cfg = _lib.make_config(clauses_per_class=8, T=5, s=3.0, dim=(16, 1, 1), n_classes=2)
     assert lib.ytm_infer_fired(ct.byref(cfg), None, None, 4, None, None, None) == 1
     assert lib.ytm_infer_fired(ct.byref(cfg), None, None, 0, None, None, None) == 0

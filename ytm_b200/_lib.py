@@ -127,7 +127,7 @@ _SIGS = {
     "ytm_infer_fired": ([_CFG, _P, _P, _I64, _P, _P, _P], ct.c_int),
     "ytm_answer": ([ct.POINTER(AnswerArgs), _P], ct.c_int),
     "ytm_class_loss": ([ct.POINTER(LossArgs), _P, _P], ct.c_int),
-    "ytm_class_loss_workspace_bytes": ([_I64, _I32, _I32], _U64),
+    "ytm_class_loss_workspace_bytes": ([_I64, _I32, _I32, _I64], _U64),
     "ytm_last_error": ([], ct.c_char_p),
     "ytm_version": ([], ct.c_char_p),
     "ytm_config_size": ([], ct.c_int32),

@@ -290,7 +290,7 @@ def class_loss(cs: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None
     dcs = None if cs.dtype == torch.int32 else torch.empty((n, k), dtype=cs.dtype, device=dev)
     dbias = None if bias is None else torch.empty(k, dtype=torch.float32, device=dev)
     dtem = torch.empty(1, dtype=torch.float32, device=dev)
-    need = lib.ytm_class_loss_workspace_bytes(n, k, _TYPES[cs.dtype])
+    need = lib.ytm_class_loss_workspace_bytes(n, k, _TYPES[cs.dtype], _row_stride(cs))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     args = LossArgs(cs.data_ptr(), _row_stride(cs), n, k, _TYPES[cs.dtype], None if bias is None else bias.data_ptr(),
                     allowed_p, allowed_stride, target.data_ptr(), None if weight is None else weight.data_ptr(), tem_p,

@@ -8,7 +8,7 @@
 //   dt = -(ln 2 / t) sum_n w (h / s - (z_y - m))
 // so that h gives the temperature's gradient without another look at z.
 //
-// Rows of up to 1024 classes stay in the registers of 4 to 32 threads between
+// Rows of up to 512 classes stay in the registers of 4 to 32 threads between
 // the sum and the gradient (k_loss_small).  Longer rows take two streams over
 // the class sums, which need no barrier: k_loss_stat for (m, s, h), then
 // k_loss_grad, whose threads keep their classes over a chunk of rows.  Both
@@ -32,9 +32,9 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// One rounding for each operation: a product fused into z - m would leave the
-// largest class's exponent off 0.
-__device__ __forceinline__ float loss_z(float v, float b, float c) { return __fmul_rn(__fadd_rn(v, b), c); }
+// z, with bc = b c; the same operations for every use of a class's z, so that
+// the largest class's exponent is 0 exactly.
+__device__ __forceinline__ float loss_z(float v, float bc, float c) { return __fmaf_rn(v, c, bc); }
 
 // A row's label, weight and label's mask bit.  y < 0: the row counts for
 // nothing; open: it has a gradient.
@@ -110,20 +110,15 @@ __global__ void __launch_bounds__(LS_THREADS, NV >= 4 ? 2 : NV == 2 ? 3 : 4) k_l
     __shared__ double red_dt[LS_THREADS / 32];
     const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR, K = a.k;
     const float rt = loss_rt(a), c = rt * LOG2E;
-    // the bias stays in registers while there is room for it
-    constexpr bool KEEP = NV < 8;
-    const auto bias_of = [&](int j, int i) {
-        const int k = small_class<TPR, NV, VEC>(lane, j, i);
-        return a.bias && k < K ? a.bias[k] : 0.f;
-    };
-    float b[KEEP ? NV : 1][4], acc[NV][4];
+    float b[NV][4], acc[NV][4];
     uint32_t shared_open = 0;  // bit 4 j + i
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         shared_open |= small_open<TPR, NV, VEC>(a.allowed_stride ? nullptr : a.allowed, lane, j, K) << (4 * j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (KEEP) b[KEEP ? j : 0][i] = bias_of(j, i);
+            const int k = small_class<TPR, NV, VEC>(lane, j, i);
+            b[j][i] = a.bias && k < K ? __fmul_rn(a.bias[k], c) : 0.f;
             acc[j][i] = 0.f;
         }
     }
@@ -168,7 +163,7 @@ __global__ void __launch_bounds__(LS_THREADS, NV >= 4 ? 2 : NV == 2 ? 3 : 4) k_l
         }
         const int y = max(label.y, 0);
         r.vy = cs[y];
-        r.by = a.bias ? a.bias[y] : 0.f;
+        r.by = a.bias ? __fmul_rn(a.bias[y], c) : 0.f;
         return r;
     };
     double dt = 0.0;
@@ -190,7 +185,7 @@ __global__ void __launch_bounds__(LS_THREADS, NV >= 4 ? 2 : NV == 2 ? 3 : 4) k_l
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 z[j][i] = (row.open >> (4 * j + i)) & 1u
-                              ? loss_z(to_f32(row.v[j].v[i]), KEEP ? b[KEEP ? j : 0][i] : bias_of(j, i), c)
+                              ? loss_z(to_f32(row.v[j].v[i]), b[j][i], c)
                               : -INFINITY;
                 m = fmaxf(m, z[j][i]);
             }
@@ -292,92 +287,208 @@ __device__ __forceinline__ LossStat merge(const LossStat &a, const LossStat &b) 
 }
 
 constexpr int LB_THREADS = 256;
-constexpr int LB_PART = LB_THREADS * 16;  // classes that a block of k_loss_stat takes in one round
 
-// E classes of a row from k0 on, as z (-inf where closed or behind the row):
-// vectors of 16 bytes THREADS apart (VEC: rows, bias and gradients on 16-byte
-// boundaries), else single classes THREADS apart, so that a warp's loads are
-// neighbours and its mask bits those of one word.
-template <typename T, int E, bool VEC>
-struct Classes {
-    static constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, NV = E / V;
-    __device__ static __forceinline__ int first(int tid) { return tid * V; }
-    __device__ static __forceinline__ int at(int e) { return e / V * LB_THREADS * V + e % V; }
+// A row of class sums (or gradients) in 16-byte vectors from the 16-byte
+// boundary at or below its start: class k is element off + k of them.
+template <typename T>
+struct RowVecs {
+    static constexpr int V = 16 / (int)sizeof(T);
+    const T *row;
+    int off;
 
-    __device__ static __forceinline__ void load_bias(const float *bias, int k0, int K, float (&b)[E]) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int k = k0 + at(j * V);
-            if (VEC && bias && k + V <= K) {
-#pragma unroll
-                for (int i = 0; i < V / 4; ++i) *(float4 *)&b[j * V + 4 * i] = *(const float4 *)(bias + k + 4 * i);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) b[j * V + i] = bias && k + i < K ? bias[k + i] : 0.f;
-            }
-        }
+    __device__ __forceinline__ RowVecs(const void *base, int64_t row_index, int64_t stride)
+        : row((const T *)base + row_index * stride), off((int)((uintptr_t)row % 16 / sizeof(T))) {}
+
+    // Vectors first .. last lie inside the row, so that they can be moved whole.
+    __device__ __forceinline__ bool inside(int first, int last, int K) const {
+        return (first > 0 || (first == 0 && off == 0)) && (int64_t)(last + 1) * V <= (int64_t)off + K;
     }
 
-    __device__ static __forceinline__ void load(const T *cs, int k0, int K, T (&raw)[E]) {
+    __device__ __forceinline__ uint4 load_whole(int i) const { return *(const uint4 *)(row - off + (int64_t)i * V); }
+    __device__ __forceinline__ void store_whole(int i, uint4 v) const { *(uint4 *)(row - off + (int64_t)i * V) = v; }
+
+    __device__ __forceinline__ uint4 load(int i, int K) const {
+        if (inside(i, i, K)) return load_whole(i);
+        if ((int64_t)i * V >= (int64_t)off + K) return make_uint4(0, 0, 0, 0);
+        alignas(16) T t[V];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int k = k0 + at(j * V);
-            if (VEC && k + V <= K) *(uint4 *)&raw[j * V] = *(const uint4 *)(cs + k);
-            else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) raw[j * V + i] = k + i < K ? cs[k + i] : T(0.f);
-            }
+        for (int j = 0; j < V; ++j) {
+            const int64_t k = (int64_t)i * V + j - off;
+            t[j] = k >= 0 && k < K ? row[k] : T(0.f);
         }
+        return *(const uint4 *)t;
     }
 
-    // Bit e: class e is there and allowed.
-    __device__ static __forceinline__ uint32_t open(const uint32_t *allowed, int k0, int K) {
-        uint32_t o = 0;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int k = k0 + at(j * V);
-            if (k < K) o |= ((allowed ? allowed[k >> 5] >> (k & 31) : ~0u) & (k + V <= K ? (1u << V) - 1u : (1u << (K - k)) - 1u)) << (j * V);
+    __device__ __forceinline__ void store(int i, int K, uint4 v) const {
+        if (inside(i, i, K)) {
+            store_whole(i, v);
+            return;
         }
-        return o;
+        if ((int64_t)i * V >= (int64_t)off + K) return;
+        const T *t = (const T *)&v;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int64_t k = (int64_t)i * V + j - off;
+            if (k >= 0 && k < K) const_cast<T *>(row)[k] = t[j];
+        }
     }
 };
 
-// (m, s, h) of `rounds` rounds of LB_PART classes of one row: block (part, row).
-template <typename T, bool VEC>
+// Two fp32 operations in one instruction, on register pairs.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair(float x, float y) {
+    F2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ void split(F2 a, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// Classes 2 q and 2 q + 1 of a vector.
+template <typename T>
+__device__ __forceinline__ F2 class_pair(const uint4 &raw, int q) {
+    const T *v = (const T *)&raw;
+    return pair(to_f32(v[2 * q]), to_f32(v[2 * q + 1]));
+}
+
+// Bits j: class k + j (of V) is there and allowed.
+template <int V, bool INSIDE>
+__device__ __forceinline__ uint32_t open_classes(const uint32_t *allowed, int k, int K) {
+    constexpr uint32_t ALL = (1u << V) - 1u;
+    uint32_t there = ALL;
+    if (!INSIDE) {
+        if (k >= K || k <= -V) return 0u;
+        if (k + V > K) there = (1u << (K - k)) - 1u;
+        if (k < 0) there &= ALL << -k;
+    }
+    if (!allowed) return there;
+    const int w = k >> 5;  // of a k below 0: the word before the first
+    const uint32_t lo = INSIDE || w >= 0 ? allowed[w] : 0u;
+    const uint32_t hi = (k & 31) + V > 32 && (INSIDE || (w + 1) * 32 < K) ? allowed[w + 1] : 0u;
+    return __funnelshift_r(lo, hi, k & 31) & there;
+}
+
+// bias[k .. k + V) (0 where there is none), k = R below a multiple of four.
+template <int V, int R, bool INSIDE>
+__device__ __forceinline__ void load_bias(const float *bias, int k, int K, F2 (&b)[V / 2]) {
+    if (!bias) {
+#pragma unroll
+        for (int q = 0; q < V / 2; ++q) b[q] = pair(0.f, 0.f);
+    } else if (INSIDE && (uintptr_t)bias % 16 == 0) {
+        float f[V + 4];  // from the boundary at or below k
+        const float *from = bias + (R ? k + R - 4 : k);
+#pragma unroll
+        for (int q = 0; q < (R ? V / 4 + 1 : V / 4); ++q) *(float4 *)&f[4 * q] = *(const float4 *)(from + 4 * q);
+#pragma unroll
+        for (int q = 0; q < V / 2; ++q) b[q] = pair(f[(R ? 4 - R : 0) + 2 * q], f[(R ? 4 - R : 0) + 2 * q + 1]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < V / 2; ++q)
+            b[q] = pair(k + 2 * q >= 0 && k + 2 * q < K ? bias[k + 2 * q] : 0.f,
+                        k + 2 * q + 1 >= 0 && k + 2 * q + 1 < K ? bias[k + 2 * q + 1] : 0.f);
+    }
+}
+
+// (m, s, h) of `rounds` rounds of NVS * LB_THREADS vectors of one row: block
+// (part, row).
+template <typename T, int NVS>
 __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args a, LossStat *__restrict__ stats, int rounds) {
-    using C = Classes<T, 16, VEC>;
+    constexpr int V = RowVecs<T>::V, STEP = NVS * LB_THREADS;
     __shared__ LossStat warp_stat[LB_THREADS / 32];
     const int K = a.k;
     const int64_t n = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
     if (n >= a.n) return;
     const float c = loss_rt(a) * LOG2E;
-    const T *cs = (const T *)a.cs + n * a.cs_stride;
+    const F2 c2 = pair(c, c);
+    const RowVecs<T> row(a.cs, n, a.cs_stride);
     const uint32_t *allowed = a.allowed ? a.allowed + n * a.allowed_stride : nullptr;
     LossStat st = {-INFINITY, 0.f, 0.f};
-    int k0 = (int)blockIdx.x * rounds * LB_PART + C::first(threadIdx.x);
-    const int end = min(K, (int)min((int64_t)K, (int64_t)(blockIdx.x + 1) * rounds * LB_PART));
-    for (; k0 < end; k0 += LB_PART) {
-        T raw[16];
-        float b[16], z[16], m = st.m;
-        C::load(cs, k0, K, raw);
-        C::load_bias(a.bias, k0, K, b);
-        const uint32_t open = C::open(allowed, k0, K);
+    const auto round = [&](int i0, auto below, auto count, auto inside) {
+        constexpr int R = decltype(below)::value, NV = decltype(count)::value;
+        constexpr bool INSIDE = decltype(inside)::value;
+        uint4 raw[NV];
+        uint32_t open[NV];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            z[e] = (open >> e) & 1u ? loss_z(to_f32(raw[e]), b[e], c) : -INFINITY;
-            m = fmaxf(m, z[e]);
+        for (int j = 0; j < NV; ++j) {
+            const int i = i0 + j * LB_THREADS + (int)threadIdx.x;
+            raw[j] = INSIDE ? row.load_whole(i) : row.load(i, K);
+            open[j] = open_classes<V, INSIDE>(allowed, i * V - row.off, K);
         }
-        const float base = m == -INFINITY ? 0.f : m;  // nothing yet: every e is 0
+        float z[NV][V], m = st.m;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            F2 b[V / 2];
+            load_bias<V, R, INSIDE>(a.bias, (i0 + j * LB_THREADS + (int)threadIdx.x) * V - row.off, K, b);
+#pragma unroll
+            for (int q = 0; q < V / 2; ++q) {
+                float x, y;
+                split(fma2(class_pair<T>(raw[j], q), c2, mul2(b[q], c2)), x, y);
+                z[j][2 * q] = open[j] & (1u << (2 * q)) ? x : -INFINITY;
+                z[j][2 * q + 1] = open[j] & (2u << (2 * q)) ? y : -INFINITY;
+                m = fmaxf(m, fmaxf(z[j][2 * q], z[j][2 * q + 1]));
+            }
+        }
+        const float base = m == -INFINITY ? 0.f : -m;  // nothing yet: every e is 0
         const float d = st.m == m ? 0.f : st.m - m, f = ex2(d);
-        st.h = f * fmaf(st.s, fmaxf(d, -1024.f), st.h);
-        st.s *= f;
+        F2 s = pair(f * st.s, 0.f), h = pair(f * fmaf(st.s, fmaxf(d, -1024.f), st.h), 0.f);
+        const F2 base2 = pair(base, base);
         st.m = m;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float x = z[e] - base, p = ex2(x);
-            st.s += p;
-            st.h = fmaf(p, fmaxf(x, -1024.f), st.h);  // 0 * -inf counts for nothing
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int q = 0; q < V / 2; ++q) {
+                float x, y;
+                split(add2(pair(z[j][2 * q], z[j][2 * q + 1]), base2), x, y);
+                const F2 e = pair(ex2(x), ex2(y));
+                s = add2(s, e);
+                h = fma2(e, pair(fmaxf(x, -1024.f), fmaxf(y, -1024.f)), h);  // 0 * -inf counts for nothing
+            }
+        float x, y;
+        split(s, x, y);
+        st.s = x + y;
+        split(h, x, y);
+        st.h = x + y;
+    };
+    const int vecs = (int)(((int64_t)row.off + K + V - 1) / V);
+    const int64_t first = (int64_t)blockIdx.x * rounds * STEP;
+    const int end = (int)min((int64_t)vecs, first + (int64_t)rounds * STEP);
+    const int warp_vec = threadIdx.x & ~31;
+    // a warp's vectors from i0 on, LB_THREADS apart, lie inside the row (and the
+    // bias up to the next boundary, to which it is read)
+    const auto warp_inside = [&](int i0, int count, int below) {
+        const int last = i0 + (count - 1) * LB_THREADS + warp_vec + 31;
+        return row.inside(i0 + warp_vec, last, K) && (int64_t)(last + 1) * V - row.off + below <= K;
+    };
+    const auto stream = [&](auto below) {
+        int i0 = (int)first;
+        for (; i0 + STEP <= end; i0 += STEP) {
+            if (warp_inside(i0, NVS, below)) round(i0, below, std::integral_constant<int, NVS>(), std::true_type());
+            else round(i0, below, std::integral_constant<int, NVS>(), std::false_type());
         }
+        for (; i0 + warp_vec < end; i0 += LB_THREADS) {
+            if (warp_inside(i0, 1, below)) round(i0, below, std::integral_constant<int, 1>(), std::true_type());
+            else round(i0, below, std::integral_constant<int, 1>(), std::false_type());
+        }
+    };
+    switch (row.off & 3) {  // where the bias lies against the vectors: the same for the block
+        case 0: stream(std::integral_constant<int, 0>()); break;
+        case 1: stream(std::integral_constant<int, 1>()); break;
+        case 2: stream(std::integral_constant<int, 2>()); break;
+        default: stream(std::integral_constant<int, 3>()); break;
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1)
@@ -385,14 +496,21 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
                         __shfl_xor_sync(0xFFFFFFFFu, st.h, d)});
     if ((threadIdx.x & 31) == 0) warp_stat[threadIdx.x >> 5] = st;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < LB_THREADS / 32; ++i) st = merge(st, warp_stat[i]);
-        stats[n * gridDim.x + blockIdx.x] = st;
-    }
+    if (threadIdx.x >= 32) return;
+    st = warp_stat[threadIdx.x % (LB_THREADS / 32)];
+#pragma unroll
+    for (int d = LB_THREADS / 64; d; d >>= 1)
+        st = merge(st, {__shfl_xor_sync(0xFFFFFFFFu, st.m, d), __shfl_xor_sync(0xFFFFFFFFu, st.s, d),
+                        __shfl_xor_sync(0xFFFFFFFFu, st.h, d)});
+    if (threadIdx.x == 0) stats[n * gridDim.x + blockIdx.x] = st;
 }
 
-// Gradients of a tile: block (tile of LB_THREADS * E classes, chunk of rows).
-// Tile 0 writes the losses and the chunk's part of the temperature's gradient.
+// Gradients of a tile: block (tile, chunk of rows), a vector of memory a
+// thread.  Where rows start off a 16-byte boundary, that vector holds other
+// classes from row to row, with a period of 2, 4 or 8 rows: a chunk takes every
+// `period`-th row only, so that its threads keep their classes, and loads,
+// stores and sums of dbias need no shift.  Tile 0 writes the losses and the
+// chunk's part of the temperature's gradient.
 constexpr int LB_ROWS = 128;  // rows of a chunk at most
 
 struct GradRow {
@@ -400,21 +518,20 @@ struct GradRow {
     int y;           // -1: no gradient
 };
 
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args a, const LossStat *__restrict__ stats,
-                                                             int parts, int chunk, const LossPart part) {
-    constexpr int E = 16 / (int)sizeof(T), U = 4;
-    using C = Classes<T, E, VEC>;
+                                                             int parts, int chunk, int period, const LossPart part) {
+    constexpr int V = RowVecs<T>::V, U = 4;
     __shared__ GradRow rows[LB_ROWS];
     __shared__ double red_dt[LB_THREADS / 32];
     cudaGridDependencySynchronize();
-    const int K = a.k, chunks = gridDim.y;
-    const int64_t n0 = (int64_t)blockIdx.y * chunk;
-    const int count = (int)min((int64_t)chunk, a.n - n0);
+    const int K = a.k, chunks = gridDim.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t n0 = blockIdx.y % period + (int64_t)(blockIdx.y / period) * chunk * period;  // the chunk's rows: n0 + i * period
+    const int count = n0 < a.n ? (int)min((int64_t)chunk, (a.n - n0 + period - 1) / period) : 0;
     const float rt = loss_rt(a), c = rt * LOG2E;
     double dt = 0.0;
     for (int i = threadIdx.x; i < count; i += LB_THREADS) {
-        const int64_t n = n0 + i;
+        const int64_t n = n0 + (int64_t)i * period;
         const LossLabel label = loss_label(a, n);
         GradRow r = {0.f, 0.f, 0.f, -1};
         float loss = label.y >= 0 ? label.w * INFINITY : 0.f;
@@ -424,7 +541,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
             r = {st.m, label.w * rt / st.s, label.w * rt, label.y};
             if (blockIdx.x == 0) {
                 const float gap = loss_z(to_f32(((const T *)a.cs)[n * a.cs_stride + label.y]),
-                                         a.bias ? a.bias[label.y] : 0.f, c) - st.m;
+                                         a.bias ? __fmul_rn(a.bias[label.y], c) : 0.f, c) - st.m;
                 loss = label.w * (logf(st.s) - gap * LN2);
                 dt += (double)label.w * (double)(st.h / st.s - gap);
             }
@@ -435,7 +552,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
     if (blockIdx.x == 0) {
 #pragma unroll
         for (int d = 16; d; d >>= 1) dt += __shfl_xor_sync(0xFFFFFFFFu, dt, d);
-        if ((threadIdx.x & 31) == 0) red_dt[threadIdx.x >> 5] = dt;
+        if (lane == 0) red_dt[warp] = dt;
     }
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -444,63 +561,106 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
         else if (a.dtemperature) *a.dtemperature = (float)(-dt * (double)LN2 * (double)rt);
     }
     if (!a.dcs && !a.dbias) return;
-    const int k0 = (int)blockIdx.x * LB_THREADS * E + C::first(threadIdx.x);
-    float b[E], acc[E];
-    C::load_bias(a.bias, k0, K, b);
+    const int64_t row0 = min(n0, a.n - 1);
+    const RowVecs<T> in0(a.cs, row0, a.cs_stride), out0(a.dcs ? a.dcs : a.cs, row0, a.dcs ? K : a.cs_stride);
+    const bool same = in0.off == out0.off;  // else the vectors are those of the gradients
+    const int vec = (int)(blockIdx.x * LB_THREADS + threadIdx.x);
+    const int k0 = vec * V - out0.off, warp_k = k0 - lane * V;
+    const F2 c2 = pair(c, c);
+    F2 bc[V / 2], acc[V / 2];
+    load_bias<V, 0, false>(a.bias, k0, K, bc);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    const uint32_t shared_open = C::open(a.allowed_stride ? nullptr : a.allowed, k0, K);
-    for (int i0 = 0; i0 < count; i0 += U) {
-        T raw[U][E];
-        uint32_t open[U];
+    for (int q = 0; q < V / 2; ++q) {
+        bc[q] = mul2(bc[q], c2);
+        acc[q] = pair(0.f, 0.f);
+    }
+    const uint32_t shared_open = open_classes<V, false>(a.allowed_stride ? nullptr : a.allowed, k0, K);
+    const int64_t in_step = (int64_t)period * a.cs_stride, out_step = (int64_t)period * K;
+    const uint32_t *mask_word = a.allowed_stride ? a.allowed + row0 * a.allowed_stride + (k0 >> 5) : nullptr;
+    const int64_t mask_step = (int64_t)period * a.allowed_stride;
+    const bool straddle = (k0 & 31) + V > 32;
+    const auto stream = [&](auto inside) {
+        constexpr bool INSIDE = decltype(inside)::value;
+        RowVecs<T> in = in0;
+        [[maybe_unused]] RowVecs<T> out = out0;
+        const uint32_t *mask = mask_word;
+        for (int i0 = 0; i0 < count; i0 += U) {
+            uint4 raw[U];
+            uint32_t open[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t n = n0 + min(i0 + u, count - 1);
-            C::load((const T *)a.cs + n * a.cs_stride, k0, K, raw[u]);
-            open[u] = shared_open;
-            if (a.allowed_stride) open[u] &= C::open(a.allowed + n * a.allowed_stride, k0, K);
-        }
+            for (int u = 0; u < U; ++u) {
+                raw[u] = make_uint4(0, 0, 0, 0);
+                open[u] = shared_open;
+                if (i0 + u < count) {
+                    if (INSIDE) {
+                        raw[u] = in.load_whole(vec);
+                        if (a.allowed_stride) open[u] = __funnelshift_r(mask[0], straddle ? mask[1] : 0u, k0 & 31);
+                    } else {
+                        if (same) {
+                            raw[u] = in.load(vec, K);
+                        } else {
+                            T *t = (T *)&raw[u];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i0 + u >= count) break;
-            const GradRow r = rows[i0 + u];
-            float d[E];
-            if (r.y >= 0) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    d[e] = (open[u] >> e) & 1u ? ex2(loss_z(to_f32(raw[u][e]), b[e], c) - r.m) * r.f : 0.f;
-                    if (k0 + C::at(e) == r.y) d[e] -= r.wt;
-                    acc[e] += d[e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) d[e] = 0.f;
-            }
-            if constexpr (!std::is_integral<T>::value) {
-                if (a.dcs) {
-                    T *dcs = (T *)a.dcs + (n0 + i0 + u) * (int64_t)K;
-#pragma unroll
-                    for (int j = 0; j < C::NV; ++j) {
-                        const int k = k0 + C::at(j * C::V);
-                        alignas(16) T out[C::V];
-#pragma unroll
-                        for (int i = 0; i < C::V; ++i) out[i] = from_f32<T>(d[j * C::V + i]);
-                        if (VEC && k + C::V <= K) *(uint4 *)(dcs + k) = *(const uint4 *)out;
-                        else {
-#pragma unroll
-                            for (int i = 0; i < C::V; ++i)
-                                if (k + i < K) dcs[k + i] = out[i];
+                            for (int j = 0; j < V; ++j) t[j] = k0 + j >= 0 && k0 + j < K ? in.row[k0 + j] : T(0.f);
                         }
+                        if (a.allowed_stride) open[u] = open_classes<V, false>(mask - (k0 >> 5), k0, K);
+                    }
+                }
+                in.row += in_step;
+                mask += mask_step;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i0 + u >= count) break;
+                const GradRow r = rows[i0 + u];
+                float d[V];
+                if (r.y >= 0) {
+                    const F2 m2 = pair(-r.m, -r.m), f2 = pair(r.f, r.f);
+#pragma unroll
+                    for (int q = 0; q < V / 2; ++q) {
+                        float x, y;
+                        split(add2(fma2(class_pair<T>(raw[u], q), c2, bc[q]), m2), x, y);
+                        x = open[u] & (1u << (2 * q)) ? ex2(x) : 0.f;
+                        y = open[u] & (2u << (2 * q)) ? ex2(y) : 0.f;
+                        split(mul2(pair(x, y), f2), d[2 * q], d[2 * q + 1]);
+                    }
+                    if (r.y >= warp_k && r.y - warp_k < 32 * V) {  // the label's class is this warp's
+#pragma unroll
+                        for (int j = 0; j < V; ++j)
+                            if (r.y - k0 == j) d[j] -= r.wt;
+                    }
+#pragma unroll
+                    for (int q = 0; q < V / 2; ++q) acc[q] = add2(acc[q], pair(d[2 * q], d[2 * q + 1]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) d[j] = 0.f;
+                }
+                if constexpr (!std::is_integral<T>::value) {
+                    if (a.dcs) {
+                        alignas(16) T t[V];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) t[j] = from_f32<T>(d[j]);
+                        const uint4 w = *(const uint4 *)t;
+                        if (INSIDE) out.store_whole(vec, w);
+                        else out.store(vec, K, w);
+                        out.row += out_step;
                     }
                 }
             }
         }
-    }
+    };
+    if (same && out0.inside(vec - lane, vec - lane + 31, K)) stream(std::true_type());
+    else stream(std::false_type());
     if (a.dbias) {
         float *db = chunks == 1 ? a.dbias : part.db + (int64_t)blockIdx.y * K;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (k0 + C::at(e) < K) db[k0 + C::at(e)] = acc[e];
+        for (int q = 0; q < V / 2; ++q) {
+            const int k = k0 + 2 * q;
+            float x, y;
+            split(acc[q], x, y);
+            if (k >= 0 && k < K) db[k] = x;
+            if (k + 1 >= 0 && k + 1 < K) db[k + 1] = y;
+        }
     }
 }
 
@@ -542,19 +702,19 @@ __global__ void __launch_bounds__(1024) k_loss_join(const ytm_loss_args a, const
 // How a call is cut: which kernels, and how many teams' parts there are to join.
 struct LossPlan {
     bool big;
-    int tpr, nv;               // small
-    int parts, rounds, chunk;  // big: parts of a row, rounds of a part, rows of a chunk
+    int tpr, nv;  // threads of a row (small), vectors of a thread (small: of four classes; big: in a round)
+    int parts, rounds, chunk, period;  // big: parts of a row, rounds of a part, rows of a chunk and their distance
     int64_t teams;             // blocks (small) or chunks (big)
 };
 
 constexpr int LOSS_CHAIN = 256;  // rows that one thread adds up in fp32 at most
 
-static LossPlan loss_plan(int64_t n, int64_t k, int64_t elem) {
+static LossPlan loss_plan(int64_t n, int64_t k, int64_t elem, int64_t cs_stride) {
     LossPlan p = {};
     const int64_t sms = sm_count();
-    if (k <= 1024) {
+    if (k <= 512) {
         p.tpr = k <= 16 ? 4 : k <= 128 ? 8 : k <= 256 ? 16 : 32;
-        p.nv = k <= 32 ? 1 : k <= 64 ? 2 : k <= 512 ? 4 : 8;
+        p.nv = k <= 32 ? 1 : k <= 64 ? 2 : 4;
         const int64_t rows = LS_THREADS / p.tpr;
         // up to four rounds of one block cost less than joining blocks
         p.teams = n <= 4 * rows ? 1 : std::min<int64_t>(cdiv(n, rows), sms * (p.nv >= 4 ? 2 : 4));
@@ -563,13 +723,18 @@ static LossPlan loss_plan(int64_t n, int64_t k, int64_t elem) {
     }
     p.big = true;
     // parts of a row until every SM has about eight blocks
-    const int64_t rounds = cdiv(k, LB_PART), want = std::max<int64_t>(1, std::min<int64_t>(32, cdiv(sms * 8, n)));
+    const int64_t vecs = cdiv(k * elem, 16) + 1;  // a row off a boundary can reach into one more
+    p.nv = vecs <= LB_THREADS ? 1 : (int)elem;    // 16 classes of a thread in a round
+    const int64_t rounds = cdiv(vecs, (int64_t)LB_THREADS * p.nv);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(32, cdiv(sms * 4, n)));
     p.rounds = (int)cdiv(rounds, std::min(want, rounds));
     p.parts = (int)cdiv(rounds, p.rounds);
-    // chunks of rows until there are about two rounds of blocks (four an SM)
-    const int64_t tiles = cdiv(k, LB_THREADS * 16 / elem);
-    p.chunk = (int)std::min<int64_t>(LB_ROWS, std::max<int64_t>(4, cdiv(n * tiles, sms * 8)));
-    p.teams = cdiv(n, p.chunk);
+    // the class sums' and the gradients' rows lie alike every `period` rows
+    p.period = 1;
+    while (k * elem * p.period % 16 || cs_stride * elem * p.period % 16) p.period *= 2;
+    // chunks of rows until there are about eight blocks an SM
+    p.chunk = (int)std::min<int64_t>(LB_ROWS, std::max<int64_t>(4, cdiv(n * cdiv(vecs, LB_THREADS), sms * 8)));
+    p.teams = (int64_t)p.period * cdiv(cdiv(n, p.period), p.chunk);
     return p;
 }
 
@@ -603,15 +768,18 @@ static LossWs loss_ws(const LossPlan &p, int64_t n, int64_t k) {
     return w;
 }
 
-template <typename T, bool VEC>
+template <typename T>
 static ytm_status launch_big(const ytm_loss_args &a, const LossPlan &p, const LossPart &part, LossStat *stats, cudaStream_t st) {
     const unsigned gz = (unsigned)cdiv(a.n, 65535), gy = (unsigned)cdiv(a.n, gz);
-    k_loss_stat<T, VEC><<<dim3(p.parts, gy, gz), LB_THREADS, 0, st>>>(a, stats, p.rounds);
+    const dim3 grid(p.parts, gy, gz);
+    if (p.nv == 1) k_loss_stat<T, 1><<<grid, LB_THREADS, 0, st>>>(a, stats, p.rounds);
+    else k_loss_stat<T, (int)sizeof(T)><<<grid, LB_THREADS, 0, st>>>(a, stats, p.rounds);
     ytm_status rc = launch_check("class loss statistics");
     if (rc) return rc;
-    const unsigned tiles = a.dcs || a.dbias ? (unsigned)cdiv(a.k, LB_THREADS * 16 / sizeof(T)) : 1;
-    return launch_after(k_loss_grad<T, VEC>, dim3(tiles, (unsigned)p.teams), LB_THREADS, st, "class loss", a, stats, p.parts,
-                        p.chunk, part);
+    const uint64_t vecs = cdiv((uint64_t)a.k * sizeof(T), 16) + (p.period > 1 || (uintptr_t)a.cs % 16 || (uintptr_t)a.dcs % 16);
+    const unsigned tiles = a.dcs || a.dbias ? (unsigned)cdiv(vecs, LB_THREADS) : 1;
+    return launch_after(k_loss_grad<T>, dim3(tiles, (unsigned)p.teams), LB_THREADS, st, "class loss", a, stats, p.parts,
+                        p.chunk, p.period, part);
 }
 
 template <typename T, int TPR, int NV>
@@ -624,19 +792,17 @@ static ytm_status launch_small(const ytm_loss_args &a, const LossPlan &p, const 
 
 template <typename T>
 static ytm_status launch_loss(const ytm_loss_args &a, const LossPlan &p, const LossPart &part, LossStat *stats, cudaStream_t st) {
-    // vectors: 16 bytes of long rows, four classes of short ones
-    const uint64_t step = p.big ? 16 : 4 * sizeof(T);
+    if (p.big) return launch_big<T>(a, p, part, stats, st);
+    // vectors of four classes
+    const uint64_t step = 4 * sizeof(T);
     const bool vec = (uintptr_t)a.cs % step == 0 && a.cs_stride * sizeof(T) % step == 0 &&
-                     (!a.dcs || ((uintptr_t)a.dcs % step == 0 && (uint64_t)a.k * sizeof(T) % step == 0)) &&
-                     (!p.big || (uintptr_t)a.bias % 16 == 0);
-    if (p.big) return vec ? launch_big<T, true>(a, p, part, stats, st) : launch_big<T, false>(a, p, part, stats, st);
+                     (!a.dcs || ((uintptr_t)a.dcs % step == 0 && (uint64_t)a.k * sizeof(T) % step == 0));
     if (p.tpr == 4) return launch_small<T, 4, 1>(a, p, part, vec, st);
     if (p.tpr == 8 && p.nv == 1) return launch_small<T, 8, 1>(a, p, part, vec, st);
     if (p.tpr == 8 && p.nv == 2) return launch_small<T, 8, 2>(a, p, part, vec, st);
     if (p.tpr == 8) return launch_small<T, 8, 4>(a, p, part, vec, st);
     if (p.tpr == 16) return launch_small<T, 16, 4>(a, p, part, vec, st);
-    if (p.nv == 4) return launch_small<T, 32, 4>(a, p, part, vec, st);
-    return launch_small<T, 32, 8>(a, p, part, vec, st);
+    return launch_small<T, 32, 4>(a, p, part, vec, st);
 }
 
 }  // namespace ytm
@@ -645,16 +811,16 @@ using namespace ytm;
 
 extern "C" {
 
-uint64_t ytm_class_loss_workspace_bytes(int64_t n, int32_t k, int32_t cs_type) {
-    if (n <= 0 || k <= 0 || !is_sum_type(cs_type)) return 0;
-    return loss_ws(loss_plan(n, k, type_bytes(cs_type)), n, k).total;
+uint64_t ytm_class_loss_workspace_bytes(int64_t n, int32_t k, int32_t cs_type, int64_t cs_stride) {
+    if (n <= 0 || k <= 0 || !is_sum_type(cs_type) || cs_stride < 0) return 0;
+    return loss_ws(loss_plan(n, k, type_bytes(cs_type), cs_stride), n, k).total;
 }
 
 ytm_status ytm_class_loss(const ytm_loss_args *args, void *workspace, void *stream) {
     if (!args) return fail(YTM_ERR_ARG, "args is NULL");
     const ytm_loss_args &a = *args;
     if (a.n < 0 || a.k <= 0) return fail(YTM_ERR_ARG, "class loss: needs n >= 0 rows of k >= 1 classes");
-    if (a.n > INT_MAX) return fail(YTM_ERR_UNSUPPORTED, "class loss: more than 2^31 - 1 rows");
+    if (a.n > INT_MAX || a.k > (1 << 30)) return fail(YTM_ERR_UNSUPPORTED, "class loss: more than 2^31 - 1 rows or 2^30 classes");
     if (!is_sum_type(a.cs_type)) return fail(YTM_ERR_ARG, "class loss: class sums must be int32, fp32, fp16 or bf16");
     if (a.cs_type == YTM_I32 && a.dcs) return fail(YTM_ERR_ARG, "class loss: int32 class sums have no gradient");
     if (a.cs_stride < 0 || a.allowed_stride < 0) return fail(YTM_ERR_ARG, "class loss: negative stride");
@@ -665,7 +831,7 @@ ytm_status ytm_class_loss(const ytm_loss_args *args, void *workspace, void *stre
         if (a.dtemperature && (rc = cuda_check(cudaMemsetAsync(a.dtemperature, 0, 4, st), "memset"))) return rc;
         return YTM_OK;
     }
-    const LossPlan p = loss_plan(a.n, a.k, type_bytes(a.cs_type));
+    const LossPlan p = loss_plan(a.n, a.k, type_bytes(a.cs_type), a.cs_stride);
     const LossWs ws = loss_ws(p, a.n, a.k);
     if (p.teams > (p.big ? 65535 : INT_MAX)) return fail(YTM_ERR_UNSUPPORTED, "class loss: too many rows for one call");
     if (!a.cs || !a.target || !a.loss || (ws.total && !workspace)) return fail(YTM_ERR_ARG, "null pointer");
