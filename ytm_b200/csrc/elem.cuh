@@ -35,15 +35,6 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Element c of the row of x that starts at element `row` (packed bits: word).
-template <int X>
-__device__ __forceinline__ float load_x(const void *x, int64_t row, int c) {
-    if (X == YTM_BITS) return (float)((((const uint32_t *)x)[row + c / 32] >> (c % 32)) & 1u);
-    if (X == YTM_F32) return ((const float *)x)[row + c];
-    if (X == YTM_F16) return __half2float(((const __half *)x)[row + c]);
-    return __bfloat162float(((const __nv_bfloat16 *)x)[row + c]);
-}
-
 // Bit k of a row of allowed-class words (NULL: every class is allowed).
 __device__ __forceinline__ bool is_allowed(const uint32_t *row, int64_t k) {
     return !row || ((row[k >> 5] >> (k & 31)) & 1u);
