@@ -77,7 +77,7 @@ struct Q4Args {
     void *y;
     int C, K, G, x_type, scale_type, y_type;
     int samples;              // of a block (grid z)
-    int wm, cluster;
+    int wm, log_wk, cluster;
     int xpitch;               // bytes between the activation columns in shared memory
 };
 
@@ -200,7 +200,7 @@ template <bool HALF, int NT, int GROUP>
 __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const Q4Args a) {
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int WM = a.wm, WK = Q4_WARPS / WM, wm = warp % WM, wk = warp / WM;
+    const int WM = a.wm, WK = 1 << a.log_wk, wm = warp % WM, wk = warp / WM;
     const int rank = a.cluster > 1 ? (int)cg::this_cluster().block_rank() : 0;
     const int64_t row_bytes = q4_row_bytes(a.C);
     const int row0 = (int)(blockIdx.x / a.cluster) * 16 * WM;
@@ -216,34 +216,49 @@ __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const 
     const int xbuf = a.samples * parts * a.xpitch;
     const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem);
 
-    const auto copy_stage = [&](int s) {  // weights of stage first + s
-        if (s < count) {
-            const int units = 8 * WK;  // 16-byte units of a row
-            const uint32_t base = smem_at + (s % Q4_STAGES) * Q4_STAGE_BYTES;
+    // Weights of stage first + s: the thread's 16-byte unit of a row is the same
+    // in its four rows.
+    const int log_units = 3 + a.log_wk;  // 16-byte units of a row in a stage
+    const int su = tid & ((1 << log_units) - 1), r0 = tid >> log_units, r_step = Q4_THREADS >> log_units;
+    const uint8_t *src[4];
+    uint32_t dst[4];
+    bool row_there[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + i * r_step;
+        row_there[i] = row0 + r < a.K;
+        src[i] = a.packed + (row_there[i] ? (row0 + r) * row_bytes : 0) + (int64_t)first * (16 << log_units) + su * 16;
+        dst[i] = smem_at + (((su >> 3) * WM + (r >> 4)) * 8 + (su & 7)) * 272 + (r & 15) * 16;
+    }
+    int64_t left = row_bytes - ((int64_t)first * (16 << log_units) + su * 16);  // bytes of the row from this stage's unit on
+    int copied = 0;
+    const auto copy_stage = [&]() {
+        if (copied < count) {
+            const uint32_t base = (copied % Q4_STAGES) * Q4_STAGE_BYTES;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int u = i * Q4_THREADS + tid, r = u / units, su = u - r * units;
-                const int64_t byte = ((int64_t)(first + s) * units + su) * 16;
-                const bool there = row0 + r < a.K && byte < row_bytes;
-                const uint32_t dst = base + (((su / 8) * WM + r / 16) * 8 + su % 8) * 272 + (r % 16) * 16;
-                cp_async16(dst, a.packed + (there ? (row0 + r) * row_bytes + byte : 0), there);
+                const bool there = row_there[i] && left > 0;
+                cp_async16(dst[i] + base, there ? src[i] : a.packed, there);
+                src[i] += 16 << log_units;
             }
+            left -= 16 << log_units;
         }
+        ++copied;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const int octets = 32 * WK;  // of a sample in a stage
+    const int log_octets = 5 + a.log_wk;  // of a sample in a stage
     const auto load_x = [&](int s, int u) {
-        const int i = u / octets;
-        return load_octet(a, (sample0 + i) * a.x_stride, (first + s) * Q4_SEG * WK + (u - i * octets) * 8);
+        const int i = u >> log_octets;
+        return load_octet(a, (sample0 + i) * a.x_stride, (first + s) * Q4_SEG * WK + (u - (i << log_octets)) * 8);
     };
     const auto store_x = [&](int s, int u, const Octet &o) {
-        const int i = u / octets;
-        store_octet(a, xs + (s & 1) * xbuf + i * parts * a.xpitch + (u - i * octets) * 16, o);
+        const int i = u >> log_octets;
+        store_octet(a, xs + (s & 1) * xbuf + i * parts * a.xpitch + (u - (i << log_octets)) * 16, o);
     };
-    const int x_units = octets * samples;
+    const int x_units = samples << log_octets;
 
 #pragma unroll
-    for (int s = 0; s < Q4_STAGES - 1; ++s) copy_stage(s);
+    for (int s = 0; s < Q4_STAGES - 1; ++s) copy_stage();
     if (count > 0)
         for (int u = tid; u < x_units; u += Q4_THREADS) store_x(0, u, load_x(0, u));
 
@@ -251,14 +266,14 @@ __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const 
     constexpr int GPS = Q4_SEG / GROUP, GPL = (GPS + 3) / 4;
     const int g = lane >> 2, t = lane & 3;
     const int class0 = row0 + wm * 16 + g, class1 = class0 + 8;
+    const int64_t at0 = class0 < a.K ? (int64_t)class0 * a.G : 0, at1 = class1 < a.K ? (int64_t)class1 * a.G : 0;
     const auto load_scales = [&](int s, float (&sc)[GPL][2]) {
 #pragma unroll
         for (int j = 0; j < GPL; ++j) {
-            const int in_stage = j * 4 + t;
-            const int64_t grp = (int64_t)((first + s) * WK + wk) * GPS + in_stage;
+            const int in_stage = j * 4 + t, grp = ((first + s) * WK + wk) * GPS + in_stage;
             const bool there = s < count && in_stage < GPS && grp < a.G;
-            sc[j][0] = there && class0 < a.K ? load_scale(a.scales, a.scale_type, (int64_t)class0 * a.G + grp) : 0.f;
-            sc[j][1] = there && class1 < a.K ? load_scale(a.scales, a.scale_type, (int64_t)class1 * a.G + grp) : 0.f;
+            sc[j][0] = there ? load_scale(a.scales, a.scale_type, at0 + grp) : 0.f;
+            sc[j][1] = there ? load_scale(a.scales, a.scale_type, at1 + grp) : 0.f;
         }
     };
     float next_sc[GPL][2];
@@ -269,12 +284,15 @@ __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const 
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) tot[n][i] = 0.f;
+    int x_col[NT];  // columns behind the last are the last once more; nobody reads their sums
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x_col[n] = min(n * 8 + g, cols - 1) * a.xpitch;
     const uint32_t mat = (warp * 8 + (lane >> 4)) * 272 + ((lane >> 3 & 1) * 8 + (lane & 7)) * 16;
 
     for (int s = 0; s < count; ++s) {
         asm volatile("cp.async.wait_group %0;" ::"n"(Q4_STAGES - 2) : "memory");
         __syncthreads();  // stage s and its activations are there; stage s - 1 is done with
-        copy_stage(s + Q4_STAGES - 1);
+        copy_stage();
         float sc[GPL][2];
 #pragma unroll
         for (int j = 0; j < GPL; ++j) {
@@ -287,7 +305,7 @@ __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const 
         if (more && tid < x_units) o = load_x(s + 1, tid);
 
         const uint32_t w_at = smem_at + (s % Q4_STAGES) * Q4_STAGE_BYTES + mat;
-        const char *x_at = xs + (s & 1) * xbuf + g * a.xpitch + wk * Q4_SEG * 2 + t * 16;
+        const char *x_at = xs + (s & 1) * xbuf + wk * Q4_SEG * 2 + t * 16;
         float acc[NT][4];
 #pragma unroll
         for (int j2 = 0; j2 < Q4_SEG / 64; ++j2) {
@@ -308,8 +326,7 @@ __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const 
                 unpack<HALF>(q[2 * h + 1], hi);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    uint4 b = make_uint4(0, 0, 0, 0);
-                    if (n * 8 + g < cols) b = *(const uint4 *)(x_at + n * 8 * a.xpitch + j * 64);
+                    const uint4 b = *(const uint4 *)(x_at + x_col[n] + j * 64);
                     mma<HALF>(acc[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
                     mma<HALF>(acc[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
                 }
@@ -370,9 +387,9 @@ __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const 
     if (a.cluster > 1) cg::this_cluster().sync();  // nobody leaves while its sums are read
 }
 
-// How the warps lie (see above).  The cost of a cut, in stages of 16 KB: rounds
-// of blocks on the GPU times the stages of a block plus about three for its
-// start and its end.
+// How the warps lie (see above).  The cost of a cut, in stages of 16 KB: the
+// blocks of the busiest SM times the stages of a block plus about three for its
+// start and its end, half of which a second block on the SM hides.
 struct Q4Plan {
     int wm, cluster, xpitch;
     size_t smem;
@@ -388,10 +405,11 @@ static Q4Plan q4_plan(int64_t C, int64_t K, int nt, int cols, int64_t z) {
         const size_t smem = std::max<size_t>((size_t)Q4_STAGES * Q4_STAGE_BYTES + 2 * (size_t)cols * xpitch, red);
         if (smem > 227 * 1024) continue;
         const int64_t tiles = cdiv(K, 16 * wm) * z, stages = cdiv(C, Q4_SEG * wk);
-        const int64_t slots = sms * (nt <= 2 && smem <= 113 * 1024 ? 2 : 1);
+        const bool two = nt <= 2 && smem <= 113 * 1024;
         for (int cl = 1; cl <= 16; cl *= 2) {
             if (cl > 1 && cl > stages) break;
-            const double cost = (double)cdiv(tiles * cl, slots) * (double)(cdiv(stages, cl) + 3);
+            // SMs that hold two blocks share their bandwidth between them
+            const double cost = (double)cdiv(tiles * cl, sms) * ((double)cdiv(stages, cl) + (two ? 1.5 : 3));
             if (!best.wm || cost < least * 0.97) {
                 best = {wm, cl, xpitch, smem};
                 least = cost;
@@ -496,7 +514,7 @@ ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t
     const int cols = samples * parts, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : cols <= 32 ? 4 : 8;
     const Q4Plan p = q4_plan(C, K, nt, cols, z);
     Q4Args a = {x, x_stride, 0, 0, packed, scales, bias, y, C, K, (int)cdiv(C, group), x_type, scale_type, y_type,
-                samples, p.wm, p.cluster, p.xpitch};
+                samples, p.wm, p.wm == 8 ? 0 : p.wm == 4 ? 1 : p.wm == 2 ? 2 : 3, p.cluster, p.xpitch};
     for (int64_t i = 0; i < N; i += z * most) {
         a.n0 = i;
         a.n = std::min<int64_t>(N - i, z * most);
