@@ -381,10 +381,12 @@ ytm_status ytm_q4_pack(const void *weights, int32_t w_type, int64_t w_stride, in
 /* Votes y[n][k] = bias[k] + sum_g scale[k][g] * sum_{c in g} (packed[k][c] - 8)
  * * x[n][c], sums in fp32, rounded once to y_type.  x [N][C] (f32, f16, bf16)
  * or clause bits (YTM_BITS, x_stride in words); packed on a 16-byte boundary,
- * halves 0..15; bias f32 [K] or NULL; y [N][K]. */
+ * halves 0..15; bias f32 [K] or NULL; y [N][K].  workspace:
+ * ytm_q4_votes_workspace_bytes(...), on a 16-byte boundary. */
 ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t N, int32_t C, const uint8_t *packed,
                         const void *scales, int32_t scale_type, int32_t group, int32_t K, const float *bias, void *y,
-                        int32_t y_type, void *stream);
+                        int32_t y_type, void *workspace, void *stream);
+uint64_t ytm_q4_votes_workspace_bytes(int32_t x_type, int64_t N, int32_t C, int32_t K);
 
 /* Fired clauses of inference as bits u32 [N][ceil(C / 32)] (bits behind the
  * last clause 0): the clauses ytm_infer counts, i.e. without those that

@@ -43,11 +43,11 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
                dict(s=None)):
         assert pack(**kw) == 1, kw
     votes = lambda **kw: lib.ytm_q4_votes(*[{**dict(x=one, xt=1, xs=8, N=1, C=8, p=one, s=one, st=1, g=64, K=4,  # noqa: E731
-                                                    b=None, y=one, yt=1), **kw}[i]
-                                            for i in ("x", "xt", "xs", "N", "C", "p", "s", "st", "g", "K", "b", "y", "yt")],
+                                                    b=None, y=one, yt=1, ws=one), **kw}[i]
+                                            for i in ("x", "xt", "xs", "N", "C", "p", "s", "st", "g", "K", "b", "y", "yt", "ws")],
                                           None)
     for kw in (dict(xt=0), dict(xt=5), dict(xs=-1), dict(N=-1), dict(C=0), dict(p=None), dict(p=ct.c_void_p(8)), dict(st=4),
-               dict(g=16), dict(K=0), dict(y=None), dict(yt=0), dict(x=None), dict(s=None)):
+               dict(g=16), dict(K=0), dict(y=None), dict(yt=0), dict(x=None), dict(s=None), dict(ws=None), dict(ws=ct.c_void_p(8))):
         assert votes(**kw) == 1, kw
     assert votes(N=0) == 0
     good = dict(cs=16, cs_stride=4, n=1, k=4, cs_type=0)

@@ -156,11 +156,14 @@ def q4_votes(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group:
         bias = _vector(bias, "bias", K, (torch.float32,), dev)
     n = x.shape[0]
     y = torch.empty((n, K), dtype=out_dtype, device=dev)
+    if n == 0:
+        return y
+    lib, x_type = _lib.load(), _lib.YTM_BITS if bits else _TYPES[x.dtype]
     with _on(dev):
-        check(_lib.load().ytm_q4_votes(x.data_ptr(), _lib.YTM_BITS if bits else _TYPES[x.dtype], _row_stride(x), n,
-                                       clauses, packed.data_ptr(), scales.data_ptr(), _TYPES[scales.dtype], group, K,
-                                       None if bias is None else bias.data_ptr(), y.data_ptr(), _TYPES[out_dtype],
-                                       _stream(dev)), "ytm_q4_votes")
+        ws = torch.empty(lib.ytm_q4_votes_workspace_bytes(x_type, n, clauses, K), dtype=torch.uint8, device=dev)
+        check(lib.ytm_q4_votes(x.data_ptr(), x_type, _row_stride(x), n, clauses, packed.data_ptr(), scales.data_ptr(),
+                               _TYPES[scales.dtype], group, K, None if bias is None else bias.data_ptr(), y.data_ptr(),
+                               _TYPES[out_dtype], ws.data_ptr(), _stream(dev)), "ytm_q4_votes")
     return y
 
 

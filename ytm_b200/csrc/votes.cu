@@ -1,5 +1,7 @@
 // votes.cu — the vote of clause weights held in 4 bits with group scales.
 #include <cooperative_groups.h>
+#include <cuda.h>
+#include <limits.h>
 
 #include "common.cuh"
 #include "elem.cuh"
@@ -45,17 +47,19 @@ __global__ void k_q4_pack(const T *__restrict__ w, int64_t w_stride, int C, int 
 // y[n][k] = bias[k] + sum_g scale[k][g] * sum_{c in g} (q - 8) x[n][c].
 //
 // The weights' bytes bound the call while there are few samples, so they are
-// what streams: a block copies 16 KB of them a stage into shared memory with
-// 16-byte asynchronous copies, four stages deep, and a warp multiplies 16
+// what streams: one thread of a block copies 16 KB of them a stage into shared
+// memory by TMA, four stages deep, and each of eight warps multiplies 16
 // classes by 256 clauses of a stage on the tensor cores (m16n8k16, fp32 sums).
 // ldmatrix hands lane (g, t) word t of 32 clauses of classes g and g + 8, i.e.
 // eight 4-bit weights, which the lane turns into bf16 or fp16 pairs (clauses i
 // and i + 4) by or-ing them into the fraction of 128 (1024) and subtracting
-// 136 (1032): exact.  The activations lie in shared memory in that order of
-// clauses.  The sum of a group is exact up to the fp32 additions; its scale is
-// applied in fp32.  Activations in fp32 take three columns, their leading,
-// middle and last 8 bits, which are bf16 values exactly; clause bits are bf16
-// zeros and ones.
+// 136 (1032): exact.  The sum of a group is exact up to the fp32 additions; its
+// scale is applied in fp32.
+//
+// k_q4_x lays the activations out before: in that order of clauses, group by
+// group of 32, so that a stage's are one piece of memory.  Activations in fp32
+// take three columns, their leading, middle and last 8 bits, which are bf16
+// values exactly; clause bits are bf16 zeros and ones.
 //
 // WM of a block's 8 warps lie along the classes, 8 / WM along the clauses, and
 // up to 16 blocks of a cluster along the clauses, which add their sums through
@@ -63,32 +67,139 @@ __global__ void k_q4_pack(const T *__restrict__ w, int64_t w_stride, int C, int 
 
 namespace cg = cooperative_groups;
 
-constexpr int Q4_THREADS = 256, Q4_WARPS = 8, Q4_STAGES = 4;
-constexpr int Q4_SEG = 256;                                       // clauses of a warp in a stage
-constexpr int Q4_WARP_BYTES = Q4_SEG / 32 * 17 * 16;              // 16 classes of a stage, rows of 17 x 16 bytes
-constexpr int Q4_STAGE_BYTES = Q4_WARPS * Q4_WARP_BYTES;
+constexpr int Q4_WARPS = 8, Q4_THREADS = 32 * (Q4_WARPS + 1);  // the last warp copies
+constexpr int Q4_STAGES = 4;
+constexpr int Q4_SEG = 256;                        // clauses of a warp in a stage: 128 bytes of a class
+constexpr int Q4_STAGE_BYTES = Q4_WARPS * 16 * 128;
+constexpr int Q4_BARS = 128;                       // bytes of the barriers and the failure flag
 
 struct Q4Args {
-    const void *x;
-    int64_t x_stride, n0, n;  // samples n0 .. n0 + n of this call
-    const uint8_t *packed;
+    const char *xs;           // k_q4_x's activations: [block of samples][group of 32][column][64 bytes]
     const void *scales;
     const float *bias;
     void *y;
-    int C, K, G, x_type, scale_type, y_type;
-    int samples;              // of a block (grid z)
-    int wm, log_wk, cluster;
-    int xpitch;               // bytes between the activation columns in shared memory
+    int64_t n0, n;            // samples n0 .. n0 + n of this launch
+    int64_t xs_block;         // bytes of a block of samples in xs
+    int K, G, stages, scale_type, y_type;
+    int samples, parts;       // of a block (grid z); columns of a sample
+    int log_wk, cluster, bars_at;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+// ---- activations
+
+struct Q4XArgs {
+    const void *x;
+    int64_t x_stride, n0, n;
+    char *xs;
+    int64_t xs_block;
+    int C, x_type, samples, parts, groups;
+};
+
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {  // of values that bf16 holds
+    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
 }
 
-__device__ __forceinline__ float load_scale(const void *p, int type, int64_t i) {
-    if (type == YTM_F32) return ((const float *)p)[i];
-    if (type == YTM_F16) return __half2float(((const __half *)p)[i]);
-    return __bfloat162float(((const __nv_bfloat16 *)p)[i]);
+// A thread takes 8 clauses of a sample and writes them in the order (0, 4, 1,
+// 5, 2, 6, 3, 7).  Within the 64 bytes of a (group, column) the four 16-byte
+// pieces are exchanged by the column's bits 1 and 2, so that the eight lanes
+// that read two columns together meet 32 different banks.
+__global__ void __launch_bounds__(256) k_q4_x(const Q4XArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int octets = a.groups * 4;
+    const int64_t i = u / octets;  // sample of this launch
+    if (i >= a.n) return;
+    const int o = (int)(u - i * octets), c = o * 8;
+    const int64_t row = (a.n0 + i) * a.x_stride;
+    const int col = (int)(i % a.samples) * a.parts;
+    char *const base = a.xs + i / a.samples * a.xs_block + (int64_t)(o >> 2) * a.samples * a.parts * 64;
+    const auto put = [&](int part, uint4 v) {
+        const int k = col + part;
+        *(uint4 *)(base + k * 64 + ((o & 3) ^ (k >> 1 & 3)) * 16) = v;
+    };
+    if (a.x_type == YTM_BITS) {
+        uint32_t w = c < a.C ? ((const uint32_t *)a.x)[row + (c >> 5)] >> (c & 31) & 255u : 0u;
+        if (c < a.C && c + 8 > a.C) w &= (1u << (a.C - c)) - 1u;
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = ((w >> j) & 1u) * 0x3F80u | ((w >> (j + 4)) & 1u) * 0x3F800000u;
+        put(0, make_uint4(v[0], v[1], v[2], v[3]));
+    } else if (a.x_type == YTM_F32) {
+        const float *p = (const float *)a.x + row + c;
+        float rest[8];
+        if (c + 8 <= a.C && (uintptr_t)p % 16 == 0) {
+            *(float4 *)&rest[0] = *(const float4 *)p;
+            *(float4 *)&rest[4] = *(const float4 *)(p + 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rest[j] = c + j < a.C ? p[j] : 0.f;
+        }
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            float top[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {  // the leading 8 bits; NaN stays NaN, infinity leaves nothing
+                top[j] = __uint_as_float(__float_as_uint(rest[j]) & 0xFFFF0000u);
+                if (part == 0 && rest[j] != rest[j]) top[j] = __uint_as_float(0x7FC00000u);
+                rest[j] = part == 0 && !(fabsf(rest[j]) < INFINITY) ? 0.f : rest[j] - top[j];
+            }
+            put(part, make_uint4(bf16_pair(top[0], top[4]), bf16_pair(top[1], top[5]), bf16_pair(top[2], top[6]),
+                                 bf16_pair(top[3], top[7])));
+        }
+    } else {
+        const uint16_t *p = (const uint16_t *)a.x + row + c;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (c + 8 <= a.C && (uintptr_t)p % 16 == 0) {
+            v = *(const uint4 *)p;
+        } else {
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < a.C) w[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        put(0, make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                          __byte_perm(v.y, v.w, 0x7632)));
+    }
+}
+
+// ---- products
+
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{.reg .pred p;\n\tmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
+__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity) {
+    uint64_t start, now;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(start));
+    for (int i = 0; i < (1 << 24); ++i) {
+        if (bar_try(bar, parity)) return true;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+        if (now - start > 2000000000ull) break;
+    }
+    return false;
+}
+// Waits for the phase with this parity; false if it did not come within about
+// two seconds.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+    return bar_try(bar, parity) || bar_wait_long(bar, parity);
+}
+
+__device__ __forceinline__ float scale_value(uint32_t raw, int type) {
+    if (type == YTM_F32) return __uint_as_float(raw);
+    if (type == YTM_F16) return __half2float(__ushort_as_half((unsigned short)raw));
+    return __uint_as_float(raw << 16);
 }
 
 // Eight 4-bit weights -> four pairs (i, i + 4) of the value minus 8.
@@ -123,254 +234,185 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {  // of values that bf16 holds
-    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
-}
-
-// Eight activations c .. c + 7 of a sample (0 behind the last clause).
-struct Octet {
-    uint32_t w[8];  // fp32: values; 16-bit: pairs in w[0..3]; bits: w[0]
-};
-
-__device__ __forceinline__ Octet load_octet(const Q4Args &a, int64_t row, int c) {
-    Octet o;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o.w[i] = 0;
-    if (c >= a.C) return o;
-    if (a.x_type == YTM_BITS) {
-        o.w[0] = ((const uint32_t *)a.x)[row + (c >> 5)] >> (c & 31) & 255u;
-        if (c + 8 > a.C) o.w[0] &= (1u << (a.C - c)) - 1u;
-        return o;
-    }
-    const bool all = c + 8 <= a.C;
-    if (a.x_type == YTM_F32) {
-        const float *p = (const float *)a.x + row + c;
-        if (all && (uintptr_t)p % 16 == 0) {
-            *(uint4 *)&o.w[0] = *(const uint4 *)p;
-            *(uint4 *)&o.w[4] = *(const uint4 *)(p + 4);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < a.C) o.w[i] = __float_as_uint(p[i]);
-        }
-        return o;
-    }
-    const uint16_t *p = (const uint16_t *)a.x + row + c;
-    if (all && (uintptr_t)p % 16 == 0) {
-        *(uint4 *)&o.w[0] = *(const uint4 *)p;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < a.C) o.w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
-    }
-    return o;
-}
-
-// The octet in the order (0, 4, 1, 5, 2, 6, 3, 7), at byte `at` of its column
-// (fp32: of its three columns).
-__device__ __forceinline__ void store_octet(const Q4Args &a, char *at, const Octet &o) {
-    if (a.x_type == YTM_BITS) {
-        uint32_t v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = ((o.w[0] >> i) & 1u) * 0x3F80u | ((o.w[0] >> (i + 4)) & 1u) * 0x3F800000u;
-        *(uint4 *)at = make_uint4(v[0], v[1], v[2], v[3]);
-    } else if (a.x_type == YTM_F32) {
-        float rest[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) rest[i] = __uint_as_float(o.w[i]);
-#pragma unroll
-        for (int part = 0; part < 3; ++part) {
-            float top[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {  // the leading 8 bits; NaN stays NaN, infinity leaves nothing
-                top[i] = __uint_as_float(__float_as_uint(rest[i]) & 0xFFFF0000u);
-                if (part == 0 && rest[i] != rest[i]) top[i] = __uint_as_float(0x7FC00000u);
-                rest[i] = part == 0 && !(fabsf(rest[i]) < INFINITY) ? 0.f : rest[i] - top[i];
-            }
-            *(uint4 *)(at + part * a.xpitch) = make_uint4(bf16_pair(top[0], top[4]), bf16_pair(top[1], top[5]),
-                                                          bf16_pair(top[2], top[6]), bf16_pair(top[3], top[7]));
-        }
-    } else {
-        *(uint4 *)at = make_uint4(__byte_perm(o.w[0], o.w[2], 0x5410), __byte_perm(o.w[0], o.w[2], 0x7632),
-                                  __byte_perm(o.w[1], o.w[3], 0x5410), __byte_perm(o.w[1], o.w[3], 0x7632));
-    }
-}
-
 template <bool HALF, int NT, int GROUP>
-__global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const Q4Args a) {
-    extern __shared__ __align__(16) char smem[];
+__global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const Q4Args a, const __grid_constant__ CUtensorMap weights) {
+    extern __shared__ __align__(1024) char smem[];  // weights, activations; barriers at the end
+    uint64_t *const bars = (uint64_t *)(smem + a.bars_at);
+    volatile int &failed = *(int *)(bars + 2 * Q4_STAGES);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int WM = a.wm, WK = 1 << a.log_wk, wm = warp % WM, wk = warp / WM;
+    const int WK = 1 << a.log_wk, WM = Q4_WARPS >> a.log_wk;
     const int rank = a.cluster > 1 ? (int)cg::this_cluster().block_rank() : 0;
-    const int64_t row_bytes = q4_row_bytes(a.C);
     const int row0 = (int)(blockIdx.x / a.cluster) * 16 * WM;
-    const int64_t sample0 = a.n0 + (int64_t)blockIdx.z * a.samples;
-    const int samples = (int)min((int64_t)a.samples, a.n0 + a.n - sample0);
-    const int parts = a.x_type == YTM_F32 ? 3 : 1, cols = samples * parts;
-    // this block's stages of the C clauses: WK segments each
-    const int stages_all = (a.C + Q4_SEG * WK - 1) / (Q4_SEG * WK);
-    const int per = (stages_all + a.cluster - 1) / a.cluster;
-    const int first = min(rank * per, stages_all), count = min(first + per, stages_all) - first;
-
-    char *xs = smem + Q4_STAGES * Q4_STAGE_BYTES;
-    const int xbuf = a.samples * parts * a.xpitch;
+    // this block's stages of the clauses: WK segments each
+    const int per = (a.stages + a.cluster - 1) / a.cluster;
+    const int first = min(rank * per, a.stages), count = min(first + per, a.stages) - first;
+    const int cols = a.samples * a.parts;
+    const int x_bytes = cols * 64 * (Q4_SEG / 32) * WK;  // of a stage
+    char *const xs = smem + Q4_STAGES * Q4_STAGE_BYTES;
     const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem);
-
-    // Weights of stage first + s: the thread's 16-byte unit of a row is the same
-    // in its four rows.
-    const int log_units = 3 + a.log_wk;  // 16-byte units of a row in a stage
-    const int su = tid & ((1 << log_units) - 1), r0 = tid >> log_units, r_step = Q4_THREADS >> log_units;
-    const uint8_t *src[4];
-    uint32_t dst[4];
-    bool row_there[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = r0 + i * r_step;
-        row_there[i] = row0 + r < a.K;
-        src[i] = a.packed + (row_there[i] ? (row0 + r) * row_bytes : 0) + (int64_t)first * (16 << log_units) + su * 16;
-        dst[i] = smem_at + (((su >> 3) * WM + (r >> 4)) * 8 + (su & 7)) * 272 + (r & 15) * 16;
+    const uint32_t full = (uint32_t)__cvta_generic_to_shared(bars), empty = full + 8 * Q4_STAGES;
+    if (tid == 0) {
+        failed = 0;
+        for (int s = 0; s < Q4_STAGES; ++s) {
+            bar_init(full + 8 * s, 1);
+            bar_init(empty + 8 * s, Q4_WARPS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    int64_t left = row_bytes - ((int64_t)first * (16 << log_units) + su * 16);  // bytes of the row from this stage's unit on
-    int copied = 0;
-    const auto copy_stage = [&]() {
-        if (copied < count) {
-            const uint32_t base = (copied % Q4_STAGES) * Q4_STAGE_BYTES;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool there = row_there[i] && left > 0;
-                cp_async16(dst[i] + base, there ? src[i] : a.packed, there);
-                src[i] += 16 << log_units;
-            }
-            left -= 16 << log_units;
-        }
-        ++copied;
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    const int log_octets = 5 + a.log_wk;  // of a sample in a stage
-    const auto load_x = [&](int s, int u) {
-        const int i = u >> log_octets;
-        return load_octet(a, (sample0 + i) * a.x_stride, (first + s) * Q4_SEG * WK + (u - (i << log_octets)) * 8);
-    };
-    const auto store_x = [&](int s, int u, const Octet &o) {
-        const int i = u >> log_octets;
-        store_octet(a, xs + (s & 1) * xbuf + i * parts * a.xpitch + (u - (i << log_octets)) * 16, o);
-    };
-    const int x_units = samples << log_octets;
+    __syncthreads();
 
-#pragma unroll
-    for (int s = 0; s < Q4_STAGES - 1; ++s) copy_stage();
-    if (count > 0)
-        for (int u = tid; u < x_units; u += Q4_THREADS) store_x(0, u, load_x(0, u));
-
-    // scales: lane t of a class holds groups t, t + 4, ... of a stage
     constexpr int GPS = Q4_SEG / GROUP, GPL = (GPS + 3) / 4;
-    const int g = lane >> 2, t = lane & 3;
-    const int class0 = row0 + wm * 16 + g, class1 = class0 + 8;
-    const int64_t at0 = class0 < a.K ? (int64_t)class0 * a.G : 0, at1 = class1 < a.K ? (int64_t)class1 * a.G : 0;
-    const auto load_scales = [&](int s, float (&sc)[GPL][2]) {
-#pragma unroll
-        for (int j = 0; j < GPL; ++j) {
-            const int in_stage = j * 4 + t, grp = ((first + s) * WK + wk) * GPS + in_stage;
-            const bool there = s < count && in_stage < GPS && grp < a.G;
-            sc[j][0] = there ? load_scale(a.scales, a.scale_type, at0 + grp) : 0.f;
-            sc[j][1] = there ? load_scale(a.scales, a.scale_type, at1 + grp) : 0.f;
-        }
-    };
-    float next_sc[GPL][2];
-    load_scales(0, next_sc);
-
+    const int g = lane >> 2, t = lane & 3, wm = warp % WM, wk = warp / WM;
     float tot[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) tot[n][i] = 0.f;
-    int x_col[NT];  // columns behind the last are the last once more; nobody reads their sums
-#pragma unroll
-    for (int n = 0; n < NT; ++n) x_col[n] = min(n * 8 + g, cols - 1) * a.xpitch;
-    const uint32_t mat = (warp * 8 + (lane >> 4)) * 272 + ((lane >> 3 & 1) * 8 + (lane & 7)) * 16;
 
-    for (int s = 0; s < count; ++s) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(Q4_STAGES - 2) : "memory");
-        __syncthreads();  // stage s and its activations are there; stage s - 1 is done with
-        copy_stage();
-        float sc[GPL][2];
-#pragma unroll
-        for (int j = 0; j < GPL; ++j) {
-            sc[j][0] = next_sc[j][0];
-            sc[j][1] = next_sc[j][1];
+    if (warp == Q4_WARPS) {
+        if (lane == 0) {
+            bool bad = false;
+            const char *const x0 = a.xs + blockIdx.z * a.xs_block + (int64_t)first * x_bytes;
+            const auto copy_weights = [&](int s) {
+                const uint32_t at = smem_at + (s % Q4_STAGES) * Q4_STAGE_BYTES, bar = full + 8 * (s % Q4_STAGES);
+                bar_expect(bar, Q4_STAGE_BYTES + x_bytes);
+                for (int k = 0; k < WK; ++k)
+                    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                                 ::"r"(at + k * WM * 2048), "l"(&weights), "r"(((first + s) * WK + k) * 128), "r"(row0), "r"(bar)
+                                 : "memory");
+            };
+            const auto copy_x = [&](int s) {
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                             ::"r"((uint32_t)__cvta_generic_to_shared(xs) + (s % Q4_STAGES) * x_bytes), "l"(x0 + (int64_t)s * x_bytes),
+                               "r"(x_bytes), "r"(full + 8 * (s % Q4_STAGES)) : "memory");
+            };
+            // the weights do not wait for k_q4_x
+            for (int s = 0; s < min(count, Q4_STAGES); ++s) copy_weights(s);
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int s = 0; s < min(count, Q4_STAGES); ++s) copy_x(s);
+            for (int s = Q4_STAGES; s < count; ++s) {
+                if (!bar_wait(empty + 8 * (s % Q4_STAGES), (s / Q4_STAGES - 1) & 1)) {
+                    bad = true;
+                    break;
+                }
+                copy_weights(s);
+                copy_x(s);
+            }
+            if (bad) failed = 1;
         }
-        load_scales(s + 1, next_sc);
-        Octet o;  // the next stage's first octet is on its way during the products
-        const bool more = s + 1 < count;
-        if (more && tid < x_units) o = load_x(s + 1, tid);
-
-        const uint32_t w_at = smem_at + (s % Q4_STAGES) * Q4_STAGE_BYTES + mat;
-        const char *x_at = xs + (s & 1) * xbuf + wk * Q4_SEG * 2 + t * 16;
-        float acc[NT][4];
+    } else {
+        // scales: lane t of a class holds groups t, t + 4, ... of a stage
+        const int class0 = row0 + wm * 16 + g, class1 = class0 + 8;
+        const int64_t at0 = class0 < a.K ? (int64_t)class0 * a.G : 0, at1 = class1 < a.K ? (int64_t)class1 * a.G : 0;
+        const bool wide = a.scale_type == YTM_F32;
+        const auto load_scales = [&](int s, uint32_t (&sc)[GPL][2]) {
 #pragma unroll
-        for (int j2 = 0; j2 < Q4_SEG / 64; ++j2) {
-            uint32_t q[4];
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(w_at + j2 * 2 * 272));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int j = j2 * 2 + h;  // 32 clauses
-                if (j % (GROUP / 32) == 0) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+            for (int j = 0; j < GPL; ++j) {
+                const int grp = min(((first + s) * WK + wk) * GPS + j * 4 + t, a.G - 1);
+                if (wide) {
+                    sc[j][0] = ((const uint32_t *)a.scales)[at0 + grp];
+                    sc[j][1] = ((const uint32_t *)a.scales)[at1 + grp];
+                } else {
+                    sc[j][0] = ((const uint16_t *)a.scales)[at0 + grp];
+                    sc[j][1] = ((const uint16_t *)a.scales)[at1 + grp];
                 }
-                uint32_t lo[4], hi[4];
-                unpack<HALF>(q[2 * h], lo);
-                unpack<HALF>(q[2 * h + 1], hi);
+            }
+        };
+        uint32_t next_sc[GPL][2];
+        load_scales(0, next_sc);
+        int x_col[NT];  // columns behind the last are the last once more; nobody reads their sums
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint4 b = *(const uint4 *)(x_at + x_col[n] + j * 64);
-                    mma<HALF>(acc[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
-                    mma<HALF>(acc[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
-                }
-                if ((j + 1) % (GROUP / 32) == 0) {
-                    const int grp = j / (GROUP / 32), from = (lane & ~3) | (grp & 3);
-                    const float s0 = __shfl_sync(0xFFFFFFFFu, sc[grp / 4][0], from), s1 = __shfl_sync(0xFFFFFFFFu, sc[grp / 4][1], from);
+        for (int n = 0; n < NT; ++n) {
+            const int k = min(n * 8 + g, cols - 1);
+            x_col[n] = k * 64 + (t ^ (k >> 1 & 3)) * 16;
+        }
+        const int x_group = cols * 64;
+        // rows of 128 bytes, their 16-byte pieces exchanged by the row's low bits (128-byte swizzle)
+        const int mrow = (lane >> 3 & 1) * 8 + (lane & 7);
+        const uint32_t mat = smem_at + (wk * WM + wm) * 2048 + mrow * 128;
+        for (int s = 0; s < count; ++s) {
+            float sc[GPL][2];
+#pragma unroll
+            for (int j = 0; j < GPL; ++j) {
+                const bool there = ((first + s) * WK + wk) * GPS + j * 4 + t < a.G;  // behind the last group: 0
+                sc[j][0] = there ? scale_value(next_sc[j][0], a.scale_type) : 0.f;
+                sc[j][1] = there ? scale_value(next_sc[j][1], a.scale_type) : 0.f;
+            }
+            load_scales(s + 1, next_sc);
+            if (!__all_sync(0xFFFFFFFFu, bar_wait(full + 8 * (s % Q4_STAGES), (s / Q4_STAGES) & 1))) {
+                if (lane == 0) failed = 1;
+                break;
+            }
+            const uint32_t w_at = mat + (s % Q4_STAGES) * Q4_STAGE_BYTES;
+            const char *x_at = xs + (s % Q4_STAGES) * x_bytes + wk * (Q4_SEG / 32) * x_group;
+            float acc[NT][4];
+#pragma unroll
+            for (int j2 = 0; j2 < Q4_SEG / 64; ++j2) {
+                uint32_t q[4];
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
+                             : "r"(w_at + (((j2 * 2 + (lane >> 4)) ^ (lane & 7)) * 16)));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int j = j2 * 2 + h;  // 32 clauses
+                    if (j % (GROUP / 32) == 0) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+                    }
+                    uint32_t lo[4], hi[4];
+                    unpack<HALF>(q[2 * h], lo);
+                    unpack<HALF>(q[2 * h + 1], hi);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        tot[n][0] = fmaf(s0, acc[n][0], tot[n][0]);
-                        tot[n][1] = fmaf(s0, acc[n][1], tot[n][1]);
-                        tot[n][2] = fmaf(s1, acc[n][2], tot[n][2]);
-                        tot[n][3] = fmaf(s1, acc[n][3], tot[n][3]);
+                        const uint4 b = *(const uint4 *)(x_at + x_col[n] + j * x_group);
+                        mma<HALF>(acc[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
+                        mma<HALF>(acc[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
+                    }
+                    if ((j + 1) % (GROUP / 32) == 0) {
+                        const int grp = j / (GROUP / 32), from = (lane & ~3) | (grp & 3);
+                        const float s0 = __shfl_sync(0xFFFFFFFFu, sc[grp / 4][0], from), s1 = __shfl_sync(0xFFFFFFFFu, sc[grp / 4][1], from);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            tot[n][0] = fmaf(s0, acc[n][0], tot[n][0]);
+                            tot[n][1] = fmaf(s0, acc[n][1], tot[n][1]);
+                            tot[n][2] = fmaf(s1, acc[n][2], tot[n][2]);
+                            tot[n][3] = fmaf(s1, acc[n][3], tot[n][3]);
+                        }
                     }
                 }
             }
-        }
-        if (more) {
-            if (tid < x_units) store_x(s + 1, tid, o);
-            for (int u = tid + Q4_THREADS; u < x_units; u += Q4_THREADS) store_x(s + 1, u, load_x(s + 1, u));
+            __syncwarp();
+            if (lane == 0) bar_arrive(empty + 8 * (s % Q4_STAGES));
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
+    __syncthreads();  // all stages have been read
     // sums of the warps along the clauses and of the parts of an activation
     constexpr int COLS = NT * 8;
     float *red = (float *)smem;                      // [warp][16][COLS]
     float *mine = red + Q4_WARPS * 16 * COLS;        // [samples][16 * WM]
+    if (warp < Q4_WARPS) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[(warp * 16 + g + (i >> 1) * 8) * COLS + n * 8 + t * 2 + (i & 1)] = tot[n][i];
+            for (int i = 0; i < 4; ++i) red[(warp * 16 + g + (i >> 1) * 8) * COLS + n * 8 + t * 2 + (i & 1)] = tot[n][i];
+    }
     __syncthreads();
-    const int rows = 16 * WM, outs = rows * samples;
+    const int64_t sample0 = a.n0 + (int64_t)blockIdx.z * a.samples;
+    const int samples = (int)min((int64_t)a.samples, a.n0 + a.n - sample0);
+    const int rows = 16 * WM, log_rows = 7 - a.log_wk, outs = rows * samples;
     for (int u = tid; u < outs; u += Q4_THREADS) {
-        const int i = u / rows, r = u - i * rows;
-        float v = 0.f;
+        const int i = u >> log_rows, r = u & (rows - 1);
+        float v = failed ? NAN : 0.f;  // NaN: a copy did not come
         for (int k = 0; k < WK; ++k)
-            for (int p = 0; p < parts; ++p) v += red[((k * WM + r / 16) * 16 + r % 16) * COLS + i * parts + p];
+            for (int p = 0; p < a.parts; ++p) v += red[((k * WM + (r >> 4)) * 16 + (r & 15)) * COLS + i * a.parts + p];
         mine[u] = v;
     }
     __syncthreads();
     if (a.cluster > 1) cg::this_cluster().sync();
     for (int u = rank * Q4_THREADS + tid; u < outs; u += a.cluster * Q4_THREADS) {
-        const int i = u / rows, r = u - i * rows;
+        const int i = u >> log_rows, r = u & (rows - 1);
         float v = 0.f;
         if (a.cluster > 1) {
             for (int k = 0; k < a.cluster; ++k) v += *cg::this_cluster().map_shared_rank(mine + u, k);
@@ -387,40 +429,68 @@ __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const 
     if (a.cluster > 1) cg::this_cluster().sync();  // nobody leaves while its sums are read
 }
 
-// How the warps lie (see above).  The cost of a cut, in stages of 16 KB: the
-// blocks of the busiest SM times the stages of a block plus about three for its
-// start and its end, half of which a second block on the SM hides.
+// How a call is cut.  The cost of a cut, in stages of 16 KB: the blocks of the
+// busiest SM times the stages of a block plus about three for its start and its
+// end, half of which a second block on the SM hides.
 struct Q4Plan {
-    int wm, cluster, xpitch;
+    int nt, samples, parts;  // of a block
+    int wm, log_wk, cluster, stages;
+    int64_t z, xs_block;     // blocks of samples of a launch, bytes of one's activations
     size_t smem;
 };
 
-static Q4Plan q4_plan(int64_t C, int64_t K, int nt, int cols, int64_t z) {
-    Q4Plan best = {};
+static Q4Plan q4_plan(int64_t N, int64_t C, int64_t K, int x_type) {
+    Q4Plan p = {};
+    p.parts = x_type == YTM_F32 ? 3 : 1;
+    const int64_t most = 64 / p.parts;
+    p.samples = (int)std::min(N, most);
+    p.z = std::min<int64_t>(cdiv(N, most), 65535);
+    const int cols = p.samples * p.parts;
+    p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : cols <= 32 ? 4 : 8;
     double least = 0;
     const int64_t sms = sm_count();
-    for (int wm = 8; wm >= 1; wm /= 2) {
-        const int wk = Q4_WARPS / wm, xpitch = Q4_SEG * 2 * wk + 64;
-        const size_t red = (size_t)Q4_WARPS * 16 * nt * 8 * 4 + (size_t)cols * 16 * wm * 4;
-        const size_t smem = std::max<size_t>((size_t)Q4_STAGES * Q4_STAGE_BYTES + 2 * (size_t)cols * xpitch, red);
+    for (int wm = 8, log_wk = 0; wm >= 1; wm /= 2, ++log_wk) {
+        const int64_t wk = Q4_WARPS / wm;
+        const size_t red = (size_t)Q4_WARPS * 16 * p.nt * 8 * 4 + (size_t)p.samples * 16 * wm * 4;
+        const size_t smem = std::max<size_t>(Q4_STAGES * (Q4_STAGE_BYTES + (size_t)cols * 64 * 8 * wk), red) + Q4_BARS;
         if (smem > 227 * 1024) continue;
-        const int64_t tiles = cdiv(K, 16 * wm) * z, stages = cdiv(C, Q4_SEG * wk);
-        const bool two = nt <= 2 && smem <= 113 * 1024;
-        for (int cl = 1; cl <= 16; cl *= 2) {
-            if (cl > 1 && cl > stages) break;
+        const int64_t tiles = cdiv(K, 16 * wm) * p.z, stages = cdiv(C, Q4_SEG * wk);
+        const bool two = p.nt <= 2 && smem <= 112 * 1024;
+        for (int cl = 1; cl <= 16 && (cl == 1 || cl <= stages); cl *= 2) {
             // SMs that hold two blocks share their bandwidth between them
             const double cost = (double)cdiv(tiles * cl, sms) * ((double)cdiv(stages, cl) + (two ? 1.5 : 3));
-            if (!best.wm || cost < least * 0.97) {
-                best = {wm, cl, xpitch, smem};
+            if (!p.wm || cost < least * 0.97) {
+                p.wm = wm;
+                p.log_wk = log_wk;
+                p.cluster = cl;
+                p.stages = (int)stages;
+                p.smem = smem;
+                p.xs_block = (int64_t)cols * 64 * 8 * wk * stages;
                 least = cost;
             }
         }
     }
-    return best;
+    return p;
+}
+
+// cuTensorMapEncodeTiled, which the driver hands out by name.
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+    static EncodeTiled f = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return (EncodeTiled)p;
+    }();
+    return f;
 }
 
 template <bool HALF, int NT, int GROUP>
-static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, dim3 grid, cudaStream_t st) {
+static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, dim3 grid, cudaStream_t st) {
     auto *f = k_q4_votes<HALF, NT, GROUP>;
     ytm_status rc;
     if ((rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem), "q4 votes smem")))
@@ -432,28 +502,30 @@ static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, dim3 grid, cudaStr
     cfg.blockDim = dim3(Q4_THREADS);
     cfg.dynamicSmemBytes = p.smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)p.cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)p.cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-    return cuda_check(cudaLaunchKernelEx(&cfg, f, a), "q4 votes");
+    cfg.numAttrs = p.cluster > 1 ? 2 : 1;
+    return cuda_check(cudaLaunchKernelEx(&cfg, f, a, map), "q4 votes");
 }
 
 template <bool HALF, int NT>
-static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, int group, dim3 grid, cudaStream_t st) {
-    if (group == 32) return launch_q4<HALF, NT, 32>(a, p, grid, st);
-    if (group == 64) return launch_q4<HALF, NT, 64>(a, p, grid, st);
-    return launch_q4<HALF, NT, 128>(a, p, grid, st);
+static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, int group, dim3 grid, cudaStream_t st) {
+    if (group == 32) return launch_q4<HALF, NT, 32>(a, p, map, grid, st);
+    if (group == 64) return launch_q4<HALF, NT, 64>(a, p, map, grid, st);
+    return launch_q4<HALF, NT, 128>(a, p, map, grid, st);
 }
 
 template <bool HALF>
-static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, int nt, int group, dim3 grid, cudaStream_t st) {
-    if (nt == 1) return launch_q4<HALF, 1>(a, p, group, grid, st);
-    if (nt == 2) return launch_q4<HALF, 2>(a, p, group, grid, st);
-    if (nt == 4) return launch_q4<HALF, 4>(a, p, group, grid, st);
-    return launch_q4<HALF, 8>(a, p, group, grid, st);
+static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, int group, dim3 grid, cudaStream_t st) {
+    if (p.nt == 1) return launch_q4<HALF, 1>(a, p, map, group, grid, st);
+    if (p.nt == 2) return launch_q4<HALF, 2>(a, p, map, group, grid, st);
+    if (p.nt == 4) return launch_q4<HALF, 4>(a, p, map, group, grid, st);
+    return launch_q4<HALF, 8>(a, p, map, group, grid, st);
 }
 
 static ytm_status check_q4(int32_t C, int32_t K, int32_t group, int32_t scale_type) {
@@ -494,9 +566,15 @@ ytm_status ytm_q4_pack(const void *weights, int32_t w_type, int64_t w_stride, in
     return launch_check("q4 pack");
 }
 
+uint64_t ytm_q4_votes_workspace_bytes(int32_t x_type, int64_t N, int32_t C, int32_t K) {
+    if (N <= 0 || C <= 0 || C > (1 << 30) || K <= 0) return 0;
+    const Q4Plan p = q4_plan(N, C, K, x_type);
+    return (uint64_t)p.z * p.xs_block;
+}
+
 ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t N, int32_t C, const uint8_t *packed,
                         const void *scales, int32_t scale_type, int32_t group, int32_t K, const float *bias, void *y,
-                        int32_t y_type, void *stream) {
+                        int32_t y_type, void *workspace, void *stream) {
     ytm_status rc = check_q4(C, K, group, scale_type);
     if (rc) return rc;
     if (N < 0) return fail(YTM_ERR_ARG, "N < 0");
@@ -504,23 +582,33 @@ ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t
     if (!is_float_type(y_type)) return fail(YTM_ERR_ARG, "q4: votes must be fp32, fp16 or bf16");
     if (x_stride < 0) return fail(YTM_ERR_ARG, "q4: negative row stride");
     if (N == 0) return YTM_OK;
-    if (!x || !packed || !scales || !y) return fail(YTM_ERR_ARG, "null pointer");
-    if ((uintptr_t)packed % 16) return fail(YTM_ERR_ARG, "q4: packed weights must start on a 16-byte boundary");
-    const int parts = x_type == YTM_F32 ? 3 : 1;
-    const int64_t most = 64 / parts;  // samples of a block
-    const int64_t z = std::min<int64_t>(cdiv(N, most), 65535);
-    // samples evenly over the blocks, in tiles of 8 columns
-    const int samples = (int)(N <= most ? N : most);
-    const int cols = samples * parts, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : cols <= 32 ? 4 : 8;
-    const Q4Plan p = q4_plan(C, K, nt, cols, z);
-    Q4Args a = {x, x_stride, 0, 0, packed, scales, bias, y, C, K, (int)cdiv(C, group), x_type, scale_type, y_type,
-                samples, p.wm, p.wm == 8 ? 0 : p.wm == 4 ? 1 : p.wm == 2 ? 2 : 3, p.cluster, p.xpitch};
-    for (int64_t i = 0; i < N; i += z * most) {
-        a.n0 = i;
-        a.n = std::min<int64_t>(N - i, z * most);
-        const dim3 grid((unsigned)(cdiv(K, 16 * p.wm) * p.cluster), 1, (unsigned)cdiv(a.n, most));
-        rc = x_type == YTM_F16 ? launch_q4<true>(a, p, nt, group, grid, as_stream(stream))
-                               : launch_q4<false>(a, p, nt, group, grid, as_stream(stream));
+    if (!x || !packed || !scales || !y || !workspace) return fail(YTM_ERR_ARG, "null pointer");
+    if ((uintptr_t)packed % 16 || (uintptr_t)workspace % 16)
+        return fail(YTM_ERR_ARG, "q4: packed weights and workspace must start on a 16-byte boundary");
+    cudaStream_t st = as_stream(stream);
+    const Q4Plan p = q4_plan(N, C, K, x_type);
+    // the weights as a matrix of bytes, tiles of 128 bytes by 16 WM classes; zeros outside
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {(cuuint64_t)q4_row_bytes(C), (cuuint64_t)K}, strides[1] = {(cuuint64_t)q4_row_bytes(C)};
+    const cuuint32_t box[2] = {128, (cuuint32_t)(16 * p.wm)}, step[2] = {1, 1};
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return fail(YTM_ERR_CUDA, "q4 votes: the driver has no cuTensorMapEncodeTiled");
+    if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)packed, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return fail(YTM_ERR_CUDA, "q4 votes: cuTensorMapEncodeTiled refused the weights");
+    const int64_t most = p.z * p.samples;  // samples of a launch
+    const int groups = p.stages * (8 << p.log_wk);
+    for (int64_t i = 0; i < N; i += most) {
+        const int64_t n = std::min(N - i, most);
+        const Q4XArgs xa = {x, x_stride, i, n, (char *)workspace, p.xs_block, C, x_type, p.samples, p.parts, groups};
+        const uint64_t blocks = cdiv((uint64_t)n * groups * 4, 256);
+        if (blocks > INT_MAX) return fail(YTM_ERR_UNSUPPORTED, "q4 votes: too many activations for one call");
+        k_q4_x<<<(unsigned)blocks, 256, 0, st>>>(xa);
+        if ((rc = launch_check("q4 activations"))) return rc;
+        const Q4Args a = {(const char *)workspace, scales, bias, y, i, n, p.xs_block, K, (int)cdiv(C, group), p.stages, scale_type,
+                          y_type, p.samples, p.parts, p.log_wk, p.cluster, (int)p.smem - Q4_BARS};
+        const dim3 grid((unsigned)(cdiv(K, 16 * p.wm) * p.cluster), 1, (unsigned)cdiv(n, p.samples));
+        rc = x_type == YTM_F16 ? launch_q4<true>(a, p, map, group, grid, st) : launch_q4<false>(a, p, map, group, grid, st);
         if (rc) return rc;
     }
     return YTM_OK;
