@@ -235,7 +235,7 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 }
 
 template <bool HALF, int NT, int GROUP>
-__global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const Q4Args a, const __grid_constant__ CUtensorMap weights) {
+__global__ void __launch_bounds__(Q4_THREADS, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_q4_votes(const Q4Args a, const __grid_constant__ CUtensorMap weights) {
     extern __shared__ __align__(1024) char smem[];  // weights, activations; barriers at the end
     uint64_t *const bars = (uint64_t *)(smem + a.bars_at);
     volatile int &failed = *(int *)(bars + 2 * Q4_STAGES);
@@ -301,25 +301,36 @@ __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const 
             if (bad) failed = 1;
         }
     } else {
-        // scales: lane t of a class holds groups t, t + 4, ... of a stage
+        // scales: lane t of a class holds groups t, t + 4, ... of a stage; the
+        // next stage's are on their way
         const int class0 = row0 + wm * 16 + g, class1 = class0 + 8;
-        const int64_t at0 = class0 < a.K ? (int64_t)class0 * a.G : 0, at1 = class1 < a.K ? (int64_t)class1 * a.G : 0;
         const bool wide = a.scale_type == YTM_F32;
-        const auto load_scales = [&](int s, uint32_t (&sc)[GPL][2]) {
+        const int group0 = (first * WK + wk) * GPS + t, group_step = WK * GPS;
+        const int bytes = wide ? 4 : 2;
+        const char *sc0 = (const char *)a.scales + ((class0 < a.K ? (int64_t)class0 * a.G : 0) + group0) * bytes;
+        const char *sc1 = (const char *)a.scales + ((class1 < a.K ? (int64_t)class1 * a.G : 0) + group0) * bytes;
+        int last[GPL];  // stages that have this lane's group (group0 + 4 j + s group_step < G)
+#pragma unroll
+        for (int j = 0; j < GPL; ++j) last[j] = (a.G - group0 - 4 * j + group_step - 1) / group_step;
+        uint32_t next_sc[GPL][2];
+        const auto load_scales = [&](int s) {
 #pragma unroll
             for (int j = 0; j < GPL; ++j) {
-                const int grp = min(((first + s) * WK + wk) * GPS + j * 4 + t, a.G - 1);
-                if (wide) {
-                    sc[j][0] = ((const uint32_t *)a.scales)[at0 + grp];
-                    sc[j][1] = ((const uint32_t *)a.scales)[at1 + grp];
-                } else {
-                    sc[j][0] = ((const uint16_t *)a.scales)[at0 + grp];
-                    sc[j][1] = ((const uint16_t *)a.scales)[at1 + grp];
+                next_sc[j][0] = next_sc[j][1] = 0u;  // behind the last group: 0
+                if (s < last[j]) {
+                    if (wide) {
+                        next_sc[j][0] = *(const uint32_t *)(sc0 + 16 * j);
+                        next_sc[j][1] = *(const uint32_t *)(sc1 + 16 * j);
+                    } else {
+                        next_sc[j][0] = *(const uint16_t *)(sc0 + 8 * j);
+                        next_sc[j][1] = *(const uint16_t *)(sc1 + 8 * j);
+                    }
                 }
             }
+            sc0 += group_step * bytes;
+            sc1 += group_step * bytes;
         };
-        uint32_t next_sc[GPL][2];
-        load_scales(0, next_sc);
+        load_scales(0);
         int x_col[NT];  // columns behind the last are the last once more; nobody reads their sums
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -334,11 +345,10 @@ __global__ void __launch_bounds__(Q4_THREADS, NT <= 2 ? 2 : 1) k_q4_votes(const 
             float sc[GPL][2];
 #pragma unroll
             for (int j = 0; j < GPL; ++j) {
-                const bool there = ((first + s) * WK + wk) * GPS + j * 4 + t < a.G;  // behind the last group: 0
-                sc[j][0] = there ? scale_value(next_sc[j][0], a.scale_type) : 0.f;
-                sc[j][1] = there ? scale_value(next_sc[j][1], a.scale_type) : 0.f;
+                sc[j][0] = scale_value(next_sc[j][0], a.scale_type);
+                sc[j][1] = scale_value(next_sc[j][1], a.scale_type);
             }
-            load_scales(s + 1, next_sc);
+            load_scales(s + 1);
             if (!__all_sync(0xFFFFFFFFu, bar_wait(full + 8 * (s % Q4_STAGES), (s / Q4_STAGES) & 1))) {
                 if (lane == 0) failed = 1;
                 break;
