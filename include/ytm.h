@@ -386,7 +386,7 @@ ytm_status ytm_q4_pack(const void *weights, int32_t w_type, int64_t w_stride, in
 ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t N, int32_t C, const uint8_t *packed,
                         const void *scales, int32_t scale_type, int32_t group, int32_t K, const float *bias, void *y,
                         int32_t y_type, void *workspace, void *stream);
-uint64_t ytm_q4_votes_workspace_bytes(int32_t x_type, int64_t N, int32_t C, int32_t K);
+uint64_t ytm_q4_votes_workspace_bytes(int32_t x_type, int64_t N, int32_t C, int32_t K, int32_t group);
 
 /* Fired clauses of inference as bits u32 [N][ceil(C / 32)] (bits behind the
  * last clause 0): the clauses ytm_infer counts, i.e. without those that

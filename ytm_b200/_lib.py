@@ -124,7 +124,7 @@ _SIGS = {
     "ytm_peer_ar_destroy": ([_P], ct.c_int),
     "ytm_q4_pack": ([_P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I32, _P], ct.c_int),
     "ytm_q4_votes": ([_P, _I32, _I64, _I64, _I32, _P, _P, _I32, _I32, _I32, _P, _P, _I32, _P, _P], ct.c_int),
-    "ytm_q4_votes_workspace_bytes": ([_I32, _I64, _I32, _I32], _U64),
+    "ytm_q4_votes_workspace_bytes": ([_I32, _I64, _I32, _I32, _I32], _U64),
     "ytm_infer_fired": ([_CFG, _P, _P, _I64, _P, _P, _P], ct.c_int),
     "ytm_answer": ([ct.POINTER(AnswerArgs), _P], ct.c_int),
     "ytm_class_loss": ([ct.POINTER(LossArgs), _P, _P], ct.c_int),

@@ -160,7 +160,7 @@ def q4_votes(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group:
         return y
     lib, x_type = _lib.load(), _lib.YTM_BITS if bits else _TYPES[x.dtype]
     with _on(dev):
-        ws = torch.empty(lib.ytm_q4_votes_workspace_bytes(x_type, n, clauses, K), dtype=torch.uint8, device=dev)
+        ws = torch.empty(lib.ytm_q4_votes_workspace_bytes(x_type, n, clauses, K, group), dtype=torch.uint8, device=dev)
         check(lib.ytm_q4_votes(x.data_ptr(), x_type, _row_stride(x), n, clauses, packed.data_ptr(), scales.data_ptr(),
                                _TYPES[scales.dtype], group, K, None if bias is None else bias.data_ptr(), y.data_ptr(),
                                _TYPES[out_dtype], ws.data_ptr(), _stream(dev)), "ytm_q4_votes")

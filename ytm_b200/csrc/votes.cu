@@ -49,17 +49,24 @@ __global__ void k_q4_pack(const T *__restrict__ w, int64_t w_stride, int C, int 
 // The weights' bytes bound the call while there are few samples, so they are
 // what streams: one thread of a block copies 16 KB of them a stage into shared
 // memory by TMA, four stages deep, and each of eight warps multiplies 16
-// classes by 256 clauses of a stage on the tensor cores (m16n8k16, fp32 sums).
-// ldmatrix hands lane (g, t) word t of 32 clauses of classes g and g + 8, i.e.
-// eight 4-bit weights, which the lane turns into bf16 or fp16 pairs (clauses i
-// and i + 4) by or-ing them into the fraction of 128 (1024) and subtracting
-// 136 (1032): exact.  The sum of a group is exact up to the fp32 additions; its
-// scale is applied in fp32.
+// classes by 256 clauses of a stage on the tensor cores.  ldmatrix hands lane
+// (g, t) word t of 32 clauses of classes g and g + 8, i.e. eight 4-bit weights.
+// What is done with a word decides the speed, as it is done for every 4 bytes:
 //
-// k_q4_x lays the activations out before: in that order of clauses, group by
-// group of 32, so that a stage's are one piece of memory.  Activations in fp32
-// take three columns, their leading, middle and last 8 bits, which are bf16
-// values exactly; clause bits are bf16 zeros and ones.
+// - whole numbers (m16n8k32): two masks and a shift make the word's low and high
+//   halves of the bytes two registers of unsigned bytes, an operand as they are.
+//   Clause bits are the other operand; real activations become four signed
+//   bytes, x = (d0 2^24 + d1 2^16 + d2 2^8 + d3) 2^e with e of the largest of 128
+//   neighbours, i.e. x to 2^-30 of that one, in four columns.  The 8 that the
+//   weights are offset by goes into the sums' start, -8 times the sum of a
+//   group's digits.  Sums of a group are exact.
+// - 16-bit products (m16n8k16), for more than eight 16-bit samples, whose four
+//   columns would cost more products than they save: the word becomes four pairs
+//   (clauses i and i + 4) by or-ing it into the fraction of 128 (fp16: 1024) and
+//   subtracting 136 (1032), exactly.
+//
+// A group's sum is scaled in fp32.  k_q4_x lays the activations out before, in
+// pieces of 256 clauses, so that a stage's are one piece of memory.
 //
 // WM of a block's 8 warps lie along the classes, 8 / WM along the clauses, and
 // up to 16 blocks of a cluster along the clauses, which add their sums through
@@ -67,14 +74,24 @@ __global__ void k_q4_pack(const T *__restrict__ w, int64_t w_stride, int C, int 
 
 namespace cg = cooperative_groups;
 
+enum Q4Mode { Q4_BITS, Q4_DIGITS, Q4_BF16, Q4_FP16 };
+
 constexpr int Q4_WARPS = 8, Q4_THREADS = 32 * (Q4_WARPS + 1);  // the last warp copies
 constexpr int Q4_STAGES = 4;
 constexpr int Q4_SEG = 256;                        // clauses of a warp in a stage: 128 bytes of a class
 constexpr int Q4_STAGE_BYTES = Q4_WARPS * 16 * 128;
 constexpr int Q4_BARS = 128;                       // bytes of the barriers and the failure flag
 
+// Bytes of 256 clauses of `cols` columns.  16-bit: [32 clauses][column][64].
+// Whole numbers: digits [64 clauses][column][t][2 groups of 32][even 4, odd 4],
+// the sums' starts i32 [group][column], and for real activations the factors
+// f32 [128 clauses][column].
+__host__ __device__ constexpr int q4_seg_bytes(Q4Mode mode, int cols, int group) {
+    return mode >= Q4_BF16 ? cols * 512 : cols * (256 + Q4_SEG / group * 4 + (mode == Q4_DIGITS ? 8 : 0));
+}
+
 struct Q4Args {
-    const char *xs;           // k_q4_x's activations: [block of samples][group of 32][column][64 bytes]
+    const char *xs;           // k_q4_x's activations: [block of samples][256 clauses][q4_seg_bytes]
     const void *scales;
     const float *bias;
     void *y;
@@ -92,74 +109,127 @@ struct Q4XArgs {
     int64_t x_stride, n0, n;
     char *xs;
     int64_t xs_block;
-    int C, x_type, samples, parts, groups;
+    int C, x_type, samples, parts, cols, segs, group;
 };
 
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {  // of values that bf16 holds
-    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
-}
-
-// A thread takes 8 clauses of a sample and writes them in the order (0, 4, 1,
-// 5, 2, 6, 3, 7).  Within the 64 bytes of a (group, column) the four 16-byte
-// pieces are exchanged by the column's bits 1 and 2, so that the eight lanes
-// that read two columns together meet 32 different banks.
-__global__ void __launch_bounds__(256) k_q4_x(const Q4XArgs a) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int octets = a.groups * 4;
-    const int64_t i = u / octets;  // sample of this launch
-    if (i >= a.n) return;
-    const int o = (int)(u - i * octets), c = o * 8;
-    const int64_t row = (a.n0 + i) * a.x_stride;
-    const int col = (int)(i % a.samples) * a.parts;
-    char *const base = a.xs + i / a.samples * a.xs_block + (int64_t)(o >> 2) * a.samples * a.parts * 64;
-    const auto put = [&](int part, uint4 v) {
-        const int k = col + part;
-        *(uint4 *)(base + k * 64 + ((o & 3) ^ (k >> 1 & 3)) * 16) = v;
-    };
-    if (a.x_type == YTM_BITS) {
-        uint32_t w = c < a.C ? ((const uint32_t *)a.x)[row + (c >> 5)] >> (c & 31) & 255u : 0u;
-        if (c < a.C && c + 8 > a.C) w &= (1u << (a.C - c)) - 1u;
-        uint32_t v[4];
+// Clauses c .. c + 7 of a row (0 behind the last clause) as fp32.
+__device__ __forceinline__ void load_octet(const Q4XArgs &a, int64_t row, int c, float (&v)[8]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = ((w >> j) & 1u) * 0x3F80u | ((w >> (j + 4)) & 1u) * 0x3F800000u;
-        put(0, make_uint4(v[0], v[1], v[2], v[3]));
-    } else if (a.x_type == YTM_F32) {
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    if (a.x_type == YTM_F32) {
         const float *p = (const float *)a.x + row + c;
-        float rest[8];
         if (c + 8 <= a.C && (uintptr_t)p % 16 == 0) {
-            *(float4 *)&rest[0] = *(const float4 *)p;
-            *(float4 *)&rest[4] = *(const float4 *)(p + 4);
+            *(float4 *)&v[0] = *(const float4 *)p;
+            *(float4 *)&v[4] = *(const float4 *)(p + 4);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) rest[j] = c + j < a.C ? p[j] : 0.f;
-        }
-#pragma unroll
-        for (int part = 0; part < 3; ++part) {
-            float top[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {  // the leading 8 bits; NaN stays NaN, infinity leaves nothing
-                top[j] = __uint_as_float(__float_as_uint(rest[j]) & 0xFFFF0000u);
-                if (part == 0 && rest[j] != rest[j]) top[j] = __uint_as_float(0x7FC00000u);
-                rest[j] = part == 0 && !(fabsf(rest[j]) < INFINITY) ? 0.f : rest[j] - top[j];
-            }
-            put(part, make_uint4(bf16_pair(top[0], top[4]), bf16_pair(top[1], top[5]), bf16_pair(top[2], top[6]),
-                                 bf16_pair(top[3], top[7])));
+            for (int j = 0; j < 8; ++j)
+                if (c + j < a.C) v[j] = p[j];
         }
     } else {
         const uint16_t *p = (const uint16_t *)a.x + row + c;
-        uint4 v = make_uint4(0, 0, 0, 0);
+        uint32_t w[4] = {0, 0, 0, 0};
         if (c + 8 <= a.C && (uintptr_t)p % 16 == 0) {
-            v = *(const uint4 *)p;
+            *(uint4 *)w = *(const uint4 *)p;
         } else {
-            uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (c + j < a.C) w[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
-            v = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        put(0, make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                          __byte_perm(v.y, v.w, 0x7632)));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t h = w[j / 2] >> (16 * (j & 1)) & 0xFFFFu;
+            v[j] = a.x_type == YTM_F16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16);
+        }
+    }
+}
+
+// A thread takes 8 clauses of a sample, 16 neighbours 128 clauses.
+template <Q4Mode MODE>
+__global__ void __launch_bounds__(256) k_q4_x(const Q4XArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int octets = a.segs * 32;
+    const int64_t i = u / octets;  // sample of this launch: one for a warp
+    if (i >= a.n) return;
+    const int o = (int)(u - i * octets), c = o * 8, in_seg = o & 31;
+    const int64_t row = (a.n0 + i) * a.x_stride;
+    const int col = (int)(i % a.samples) * a.parts;
+    char *const seg = a.xs + i / a.samples * a.xs_block + (int64_t)(o >> 5) * q4_seg_bytes(MODE, a.cols, a.group);
+    if (MODE >= Q4_BF16) {
+        // order (0, 4, 1, 5, 2, 6, 3, 7); the four 16-byte pieces of a (group,
+        // column) are exchanged by the column's bits 1 and 2, so that the eight
+        // lanes that read two columns together meet 32 different banks
+        const uint16_t *p = (const uint16_t *)a.x + row + c;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (c + 8 <= a.C && (uintptr_t)p % 16 == 0) {
+            *(uint4 *)w = *(const uint4 *)p;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < a.C) w[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
+        }
+        *(uint4 *)(seg + ((in_seg >> 2) * a.cols + col) * 64 + ((o & 3) ^ (col >> 1 & 3)) * 16) =
+            make_uint4(__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x5410),
+                       __byte_perm(w[1], w[3], 0x7632));
+        return;
+    }
+    char *const digits = seg + ((in_seg >> 3) * a.cols + col) * 64 + (o & 3) * 16 + (in_seg >> 2 & 1) * 8;
+    int *const starts = (int *)(seg + a.cols * 256) + in_seg * 8 / a.group * a.cols + col;
+    const int lanes = a.group / 8;  // of a group
+    const bool lead = (in_seg & (lanes - 1)) == 0;
+    const auto start = [&](int part, int sum) {
+        for (int d = lanes / 2; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        if (lead) starts[part] = -8 * sum;
+    };
+    if (MODE == Q4_BITS) {
+        uint32_t w = c < a.C ? ((const uint32_t *)a.x)[row + (c >> 5)] >> (c & 31) & 255u : 0u;
+        if (c < a.C && c + 8 > a.C) w &= (1u << (a.C - c)) - 1u;
+        const auto spread = [](uint32_t v) { return (v & 1u) | (v & 4u) << 6 | (v & 16u) << 12 | (v & 64u) << 18; };
+        *(uint2 *)digits = make_uint2(spread(w), spread(w >> 1));
+        start(0, __popc(w));
+        return;
+    }
+    float v[8], top = 0.f;
+    load_octet(a, row, c, v);
+    bool nan = false;
+    int infs = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        nan |= v[j] != v[j];
+        infs += fabsf(v[j]) == INFINITY;
+        top = fmaxf(top, fabsf(v[j]));
+    }
+    for (int d = 8; d; d >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+        nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, d);
+        infs += __shfl_xor_sync(0xFFFFFFFFu, infs, d);
+    }
+    // top < 2^(e + 1): |x| 2^(29 - e) < 2^30.  An infinity among the 128 becomes
+    // the digit 1 of an infinite factor and the others 0; several of them, whose
+    // signs would have to be told apart class by class, give NaN.
+    const int e = (int)(__float_as_uint(top) >> 23) - 127;
+    uint32_t even[4] = {0, 0, 0, 0}, odd[4] = {0, 0, 0, 0};
+    int sums[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        int X = infs ? (fabsf(v[j]) == INFINITY ? (v[j] > 0.f ? 1 << 24 : -(1 << 24)) : 0) : __float2int_rn(scalbnf(v[j], 29 - e));
+        if (nan) X = 0;
+#pragma unroll
+        for (int part = 3; part >= 0; --part) {
+            const int d = part ? (int)(int8_t)(X & 255) : X;
+            X = (X - d) >> 8;
+            sums[part] += d;
+            (j & 1 ? odd : even)[part] |= (uint32_t)(d & 255) << (8 * (j / 2));
+        }
+    }
+    float *const factors = (float *)(seg + a.cols * (256 + Q4_SEG / a.group * 4)) + (in_seg >> 4) * a.cols + col;
+#pragma unroll
+    for (int part = 0; part < 4; ++part) {
+        *(uint2 *)(digits + part * 64) = make_uint2(even[part], odd[part]);
+        start(part, sums[part]);
+        if ((in_seg & 15) == 0)
+            factors[part] = nan || infs > 1 ? NAN : infs ? (part ? 0.f : INFINITY) : scalbnf(1.f, e - 5 - 8 * part);
     }
 }
 
@@ -180,20 +250,22 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok;
 }
-__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity) {
+__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volatile int &failed) {
     uint64_t start, now;
+    if (failed) return false;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(start));
     for (int i = 0; i < (1 << 24); ++i) {
         if (bar_try(bar, parity)) return true;
         asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
         if (now - start > 2000000000ull) break;
     }
+    failed = 1;
     return false;
 }
-// Waits for the phase with this parity; false if it did not come within about
-// two seconds.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-    return bar_try(bar, parity) || bar_wait_long(bar, parity);
+// Waits for the phase with this parity; false, and `failed` set, if it did not
+// come within about two seconds, and at once after that.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int &failed) {
+    return bar_try(bar, parity) || bar_wait_long(bar, parity, failed);
 }
 
 __device__ __forceinline__ float scale_value(uint32_t raw, int type) {
@@ -224,6 +296,14 @@ __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&p)[4]) {
     }
 }
 
+// Unsigned by signed bytes; `from`: the sums' start.
+__device__ __forceinline__ void mma_int(int (&d)[4], const int (&from)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(from[0]), "r"(from[1]), "r"(from[2]), "r"(from[3]));
+}
+
 template <bool HALF>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if (HALF)
@@ -234,8 +314,10 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <bool HALF, int NT, int GROUP>
-__global__ void __launch_bounds__(Q4_THREADS, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_q4_votes(const Q4Args a, const __grid_constant__ CUtensorMap weights) {
+// COLS: the columns of a block, padded to a multiple of 8.
+template <Q4Mode MODE, int COLS, int GROUP>
+__global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS == 16 ? 2 : 1) k_q4_votes(const Q4Args a, const __grid_constant__ CUtensorMap weights) {
+    constexpr int NT = COLS / 8, SEG_BYTES = q4_seg_bytes(MODE, COLS, GROUP);
     extern __shared__ __align__(1024) char smem[];  // weights, activations; barriers at the end
     uint64_t *const bars = (uint64_t *)(smem + a.bars_at);
     volatile int &failed = *(int *)(bars + 2 * Q4_STAGES);
@@ -246,8 +328,7 @@ __global__ void __launch_bounds__(Q4_THREADS, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_q
     // this block's stages of the clauses: WK segments each
     const int per = (a.stages + a.cluster - 1) / a.cluster;
     const int first = min(rank * per, a.stages), count = min(first + per, a.stages) - first;
-    const int cols = a.samples * a.parts;
-    const int x_bytes = cols * 64 * (Q4_SEG / 32) * WK;  // of a stage
+    const int x_bytes = SEG_BYTES * WK;  // of a stage
     char *const xs = smem + Q4_STAGES * Q4_STAGE_BYTES;
     const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem);
     const uint32_t full = (uint32_t)__cvta_generic_to_shared(bars), empty = full + 8 * Q4_STAGES;
@@ -271,7 +352,6 @@ __global__ void __launch_bounds__(Q4_THREADS, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_q
 
     if (warp == Q4_WARPS) {
         if (lane == 0) {
-            bool bad = false;
             const char *const x0 = a.xs + blockIdx.z * a.xs_block + (int64_t)first * x_bytes;
             const auto copy_weights = [&](int s) {
                 const uint32_t at = smem_at + (s % Q4_STAGES) * Q4_STAGE_BYTES, bar = full + 8 * (s % Q4_STAGES);
@@ -291,14 +371,10 @@ __global__ void __launch_bounds__(Q4_THREADS, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_q
             asm volatile("griddepcontrol.wait;" ::: "memory");
             for (int s = 0; s < min(count, Q4_STAGES); ++s) copy_x(s);
             for (int s = Q4_STAGES; s < count; ++s) {
-                if (!bar_wait(empty + 8 * (s % Q4_STAGES), (s / Q4_STAGES - 1) & 1)) {
-                    bad = true;
-                    break;
-                }
+                if (!bar_wait(empty + 8 * (s % Q4_STAGES), (s / Q4_STAGES - 1) & 1, failed)) break;
                 copy_weights(s);
                 copy_x(s);
             }
-            if (bad) failed = 1;
         }
     } else {
         // scales: lane t of a class holds groups t, t + 4, ... of a stage; the
@@ -331,13 +407,6 @@ __global__ void __launch_bounds__(Q4_THREADS, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_q
             sc1 += group_step * bytes;
         };
         load_scales(0);
-        int x_col[NT];  // columns behind the last are the last once more; nobody reads their sums
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int k = min(n * 8 + g, cols - 1);
-            x_col[n] = k * 64 + (t ^ (k >> 1 & 3)) * 16;
-        }
-        const int x_group = cols * 64;
         // rows of 128 bytes, their 16-byte pieces exchanged by the row's low bits (128-byte swizzle)
         const int mrow = (lane >> 3 & 1) * 8 + (lane & 7);
         const uint32_t mat = smem_at + (wk * WM + wm) * 2048 + mrow * 128;
@@ -349,47 +418,108 @@ __global__ void __launch_bounds__(Q4_THREADS, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_q
                 sc[j][1] = scale_value(next_sc[j][1], a.scale_type);
             }
             load_scales(s + 1);
-            if (!__all_sync(0xFFFFFFFFu, bar_wait(full + 8 * (s % Q4_STAGES), (s / Q4_STAGES) & 1))) {
-                if (lane == 0) failed = 1;
-                break;
-            }
+            bar_wait(full + 8 * (s % Q4_STAGES), (s / Q4_STAGES) & 1, failed);
+            __syncwarp();
             const uint32_t w_at = mat + (s % Q4_STAGES) * Q4_STAGE_BYTES;
-            const char *x_at = xs + (s % Q4_STAGES) * x_bytes + wk * (Q4_SEG / 32) * x_group;
-            float acc[NT][4];
-#pragma unroll
-            for (int j2 = 0; j2 < Q4_SEG / 64; ++j2) {
-                uint32_t q[4];
+            const char *x_at = xs + (s % Q4_STAGES) * x_bytes + wk * SEG_BYTES;
+            const auto words = [&](int j2, uint32_t (&q)[4]) {  // 64 clauses: classes g, g + 8 of the first 32, then of the others
                 asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                              : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
                              : "r"(w_at + (((j2 * 2 + (lane >> 4)) ^ (lane & 7)) * 16)));
+            };
+            const auto scales_of = [&](int grp, float &s0, float &s1) {
+                const int from = (lane & ~3) | (grp & 3);
+                s0 = __shfl_sync(0xFFFFFFFFu, sc[grp / 4][0], from);
+                s1 = __shfl_sync(0xFFFFFFFFu, sc[grp / 4][1], from);
+            };
+            if constexpr (MODE <= Q4_DIGITS) {
+                const int *starts = (const int *)(x_at + COLS * 256) + t * 2;
+                const float *factors = (const float *)(x_at + COLS * (256 + GPS * 4)) + t * 2;
+                constexpr bool SPLIT = MODE == Q4_DIGITS && GROUP < 128;  // several scales under one factor
+                int acc[NT][4];
+                float sum[SPLIT ? NT : 1][4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int j = j2 * 2 + h;  // 32 clauses
-                    if (j % (GROUP / 32) == 0) {
+                for (int j2 = 0; j2 < Q4_SEG / 64; ++j2) {
+                    uint32_t q[4];
+                    words(j2, q);
+                    uint4 b[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) b[n] = *(const uint4 *)(x_at + (j2 * COLS + n * 8 + g) * 64 + t * 16);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int j = j2 * 2 + h, grp = j / (GROUP / 32);  // 32 clauses
+                        const uint32_t a0 = q[2 * h] & 0x0F0F0F0Fu, a1 = q[2 * h + 1] & 0x0F0F0F0Fu;
+                        const uint32_t a2 = q[2 * h] >> 4 & 0x0F0F0F0Fu, a3 = q[2 * h + 1] >> 4 & 0x0F0F0F0Fu;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const uint32_t b0 = h ? b[n].z : b[n].x, b1 = h ? b[n].w : b[n].y;
+                            if (j % (GROUP / 32) == 0) {
+                                const int2 c = *(const int2 *)(starts + grp * COLS + n * 8);
+                                const int from[4] = {c.x, c.y, c.x, c.y};
+                                mma_int(acc[n], from, a0, a1, a2, a3, b0, b1);
+                            } else {
+                                mma_int(acc[n], acc[n], a0, a1, a2, a3, b0, b1);
+                            }
+                        }
+                        if ((j + 1) % (GROUP / 32)) continue;
+                        float s0, s1;
+                        scales_of(grp, s0, s1);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            if constexpr (SPLIT) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    sum[n][i] = fmaf(i < 2 ? s0 : s1, (float)acc[n][i], j % 4 == GROUP / 32 - 1 ? 0.f : sum[n][i]);
+                                if (j % 4 == 3) {
+                                    const float2 f = *(const float2 *)(factors + j / 4 * COLS + n * 8);
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) tot[n][i] = fmaf(i & 1 ? f.y : f.x, sum[n][i], tot[n][i]);
+                                }
+                            } else if constexpr (MODE == Q4_DIGITS) {
+                                const float2 f = *(const float2 *)(factors + j / 4 * COLS + n * 8);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    tot[n][i] = fmaf((i & 1 ? f.y : f.x), (i < 2 ? s0 : s1) * (float)acc[n][i], tot[n][i]);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) tot[n][i] = fmaf(i < 2 ? s0 : s1, (float)acc[n][i], tot[n][i]);
+                            }
+                        }
+                    }
+                }
+            } else {
+                constexpr bool HALF = MODE == Q4_FP16;
+                const char *x_lane = x_at + g * 64 + (t ^ (g >> 1 & 3)) * 16;
+                float acc[NT][4];
+#pragma unroll
+                for (int j2 = 0; j2 < Q4_SEG / 64; ++j2) {
+                    uint32_t q[4];
+                    words(j2, q);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int j = j2 * 2 + h;  // 32 clauses
+                        if (j % (GROUP / 32) == 0) {
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+                        }
+                        uint32_t lo[4], hi[4];
+                        unpack<HALF>(q[2 * h], lo);
+                        unpack<HALF>(q[2 * h + 1], hi);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const uint4 b = *(const uint4 *)(x_lane + (j * COLS + n * 8) * 64);
+                            mma<HALF>(acc[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
+                            mma<HALF>(acc[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
+                        }
+                        if ((j + 1) % (GROUP / 32)) continue;
+                        float s0, s1;
+                        scales_of(j / (GROUP / 32), s0, s1);
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-                    }
-                    uint32_t lo[4], hi[4];
-                    unpack<HALF>(q[2 * h], lo);
-                    unpack<HALF>(q[2 * h + 1], hi);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const uint4 b = *(const uint4 *)(x_at + x_col[n] + j * x_group);
-                        mma<HALF>(acc[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
-                        mma<HALF>(acc[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
-                    }
-                    if ((j + 1) % (GROUP / 32) == 0) {
-                        const int grp = j / (GROUP / 32), from = (lane & ~3) | (grp & 3);
-                        const float s0 = __shfl_sync(0xFFFFFFFFu, sc[grp / 4][0], from), s1 = __shfl_sync(0xFFFFFFFFu, sc[grp / 4][1], from);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            tot[n][0] = fmaf(s0, acc[n][0], tot[n][0]);
-                            tot[n][1] = fmaf(s0, acc[n][1], tot[n][1]);
-                            tot[n][2] = fmaf(s1, acc[n][2], tot[n][2]);
-                            tot[n][3] = fmaf(s1, acc[n][3], tot[n][3]);
-                        }
+                            for (int i = 0; i < 4; ++i) tot[n][i] = fmaf(i < 2 ? s0 : s1, acc[n][i], tot[n][i]);
                     }
                 }
             }
@@ -399,7 +529,6 @@ __global__ void __launch_bounds__(Q4_THREADS, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_q
     }
     __syncthreads();  // all stages have been read
     // sums of the warps along the clauses and of the parts of an activation
-    constexpr int COLS = NT * 8;
     float *red = (float *)smem;                      // [warp][16][COLS]
     float *mine = red + Q4_WARPS * 16 * COLS;        // [samples][16 * WM]
     if (warp < Q4_WARPS) {
@@ -443,29 +572,32 @@ __global__ void __launch_bounds__(Q4_THREADS, NT == 1 ? 3 : NT == 2 ? 2 : 1) k_q
 // busiest SM times the stages of a block plus about three for its start and its
 // end, half of which a second block on the SM hides.
 struct Q4Plan {
-    int nt, samples, parts;  // of a block
+    Q4Mode mode;
+    int cols, samples, parts;  // of a block (columns padded); columns of a sample
     int wm, log_wk, cluster, stages;
-    int64_t z, xs_block;     // blocks of samples of a launch, bytes of one's activations
+    int64_t z, xs_block;       // blocks of samples of a launch, bytes of one's activations
     size_t smem;
 };
 
-static Q4Plan q4_plan(int64_t N, int64_t C, int64_t K, int x_type) {
+static Q4Plan q4_plan(int64_t N, int64_t C, int64_t K, int x_type, int group) {
     Q4Plan p = {};
-    p.parts = x_type == YTM_F32 ? 3 : 1;
+    p.mode = x_type == YTM_BITS ? Q4_BITS : x_type == YTM_F32 || N <= 8 ? Q4_DIGITS : x_type == YTM_F16 ? Q4_FP16 : Q4_BF16;
+    p.parts = p.mode == Q4_DIGITS ? 4 : 1;
     const int64_t most = 64 / p.parts;
     p.samples = (int)std::min(N, most);
     p.z = std::min<int64_t>(cdiv(N, most), 65535);
-    const int cols = p.samples * p.parts;
-    p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : cols <= 32 ? 4 : 8;
+    const int used = p.samples * p.parts;
+    p.cols = used <= 8 ? 8 : used <= 16 ? 16 : used <= 32 ? 32 : used <= 48 ? 48 : 64;
+    const int seg_bytes = q4_seg_bytes(p.mode, p.cols, group);
     double least = 0;
     const int64_t sms = sm_count();
     for (int wm = 8, log_wk = 0; wm >= 1; wm /= 2, ++log_wk) {
         const int64_t wk = Q4_WARPS / wm;
-        const size_t red = (size_t)Q4_WARPS * 16 * p.nt * 8 * 4 + (size_t)p.samples * 16 * wm * 4;
-        const size_t smem = std::max<size_t>(Q4_STAGES * (Q4_STAGE_BYTES + (size_t)cols * 64 * 8 * wk), red) + Q4_BARS;
+        const size_t red = (size_t)Q4_WARPS * 16 * p.cols * 4 + (size_t)p.samples * 16 * wm * 4;
+        const size_t smem = std::max<size_t>(Q4_STAGES * (Q4_STAGE_BYTES + (size_t)seg_bytes * wk), red) + Q4_BARS;
         if (smem > 227 * 1024) continue;
         const int64_t tiles = cdiv(K, 16 * wm) * p.z, stages = cdiv(C, Q4_SEG * wk);
-        const bool two = p.nt <= 2 && smem <= 112 * 1024;
+        const bool two = p.cols <= 16 && smem <= 112 * 1024;
         for (int cl = 1; cl <= 16 && (cl == 1 || cl <= stages); cl *= 2) {
             // SMs that hold two blocks share their bandwidth between them
             const double cost = (double)cdiv(tiles * cl, sms) * ((double)cdiv(stages, cl) + (two ? 1.5 : 3));
@@ -475,7 +607,7 @@ static Q4Plan q4_plan(int64_t N, int64_t C, int64_t K, int x_type) {
                 p.cluster = cl;
                 p.stages = (int)stages;
                 p.smem = smem;
-                p.xs_block = (int64_t)cols * 64 * 8 * wk * stages;
+                p.xs_block = (int64_t)seg_bytes * wk * stages;
                 least = cost;
             }
         }
@@ -499,9 +631,9 @@ static EncodeTiled encode_tiled() {
     return f;
 }
 
-template <bool HALF, int NT, int GROUP>
+template <Q4Mode MODE, int COLS, int GROUP>
 static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, dim3 grid, cudaStream_t st) {
-    auto *f = k_q4_votes<HALF, NT, GROUP>;
+    auto *f = k_q4_votes<MODE, COLS, GROUP>;
     ytm_status rc;
     if ((rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem), "q4 votes smem")))
         return rc;
@@ -523,19 +655,27 @@ static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap 
     return cuda_check(cudaLaunchKernelEx(&cfg, f, a, map), "q4 votes");
 }
 
-template <bool HALF, int NT>
+template <Q4Mode MODE, int COLS>
 static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, int group, dim3 grid, cudaStream_t st) {
-    if (group == 32) return launch_q4<HALF, NT, 32>(a, p, map, grid, st);
-    if (group == 64) return launch_q4<HALF, NT, 64>(a, p, map, grid, st);
-    return launch_q4<HALF, NT, 128>(a, p, map, grid, st);
+    if (group == 32) return launch_q4<MODE, COLS, 32>(a, p, map, grid, st);
+    if (group == 64) return launch_q4<MODE, COLS, 64>(a, p, map, grid, st);
+    return launch_q4<MODE, COLS, 128>(a, p, map, grid, st);
 }
 
-template <bool HALF>
-static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, int group, dim3 grid, cudaStream_t st) {
-    if (p.nt == 1) return launch_q4<HALF, 1>(a, p, map, group, grid, st);
-    if (p.nt == 2) return launch_q4<HALF, 2>(a, p, map, group, grid, st);
-    if (p.nt == 4) return launch_q4<HALF, 4>(a, p, map, group, grid, st);
-    return launch_q4<HALF, 8>(a, p, map, group, grid, st);
+template <Q4Mode MODE>
+static ytm_status launch_q4(const Q4XArgs &xa, unsigned x_blocks, const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, int group,
+                            dim3 grid, cudaStream_t st) {
+    k_q4_x<MODE><<<x_blocks, 256, 0, st>>>(xa);
+    ytm_status rc = launch_check("q4 activations");
+    if (rc) return rc;
+    switch (p.cols) {
+        case 8:  // more than eight samples of 16 bits take 16 columns and more
+            if constexpr (MODE <= Q4_DIGITS) return launch_q4<MODE, 8>(a, p, map, group, grid, st);
+        case 16: return launch_q4<MODE, 16>(a, p, map, group, grid, st);
+        case 32: return launch_q4<MODE, 32>(a, p, map, group, grid, st);
+        case 48: return launch_q4<MODE, 48>(a, p, map, group, grid, st);
+        default: return launch_q4<MODE, 64>(a, p, map, group, grid, st);
+    }
 }
 
 static ytm_status check_q4(int32_t C, int32_t K, int32_t group, int32_t scale_type) {
@@ -576,9 +716,9 @@ ytm_status ytm_q4_pack(const void *weights, int32_t w_type, int64_t w_stride, in
     return launch_check("q4 pack");
 }
 
-uint64_t ytm_q4_votes_workspace_bytes(int32_t x_type, int64_t N, int32_t C, int32_t K) {
-    if (N <= 0 || C <= 0 || C > (1 << 30) || K <= 0) return 0;
-    const Q4Plan p = q4_plan(N, C, K, x_type);
+uint64_t ytm_q4_votes_workspace_bytes(int32_t x_type, int64_t N, int32_t C, int32_t K, int32_t group) {
+    if (N <= 0 || check_q4(C, K, group, YTM_F32)) return 0;
+    const Q4Plan p = q4_plan(N, C, K, x_type, group);
     return (uint64_t)p.z * p.xs_block;
 }
 
@@ -596,7 +736,7 @@ ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t
     if ((uintptr_t)packed % 16 || (uintptr_t)workspace % 16)
         return fail(YTM_ERR_ARG, "q4: packed weights and workspace must start on a 16-byte boundary");
     cudaStream_t st = as_stream(stream);
-    const Q4Plan p = q4_plan(N, C, K, x_type);
+    const Q4Plan p = q4_plan(N, C, K, x_type, group);
     // the weights as a matrix of bytes, tiles of 128 bytes by 16 WM classes; zeros outside
     CUtensorMap map;
     const cuuint64_t dims[2] = {(cuuint64_t)q4_row_bytes(C), (cuuint64_t)K}, strides[1] = {(cuuint64_t)q4_row_bytes(C)};
@@ -607,18 +747,21 @@ ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return fail(YTM_ERR_CUDA, "q4 votes: cuTensorMapEncodeTiled refused the weights");
     const int64_t most = p.z * p.samples;  // samples of a launch
-    const int groups = p.stages * (8 << p.log_wk);
+    const int segs = p.stages << p.log_wk;
     for (int64_t i = 0; i < N; i += most) {
         const int64_t n = std::min(N - i, most);
-        const Q4XArgs xa = {x, x_stride, i, n, (char *)workspace, p.xs_block, C, x_type, p.samples, p.parts, groups};
-        const uint64_t blocks = cdiv((uint64_t)n * groups * 4, 256);
+        const Q4XArgs xa = {x, x_stride, i, n, (char *)workspace, p.xs_block, C, x_type, p.samples, p.parts, p.cols, segs, group};
+        const uint64_t blocks = cdiv((uint64_t)n * segs * 32, 256);
         if (blocks > INT_MAX) return fail(YTM_ERR_UNSUPPORTED, "q4 votes: too many activations for one call");
-        k_q4_x<<<(unsigned)blocks, 256, 0, st>>>(xa);
-        if ((rc = launch_check("q4 activations"))) return rc;
         const Q4Args a = {(const char *)workspace, scales, bias, y, i, n, p.xs_block, K, (int)cdiv(C, group), p.stages, scale_type,
                           y_type, p.samples, p.parts, p.log_wk, p.cluster, (int)p.smem - Q4_BARS};
         const dim3 grid((unsigned)(cdiv(K, 16 * p.wm) * p.cluster), 1, (unsigned)cdiv(n, p.samples));
-        rc = x_type == YTM_F16 ? launch_q4<true>(a, p, map, group, grid, st) : launch_q4<false>(a, p, map, group, grid, st);
+        switch (p.mode) {
+            case Q4_BITS: rc = launch_q4<Q4_BITS>(xa, (unsigned)blocks, a, p, map, group, grid, st); break;
+            case Q4_DIGITS: rc = launch_q4<Q4_DIGITS>(xa, (unsigned)blocks, a, p, map, group, grid, st); break;
+            case Q4_BF16: rc = launch_q4<Q4_BF16>(xa, (unsigned)blocks, a, p, map, group, grid, st); break;
+            default: rc = launch_q4<Q4_FP16>(xa, (unsigned)blocks, a, p, map, group, grid, st); break;
+        }
         if (rc) return rc;
     }
     return YTM_OK;
