@@ -60,10 +60,13 @@ __global__ void k_q4_pack(const T *__restrict__ w, int64_t w_stride, int C, int 
 //   neighbours, i.e. x to 2^-30 of that one, in four columns.  The 8 that the
 //   weights are offset by goes into the sums' start, -8 times the sum of a
 //   group's digits.  Sums of a group are exact.
-// - 16-bit products (m16n8k16), for more than eight 16-bit samples, whose four
-//   columns would cost more products than they save: the word becomes four pairs
-//   (clauses i and i + 4) by or-ing it into the fraction of 128 (fp16: 1024) and
-//   subtracting 136 (1032), exactly.
+// - 16-bit products (m16n8k16): the word becomes four pairs (clauses i and i + 4)
+//   by or-ing it into the fraction of 128 (fp16: 1024) and subtracting 136
+//   (1032), exactly; four times the logic, but a column a sample.  Taken for 16-bit
+//   activations from three samples on (16384 x 32768, bf16: one sample 71 us against
+//   53 in digits, three 71 against 67, five 71 against 110; 8192 x 8192: 13.6
+//   against 12.2, 13.9 against 14.5, 14.2 against 19.9), and where few classes leave
+//   the weights' stream short (65536 x 100: 7.9 against 9.4).
 //
 // A group's sum is scaled in fp32.  k_q4_x lays the activations out before, in
 // pieces of 256 clauses, so that a stage's are one piece of memory.
@@ -388,25 +391,26 @@ __global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS == 16 ? 2 : 1
         int last[GPL];  // stages that have this lane's group (group0 + 4 j + s group_step < G)
 #pragma unroll
         for (int j = 0; j < GPL; ++j) last[j] = (a.G - group0 - 4 * j + group_step - 1) / group_step;
-        uint32_t next_sc[GPL][2];
-        const auto load_scales = [&](int s) {
+        uint32_t next_sc[2][GPL][2];
+        const auto load_scales = [&](int s, uint32_t (&to)[GPL][2]) {
 #pragma unroll
             for (int j = 0; j < GPL; ++j) {
-                next_sc[j][0] = next_sc[j][1] = 0u;  // behind the last group: 0
+                to[j][0] = to[j][1] = 0u;  // behind the last group: 0
                 if (s < last[j]) {
                     if (wide) {
-                        next_sc[j][0] = *(const uint32_t *)(sc0 + 16 * j);
-                        next_sc[j][1] = *(const uint32_t *)(sc1 + 16 * j);
+                        to[j][0] = *(const uint32_t *)(sc0 + 16 * j);
+                        to[j][1] = *(const uint32_t *)(sc1 + 16 * j);
                     } else {
-                        next_sc[j][0] = *(const uint16_t *)(sc0 + 8 * j);
-                        next_sc[j][1] = *(const uint16_t *)(sc1 + 8 * j);
+                        to[j][0] = *(const uint16_t *)(sc0 + 8 * j);
+                        to[j][1] = *(const uint16_t *)(sc1 + 8 * j);
                     }
                 }
             }
             sc0 += group_step * bytes;
             sc1 += group_step * bytes;
         };
-        load_scales(0);
+        load_scales(0, next_sc[0]);
+        load_scales(1, next_sc[1]);
         // rows of 128 bytes, their 16-byte pieces exchanged by the row's low bits (128-byte swizzle)
         const int mrow = (lane >> 3 & 1) * 8 + (lane & 7);
         const uint32_t mat = smem_at + (wk * WM + wm) * 2048 + mrow * 128;
@@ -414,10 +418,12 @@ __global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS == 16 ? 2 : 1
             float sc[GPL][2];
 #pragma unroll
             for (int j = 0; j < GPL; ++j) {
-                sc[j][0] = scale_value(next_sc[j][0], a.scale_type);
-                sc[j][1] = scale_value(next_sc[j][1], a.scale_type);
+                sc[j][0] = scale_value(next_sc[0][j][0], a.scale_type);
+                sc[j][1] = scale_value(next_sc[0][j][1], a.scale_type);
+                next_sc[0][j][0] = next_sc[1][j][0];
+                next_sc[0][j][1] = next_sc[1][j][1];
             }
-            load_scales(s + 1);
+            load_scales(s + 2, next_sc[1]);
             bar_wait(full + 8 * (s % Q4_STAGES), (s / Q4_STAGES) & 1, failed);
             __syncwarp();
             const uint32_t w_at = mat + (s % Q4_STAGES) * Q4_STAGE_BYTES;
@@ -568,9 +574,12 @@ __global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS == 16 ? 2 : 1
     if (a.cluster > 1) cg::this_cluster().sync();  // nobody leaves while its sums are read
 }
 
-// How a call is cut.  The cost of a cut, in stages of 16 KB: the blocks of the
-// busiest SM times the stages of a block plus about three for its start and its
-// end, half of which a second block on the SM hides.
+// How a call is cut.  The cost of a cut in microseconds, as measured: a stage of
+// 16 KB takes 0.37 for each block that its SM holds (the SM's share of the
+// memory's rate), or 0.15 to 0.3 for every 8 columns where the products bound
+// it; every further round of blocks takes 3 to end and to start, and 6 if they
+// are clusters (16384 x 32768, one sample: 256 blocks 49 us, 1024 in clusters of
+// four 60 us; 65536 x 100: clusters of 16 6.8 us, 7 blocks 24 us).
 struct Q4Plan {
     Q4Mode mode;
     int cols, samples, parts;  // of a block (columns padded); columns of a sample
@@ -581,7 +590,7 @@ struct Q4Plan {
 
 static Q4Plan q4_plan(int64_t N, int64_t C, int64_t K, int x_type, int group) {
     Q4Plan p = {};
-    p.mode = x_type == YTM_BITS ? Q4_BITS : x_type == YTM_F32 || N <= 8 ? Q4_DIGITS : x_type == YTM_F16 ? Q4_FP16 : Q4_BF16;
+    p.mode = x_type == YTM_BITS ? Q4_BITS : x_type == YTM_F32 || (N <= 2 && K >= 1024) ? Q4_DIGITS : x_type == YTM_F16 ? Q4_FP16 : Q4_BF16;
     p.parts = p.mode == Q4_DIGITS ? 4 : 1;
     const int64_t most = 64 / p.parts;
     p.samples = (int)std::min(N, most);
@@ -589,18 +598,23 @@ static Q4Plan q4_plan(int64_t N, int64_t C, int64_t K, int x_type, int group) {
     const int used = p.samples * p.parts;
     p.cols = used <= 8 ? 8 : used <= 16 ? 16 : used <= 32 ? 32 : used <= 48 ? 48 : 64;
     const int seg_bytes = q4_seg_bytes(p.mode, p.cols, group);
-    double least = 0;
     const int64_t sms = sm_count();
+    const int nt = p.cols / 8;
+    double least = 0;
     for (int wm = 8, log_wk = 0; wm >= 1; wm /= 2, ++log_wk) {
         const int64_t wk = Q4_WARPS / wm;
         const size_t red = (size_t)Q4_WARPS * 16 * p.cols * 4 + (size_t)p.samples * 16 * wm * 4;
         const size_t smem = std::max<size_t>(Q4_STAGES * (Q4_STAGE_BYTES + (size_t)seg_bytes * wk), red) + Q4_BARS;
         if (smem > 227 * 1024) continue;
         const int64_t tiles = cdiv(K, 16 * wm) * p.z, stages = cdiv(C, Q4_SEG * wk);
-        const bool two = p.cols <= 16 && smem <= 112 * 1024;
+        const int64_t held = std::min<int64_t>(nt == 1 ? 3 : nt == 2 ? 2 : 1, 227 * 1024 / (smem + 1024));  // blocks of an SM
         for (int cl = 1; cl <= 16 && (cl == 1 || cl <= stages); cl *= 2) {
-            // SMs that hold two blocks share their bandwidth between them
-            const double cost = (double)cdiv(tiles * cl, sms) * ((double)cdiv(stages, cl) + (two ? 1.5 : 3));
+            const int64_t place = cl == 16 ? sms * 3 / 4 : cl == 8 ? sms * 6 / 7 : sms;  // SMs that such clusters reach
+            const int64_t rounds = tiles * cl / (place * held), rest = tiles * cl % (place * held);
+            const auto stage = [&](int64_t r) { return std::max(0.37 * r, 0.15 * nt * (1 + r)); };
+            const double per = (double)cdiv(stages, cl);
+            const double cost = per * (rounds * stage(held) + (rest ? stage(cdiv(rest, place)) : 0)) +
+                                (rounds - (rest ? 0 : 1)) * (cl > 1 ? 6 : 3);
             if (!p.wm || cost < least * 0.97) {
                 p.wm = wm;
                 p.log_wk = log_wk;
@@ -669,8 +683,7 @@ static ytm_status launch_q4(const Q4XArgs &xa, unsigned x_blocks, const Q4Args &
     ytm_status rc = launch_check("q4 activations");
     if (rc) return rc;
     switch (p.cols) {
-        case 8:  // more than eight samples of 16 bits take 16 columns and more
-            if constexpr (MODE <= Q4_DIGITS) return launch_q4<MODE, 8>(a, p, map, group, grid, st);
+        case 8: return launch_q4<MODE, 8>(a, p, map, group, grid, st);
         case 16: return launch_q4<MODE, 16>(a, p, map, group, grid, st);
         case 32: return launch_q4<MODE, 32>(a, p, map, group, grid, st);
         case 48: return launch_q4<MODE, 48>(a, p, map, group, grid, st);
