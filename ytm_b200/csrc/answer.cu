@@ -1,5 +1,19 @@
 // answer.cu — from class sums to an answer: biases, allowed classes and
-// penalties, the choice of a class and its log-probability.
+// penalties, the choice of a class and its log-probability, in one pass.
+//
+// z = allowed ? (pen(v) + b) / t : -inf, formed in 64 bits and rounded once, so
+// that equal and nearly equal class sums compare as the real numbers they
+// stand for.  A thread forms E of a row's z at a time, finds their best, and
+// sums exp(z' - z) over the others; two such triples (z, class, sum) merge into
+// one.  The choice's log-probability is then -log1p(sum): without the
+// cancellation of z - logsumexp(z) where the choice is nearly certain.
+//
+// Rows of up to 512 classes belong to 4 to 32 threads, whose next row is on its
+// way while they work; longer ones to a block, or to a cluster of up to 16
+// blocks where there are few rows, which merge through distributed shared
+// memory.  How often a class stands in the row's history is counted in shared
+// memory first, for the classes that the block holds.
+#include <cooperative_groups.h>
 #include <limits.h>
 #include <math.h>
 
@@ -8,13 +22,7 @@
 
 namespace ytm {
 
-// ------------------------------------------------------------ the choice
-// z = allowed ? (pen(v) + b) / t : -inf, formed in 64 bits and rounded once, so
-// that equal and nearly equal class sums compare as the real numbers they
-// stand for.  One pass keeps, per thread, the best (z, class) and the sum s of
-// exp(z' - z) over the other allowed classes; two such triples merge into
-// one.  The choice's log-probability is then -log1p(s): without the
-// cancellation of z - logsumexp(z) where the choice is nearly certain.
+namespace cg = cooperative_groups;
 
 struct Best {
     float z;
@@ -29,82 +37,286 @@ __device__ __forceinline__ bool above(float z, int k, float z2, int k2) {
     return z > z2 || (z == z2 && k < k2);
 }
 
+__device__ __forceinline__ float exp_of(float x) {  // within a few steps and x's rounding
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+
 __device__ __forceinline__ Best merge(const Best &a, const Best &b) {
-    if (a.k == INT_MAX) return b;
-    if (b.k == INT_MAX) return a;
-    const bool ab = above(a.z, a.k, b.z, b.k);
+    const bool ab = b.k == INT_MAX || (a.k != INT_MAX && above(a.z, a.k, b.z, b.k));
     const Best hi = ab ? a : b, lo = ab ? b : a;
-    const float f = expf(lo.z - hi.z);
+    if (lo.k == INT_MAX) return hi;
+    const float f = exp_of(lo.z - hi.z);
     // a term of -inf adds nothing, whatever its own sum came to
-    return {hi.z, hi.k, f == 0.f ? hi.s : hi.s + f * (1.f + lo.s)};
+    return {hi.z, hi.k, f == 0.f ? hi.s : __fadd_rn(hi.s, __fmul_rn(f, 1.f + lo.s))};
+}
+
+__device__ __forceinline__ Best merge_lanes(Best b, int lanes) {
+    for (int d = lanes / 2; d; d >>= 1)
+        b = merge(b, {__shfl_xor_sync(0xFFFFFFFFu, b.z, d), __shfl_xor_sync(0xFFFFFFFFu, b.k, d),
+                      __shfl_xor_sync(0xFFFFFFFFu, b.s, d)});
+    return b;
 }
 
 struct AnswerRow {
-    double rt, r, f, p;
+    double rt;
+    float r, f, p;
+    int64_t len;  // of the history
 };
 
 __device__ __forceinline__ AnswerRow answer_row(const ytm_answer_args &a, int64_t n) {
     AnswerRow o;
     o.rt = 1.0 / (double)(a.temperature ? a.temperature[n] : a.temperature_all);
-    o.r = (double)(a.repetition ? a.repetition[n] : a.repetition_all);
-    o.f = (double)(a.frequency ? a.frequency[n] : a.frequency_all);
-    o.p = (double)(a.presence ? a.presence[n] : a.presence_all);
+    o.len = 0;
+    if (a.history) {
+        o.r = a.repetition ? a.repetition[n] : a.repetition_all;
+        o.f = a.frequency ? a.frequency[n] : a.frequency_all;
+        o.p = a.presence ? a.presence[n] : a.presence_all;
+        o.len = a.lengths ? max(0, min(a.history_len, a.lengths[n])) : a.history_len;
+    }
     return o;
 }
 
-__device__ __forceinline__ float adjust(double v, uint32_t count, double b, const AnswerRow &o) {
-    if (count) v = (v > 0.0 ? v / o.r : v * o.r) - o.f * (double)count - o.p;
-    return (float)((v + b) * o.rt);
+// Penalties for a class that stands `count` times in the history.
+__device__ __noinline__ double penalised(double v, uint32_t count, float r, float f, float p) {
+    return (v > 0.0 ? v / (double)r : v * (double)r) - (double)f * (double)count - (double)p;
 }
 
-constexpr int AN_THREADS = 256, AN_CHUNK = 8192;
+// The best of E classes of a thread and the others' sum.
+template <int E, typename K>
+__device__ __forceinline__ Best best_of(const float (&z)[E], uint32_t open, K class_of) {
+    Best b = {-INFINITY, INT_MAX, 0.f};
+    int at = -1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (!((open >> e) & 1u)) continue;
+        if (at < 0 || z[e] > b.z || (z[e] != z[e] && b.z == b.z)) {
+            b.z = z[e];
+            at = e;
+        }
+    }
+    if (at < 0) return b;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float x = exp_of(z[e] - b.z);
+        if ((open >> e) & 1u && e != at) b.s += x;
+    }
+    b.k = class_of(at);
+    return b;
+}
+
+__device__ __forceinline__ void write_answer(const ytm_answer_args &a, int64_t n, const Best &b) {
+    const bool none = b.k == INT_MAX;
+    if (a.choice) a.choice[n] = none ? -1 : b.k;
+    if (a.logprob) a.logprob[n] = none ? -INFINITY : b.z != b.z ? b.z : -log1pf(b.s);
+}
+
+constexpr int AN_THREADS = 256;
+
+// -------------------------------------------------- rows of few classes
+// TPR threads hold a row, E classes each, neighbouring lanes neighbouring classes.
+
+template <typename T, int TPR, int E>
+__global__ void __launch_bounds__(AN_THREADS, E == 16 ? 3 : 4) k_answer_small(const ytm_answer_args a) {
+    constexpr int ROWS = AN_THREADS / TPR;
+    extern __shared__ uint32_t counts[];  // [ROWS][TPR * E], with a history
+    const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR, K = a.k;
+    uint32_t *const mine = counts + team * TPR * E;
+    uint32_t there = 0, shared_open = 0;
+    float b[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int k = e * TPR + lane;
+        b[e] = a.bias && k < K && !a.bias_stride ? a.bias[k] : 0.f;
+        if (k < K) there |= 1u << e;
+        if (k < K && (a.allowed_stride || is_allowed(a.allowed, k))) shared_open |= 1u << e;
+    }
+    struct Row {
+        T v[E];
+        uint32_t open;
+    };
+    const auto clamped = [&](int64_t n) { return n < a.n ? n : a.n - 1; };
+    const auto fetch = [&](int64_t n0) {
+        Row r;
+        const int64_t n = clamped(n0 + team);
+        const T *cs = (const T *)a.cs + n * a.cs_stride;
+        r.open = shared_open;
+#pragma unroll
+        for (int e = 0; e < E; ++e) r.v[e] = (there >> e) & 1u ? cs[e * TPR + lane] : T(0.f);
+        if (a.allowed_stride) {
+            const uint32_t *w = a.allowed + n * a.allowed_stride;
+            uint32_t bits = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if ((there >> e) & 1u) bits |= (w[(e * TPR + lane) >> 5] >> ((e * TPR + lane) & 31) & 1u) << e;
+            r.open &= bits;
+        }
+        return r;
+    };
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t n0 = (int64_t)blockIdx.x * ROWS;
+    Row next = fetch(n0);
+    for (; n0 < a.n; n0 += step) {
+        const Row row = next;
+        if (n0 + step < a.n) next = fetch(n0 + step);
+        const bool live = n0 + team < a.n;
+        const int64_t n = clamped(n0 + team);
+        const AnswerRow o = answer_row(a, n);
+        if (a.history) {
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < E; ++e) mine[e * TPR + lane] = 0;
+            __syncwarp();
+            for (int64_t i = lane; i < o.len; i += TPR) {
+                const int64_t h = index_at(a.history, a.history_64, n * a.history_stride + i);
+                if (h >= 0 && h < K) atomicAdd(&mine[h], 1u);
+            }
+            __syncwarp();
+        }
+        float z[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            double v = to_f64(row.v[e]);
+            if (a.history) {
+                const uint32_t c = mine[e * TPR + lane];
+                if (c) v = penalised(v, c, o.r, o.f, o.p);
+            }
+            if (a.bias) v += (double)(a.bias_stride ? ((there >> e) & 1u ? a.bias[n * a.bias_stride + e * TPR + lane] : 0.f) : b[e]);
+            z[e] = (row.open >> e) & 1u ? (float)(v * o.rt) : -INFINITY;
+        }
+        Best best = best_of(z, row.open, [&](int e) { return e * TPR + lane; });
+        best = merge_lanes(best, TPR);
+        if (!live) continue;
+        if (a.adjusted) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if ((there >> e) & 1u) a.adjusted[n * (int64_t)K + e * TPR + lane] = z[e];
+        }
+        if (lane == 0) write_answer(a, n, best);
+    }
+}
+
+// -------------------------------------------------- rows of many classes
+
+constexpr int AN_E = 16, AN_TILE = AN_THREADS * AN_E;
+constexpr int AN_COUNTS = 2 * AN_TILE;  // classes whose counts a block holds
 
 template <typename T>
-__global__ void __launch_bounds__(AN_THREADS) k_answer(const ytm_answer_args a) {
-    __shared__ uint32_t cnt[AN_CHUNK];
-    __shared__ Best part[AN_THREADS / 32];
-    const int64_t n = blockIdx.x;
+__global__ void __launch_bounds__(AN_THREADS, 3) k_answer_big(const ytm_answer_args a, int cluster, int part) {
+    __shared__ Best warp_best[AN_THREADS / 32], block_best;
+    extern __shared__ uint32_t counts[];  // [AN_COUNTS], with a history
+    const int tid = threadIdx.x;
+    const int64_t n = blockIdx.x / cluster;
+    const int rank = (int)(blockIdx.x % cluster);
+    const int from = (int)min((int64_t)a.k, (int64_t)rank * part), to = (int)min((int64_t)a.k, (int64_t)from + part);
     const T *cs = (const T *)a.cs + n * a.cs_stride;
     const float *bias = a.bias ? a.bias + n * a.bias_stride : nullptr;
     const uint32_t *allowed = a.allowed ? a.allowed + n * a.allowed_stride : nullptr;
     const AnswerRow o = answer_row(a, n);
-    const int64_t len = a.history ? (a.lengths ? max(0, min(a.history_len, a.lengths[n])) : a.history_len) : 0;
     Best best = {-INFINITY, INT_MAX, 0.f};
-    for (int k0 = 0; k0 < a.k; k0 += AN_CHUNK) {
-        const int kn = min(AN_CHUNK, a.k - k0);
-        if (len) {
-            for (int i = threadIdx.x; i < kn; i += AN_THREADS) cnt[i] = 0;
+    for (int c0 = from; c0 < to; c0 += AN_COUNTS) {
+        const int c1 = (int)min((int64_t)to, (int64_t)c0 + AN_COUNTS);
+        if (o.len) {
             __syncthreads();
-            for (int64_t i = threadIdx.x; i < len; i += AN_THREADS) {
-                const int64_t h = index_at(a.history, a.history_64, n * a.history_stride + i) - k0;
-                if (h >= 0 && h < kn) atomicAdd(&cnt[h], 1u);
+            for (int i = tid; i < c1 - c0; i += AN_THREADS) counts[i] = 0;
+            __syncthreads();
+            for (int64_t i = tid; i < o.len; i += AN_THREADS) {
+                const int64_t h = index_at(a.history, a.history_64, n * a.history_stride + i) - c0;
+                if (h >= 0 && h < c1 - c0) atomicAdd(&counts[h], 1u);
             }
             __syncthreads();
         }
-        for (int i = threadIdx.x; i < kn; i += AN_THREADS) {
-            const int k = k0 + i;
-            float z = -INFINITY;
-            if (is_allowed(allowed, k)) {
-                z = adjust(to_f64(cs[k]), len ? cnt[i] : 0u, bias ? (double)bias[k] : 0.0, o);
-                best = merge(best, {z, k, 0.f});
+        for (int k0 = c0 + tid; k0 - tid < c1; k0 += AN_TILE) {
+            float z[AN_E];
+            uint32_t open = 0;
+            T v[AN_E];
+            float b[AN_E];
+#pragma unroll
+            for (int e = 0; e < AN_E; ++e) {
+                const int k = k0 + e * AN_THREADS;
+                const bool there = k < c1;
+                v[e] = there ? cs[k] : T(0.f);
+                b[e] = there && bias ? bias[k] : 0.f;
+                // c0 and the tiles are multiples of 32: a warp's bits are one word
+                if (there) open |= (allowed ? allowed[k >> 5] >> (k & 31) & 1u : 1u) << e;
             }
-            if (a.adjusted) a.adjusted[n * a.k + k] = z;
+#pragma unroll
+            for (int e = 0; e < AN_E; ++e) {
+                const int k = k0 + e * AN_THREADS;
+                double x = to_f64(v[e]);
+                if (o.len && k < c1) {
+                    const uint32_t c = counts[k - c0];
+                    if (c) x = penalised(x, c, o.r, o.f, o.p);
+                }
+                x = (x + (double)b[e]) * o.rt;
+                z[e] = (open >> e) & 1u ? (float)x : -INFINITY;
+                if (a.adjusted && k < c1) a.adjusted[n * a.k + k] = z[e];
+            }
+            best = merge(best, best_of(z, open, [&](int e) { return k0 + e * AN_THREADS; }));
         }
-        if (len) __syncthreads();
     }
-    for (int d = 16; d; d >>= 1) {
-        const Best b = {__shfl_xor_sync(0xFFFFFFFFu, best.z, d), __shfl_xor_sync(0xFFFFFFFFu, best.k, d),
-                        __shfl_xor_sync(0xFFFFFFFFu, best.s, d)};
-        best = merge(best, b);
-    }
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = best;
+    best = merge_lanes(best, 32);
+    if ((tid & 31) == 0) warp_best[tid >> 5] = best;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < AN_THREADS / 32; ++i) best = merge(best, part[i]);
-        const bool none = best.k == INT_MAX;
-        if (a.choice) a.choice[n] = none ? -1 : best.k;
-        if (a.logprob) a.logprob[n] = none ? -INFINITY : best.z != best.z ? best.z : -log1pf(best.s);
+    if (tid < 32) {
+        best = merge_lanes(warp_best[tid % (AN_THREADS / 32)], AN_THREADS / 32);
+        if (tid == 0) block_best = best;
     }
+    if (cluster > 1) {
+        cg::cluster_group cl = cg::this_cluster();
+        cl.sync();
+        if (rank == 0 && tid < 32) {
+            best = {-INFINITY, INT_MAX, 0.f};
+            if (tid < cluster) best = *cl.map_shared_rank(&block_best, tid);
+            best = merge_lanes(best, 16);
+        }
+        cl.sync();  // nobody leaves while its best is read
+    }
+    if (rank == 0 && tid == 0) write_answer(a, n, best);
+}
+
+template <typename T, int TPR, int E>
+static ytm_status launch_small(const ytm_answer_args &a, cudaStream_t st) {
+    const int64_t rows = AN_THREADS / TPR;
+    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.n, rows), (int64_t)sm_count() * (E == 16 ? 3 : 4) * 2);
+    k_answer_small<T, TPR, E><<<grid, AN_THREADS, a.history ? AN_THREADS * E * 4 : 0, st>>>(a);
+    return launch_check("answer");
+}
+
+template <typename T>
+static ytm_status launch_big(const ytm_answer_args &a, cudaStream_t st) {
+    // blocks of a row until there are about two an SM, of at least a tile each
+    int cluster = 1;
+    while (cluster < 16 && a.n * cluster < 2 * (int64_t)sm_count() && a.k > cluster * AN_TILE) cluster *= 2;
+    if (a.n * cluster > INT_MAX) return fail(YTM_ERR_UNSUPPORTED, "answer: too many rows for one call");
+    const int part = (int)(cdiv(cdiv(a.k, cluster), 32) * 32);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.n * cluster));
+    cfg.blockDim = dim3(AN_THREADS);
+    cfg.dynamicSmemBytes = a.history ? AN_COUNTS * 4 : 0;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    auto *f = k_answer_big<T>;
+    ytm_status rc;
+    if (cluster > 8 && (rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "answer cluster")))
+        return rc;
+    return cuda_check(cudaLaunchKernelEx(&cfg, f, a, cluster, part), "answer");
+}
+
+template <typename T>
+static ytm_status launch_answer(const ytm_answer_args &a, cudaStream_t st) {
+    if (a.k > 512) return launch_big<T>(a, st);
+    if (a.k <= 16) return launch_small<T, 4, 4>(a, st);
+    if (a.k <= 64) return launch_small<T, 8, 8>(a, st);
+    if (a.k <= 128) return launch_small<T, 8, 16>(a, st);
+    if (a.k <= 256) return launch_small<T, 16, 16>(a, st);
+    return launch_small<T, 32, 16>(a, st);
 }
 
 }  // namespace ytm
@@ -117,7 +329,7 @@ ytm_status ytm_answer(const ytm_answer_args *args, void *stream) {
     if (!args) return fail(YTM_ERR_ARG, "args is NULL");
     const ytm_answer_args &a = *args;
     if (a.n < 0 || a.k <= 0) return fail(YTM_ERR_ARG, "answer: needs n >= 0 rows of k >= 1 classes");
-    if (a.n > INT_MAX) return fail(YTM_ERR_UNSUPPORTED, "answer: more than 2^31 - 1 rows");
+    if (a.n > INT_MAX || a.k > (1 << 30)) return fail(YTM_ERR_UNSUPPORTED, "answer: more than 2^31 - 1 rows or 2^30 classes");
     if (!is_sum_type(a.cs_type)) return fail(YTM_ERR_ARG, "answer: class sums must be int32, fp32, fp16 or bf16");
     if (a.cs_stride < 0 || a.bias_stride < 0 || a.allowed_stride < 0 || a.history_stride < 0 || a.history_len < 0)
         return fail(YTM_ERR_ARG, "answer: negative stride or length");
@@ -125,12 +337,11 @@ ytm_status ytm_answer(const ytm_answer_args *args, void *stream) {
     if (!a.cs || (a.lengths && !a.history)) return fail(YTM_ERR_ARG, "null pointer");
     cudaStream_t st = as_stream(stream);
     switch (a.cs_type) {
-        case YTM_I32: k_answer<int32_t><<<(unsigned)a.n, AN_THREADS, 0, st>>>(a); break;
-        case YTM_F32: k_answer<float><<<(unsigned)a.n, AN_THREADS, 0, st>>>(a); break;
-        case YTM_F16: k_answer<__half><<<(unsigned)a.n, AN_THREADS, 0, st>>>(a); break;
-        default: k_answer<__nv_bfloat16><<<(unsigned)a.n, AN_THREADS, 0, st>>>(a); break;
+        case YTM_I32: return launch_answer<int32_t>(a, st);
+        case YTM_F32: return launch_answer<float>(a, st);
+        case YTM_F16: return launch_answer<__half>(a, st);
+        default: return launch_answer<__nv_bfloat16>(a, st);
     }
-    return launch_check("answer");
 }
 
 }  // extern "C"
