@@ -60,9 +60,9 @@ __device__ __forceinline__ Best merge_lanes(Best b, int lanes) {
 }
 
 struct AnswerRow {
-    double rt;
+    double rt, rr;  // 1 / temperature, 1 / repetition
     float r, f, p;
-    int64_t len;  // of the history
+    int64_t len;    // of the history
 };
 
 __device__ __forceinline__ AnswerRow answer_row(const ytm_answer_args &a, int64_t n) {
@@ -71,6 +71,7 @@ __device__ __forceinline__ AnswerRow answer_row(const ytm_answer_args &a, int64_
     o.len = 0;
     if (a.history) {
         o.r = a.repetition ? a.repetition[n] : a.repetition_all;
+        o.rr = 1.0 / (double)o.r;
         o.f = a.frequency ? a.frequency[n] : a.frequency_all;
         o.p = a.presence ? a.presence[n] : a.presence_all;
         o.len = a.lengths ? max(0, min(a.history_len, a.lengths[n])) : a.history_len;
@@ -79,8 +80,8 @@ __device__ __forceinline__ AnswerRow answer_row(const ytm_answer_args &a, int64_
 }
 
 // Penalties for a class that stands `count` times in the history.
-__device__ __noinline__ double penalised(double v, uint32_t count, float r, float f, float p) {
-    return (v > 0.0 ? v / (double)r : v * (double)r) - (double)f * (double)count - (double)p;
+__device__ __forceinline__ double penalised(double v, uint32_t count, const AnswerRow &o) {
+    return v * (v > 0.0 ? o.rr : (double)o.r) - (double)o.f * (double)count - (double)o.p;
 }
 
 // The best of E classes of a thread and the others' sum.
@@ -118,7 +119,7 @@ constexpr int AN_THREADS = 256;
 // TPR threads hold a row, E classes each, neighbouring lanes neighbouring classes.
 
 template <typename T, int TPR, int E>
-__global__ void __launch_bounds__(AN_THREADS, E == 16 ? 3 : 4) k_answer_small(const ytm_answer_args a) {
+__global__ void __launch_bounds__(AN_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_answer_small(const ytm_answer_args a) {
     constexpr int ROWS = AN_THREADS / TPR;
     extern __shared__ uint32_t counts[];  // [ROWS][TPR * E], with a history
     const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR, K = a.k;
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(AN_THREADS, E == 16 ? 3 : 4) k_answer_small(co
             double v = to_f64(row.v[e]);
             if (a.history) {
                 const uint32_t c = mine[e * TPR + lane];
-                if (c) v = penalised(v, c, o.r, o.f, o.p);
+                if (c) v = penalised(v, c, o);
             }
             if (a.bias) v += (double)(a.bias_stride ? ((there >> e) & 1u ? a.bias[n * a.bias_stride + e * TPR + lane] : 0.f) : b[e]);
             z[e] = (row.open >> e) & 1u ? (float)(v * o.rt) : -INFINITY;
@@ -199,12 +200,12 @@ __global__ void __launch_bounds__(AN_THREADS, E == 16 ? 3 : 4) k_answer_small(co
 
 // -------------------------------------------------- rows of many classes
 
-constexpr int AN_E = 16, AN_TILE = AN_THREADS * AN_E;
-constexpr int AN_COUNTS = 2 * AN_TILE;  // classes whose counts a block holds
+// Classes whose counts a block holds.
+constexpr int AN_COUNTS = 8192;
 
-template <typename T>
-__global__ void __launch_bounds__(AN_THREADS, 3) k_answer_big(const ytm_answer_args a, int cluster, int part) {
-    __shared__ Best warp_best[AN_THREADS / 32], block_best;
+template <typename T, int THREADS, int E>
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : E == 16 ? 3 : 4) k_answer_big(const ytm_answer_args a, int cluster, int part) {
+    __shared__ Best warp_best[32], block_best;
     extern __shared__ uint32_t counts[];  // [AN_COUNTS], with a history
     const int tid = threadIdx.x;
     const int64_t n = blockIdx.x / cluster;
@@ -219,48 +220,47 @@ __global__ void __launch_bounds__(AN_THREADS, 3) k_answer_big(const ytm_answer_a
         const int c1 = (int)min((int64_t)to, (int64_t)c0 + AN_COUNTS);
         if (o.len) {
             __syncthreads();
-            for (int i = tid; i < c1 - c0; i += AN_THREADS) counts[i] = 0;
+            for (int i = tid; i < c1 - c0; i += THREADS) counts[i] = 0;
             __syncthreads();
-            for (int64_t i = tid; i < o.len; i += AN_THREADS) {
+            for (int64_t i = tid; i < o.len; i += THREADS) {
                 const int64_t h = index_at(a.history, a.history_64, n * a.history_stride + i) - c0;
                 if (h >= 0 && h < c1 - c0) atomicAdd(&counts[h], 1u);
             }
-            __syncthreads();
         }
-        for (int k0 = c0 + tid; k0 - tid < c1; k0 += AN_TILE) {
-            float z[AN_E];
+        for (int k0 = c0 + tid; k0 - tid < c1; k0 += THREADS * E) {
+            float z[E], b[E];
             uint32_t open = 0;
-            T v[AN_E];
-            float b[AN_E];
+            T v[E];
 #pragma unroll
-            for (int e = 0; e < AN_E; ++e) {
-                const int k = k0 + e * AN_THREADS;
+            for (int e = 0; e < E; ++e) {
+                const int k = k0 + e * THREADS;
                 const bool there = k < c1;
                 v[e] = there ? cs[k] : T(0.f);
                 b[e] = there && bias ? bias[k] : 0.f;
                 // c0 and the tiles are multiples of 32: a warp's bits are one word
                 if (there) open |= (allowed ? allowed[k >> 5] >> (k & 31) & 1u : 1u) << e;
             }
+            if (o.len && k0 == c0 + tid) __syncthreads();  // the counts are there
 #pragma unroll
-            for (int e = 0; e < AN_E; ++e) {
-                const int k = k0 + e * AN_THREADS;
+            for (int e = 0; e < E; ++e) {
+                const int k = k0 + e * THREADS;
                 double x = to_f64(v[e]);
                 if (o.len && k < c1) {
                     const uint32_t c = counts[k - c0];
-                    if (c) x = penalised(x, c, o.r, o.f, o.p);
+                    if (c) x = penalised(x, c, o);
                 }
-                x = (x + (double)b[e]) * o.rt;
-                z[e] = (open >> e) & 1u ? (float)x : -INFINITY;
+                if (bias) x += (double)b[e];
+                z[e] = (open >> e) & 1u ? (float)(x * o.rt) : -INFINITY;
                 if (a.adjusted && k < c1) a.adjusted[n * a.k + k] = z[e];
             }
-            best = merge(best, best_of(z, open, [&](int e) { return k0 + e * AN_THREADS; }));
+            best = merge(best, best_of(z, open, [&](int e) { return k0 + e * THREADS; }));
         }
     }
     best = merge_lanes(best, 32);
     if ((tid & 31) == 0) warp_best[tid >> 5] = best;
     __syncthreads();
     if (tid < 32) {
-        best = merge_lanes(warp_best[tid % (AN_THREADS / 32)], AN_THREADS / 32);
+        best = merge_lanes(warp_best[tid % (THREADS / 32)], THREADS / 32);
         if (tid == 0) block_best = best;
     }
     if (cluster > 1) {
@@ -279,21 +279,18 @@ __global__ void __launch_bounds__(AN_THREADS, 3) k_answer_big(const ytm_answer_a
 template <typename T, int TPR, int E>
 static ytm_status launch_small(const ytm_answer_args &a, cudaStream_t st) {
     const int64_t rows = AN_THREADS / TPR;
-    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.n, rows), (int64_t)sm_count() * (E == 16 ? 3 : 4) * 2);
+    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.n, rows), (int64_t)sm_count() * (E == 16 ? 2 : E == 8 ? 3 : 4));
     k_answer_small<T, TPR, E><<<grid, AN_THREADS, a.history ? AN_THREADS * E * 4 : 0, st>>>(a);
     return launch_check("answer");
 }
 
-template <typename T>
-static ytm_status launch_big(const ytm_answer_args &a, cudaStream_t st) {
-    // blocks of a row until there are about two an SM, of at least a tile each
-    int cluster = 1;
-    while (cluster < 16 && a.n * cluster < 2 * (int64_t)sm_count() && a.k > cluster * AN_TILE) cluster *= 2;
+template <typename T, int THREADS, int E>
+static ytm_status launch_big(const ytm_answer_args &a, int cluster, cudaStream_t st) {
     if (a.n * cluster > INT_MAX) return fail(YTM_ERR_UNSUPPORTED, "answer: too many rows for one call");
     const int part = (int)(cdiv(cdiv(a.k, cluster), 32) * 32);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.n * cluster));
-    cfg.blockDim = dim3(AN_THREADS);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = a.history ? AN_COUNTS * 4 : 0;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -302,7 +299,7 @@ static ytm_status launch_big(const ytm_answer_args &a, cudaStream_t st) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    auto *f = k_answer_big<T>;
+    auto *f = k_answer_big<T, THREADS, E>;
     ytm_status rc;
     if (cluster > 8 && (rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "answer cluster")))
         return rc;
@@ -311,12 +308,20 @@ static ytm_status launch_big(const ytm_answer_args &a, cudaStream_t st) {
 
 template <typename T>
 static ytm_status launch_answer(const ytm_answer_args &a, cudaStream_t st) {
-    if (a.k > 512) return launch_big<T>(a, st);
     if (a.k <= 16) return launch_small<T, 4, 4>(a, st);
     if (a.k <= 64) return launch_small<T, 8, 8>(a, st);
     if (a.k <= 128) return launch_small<T, 8, 16>(a, st);
     if (a.k <= 256) return launch_small<T, 16, 16>(a, st);
-    return launch_small<T, 32, 16>(a, st);
+    if (a.k <= 512) return launch_small<T, 32, 16>(a, st);
+    if (a.k <= 1024) return launch_big<T, 256, 4>(a, 1, st);
+    if (a.k <= 2048) return launch_big<T, 256, 8>(a, 1, st);
+    // few rows: wide blocks, and clusters of them while every block has an SM
+    if (a.n <= sm_count()) {
+        int cluster = 1;
+        while (cluster < 16 && a.n * cluster * 2 <= sm_count() && a.k > cluster * 8192) cluster *= 2;
+        return launch_big<T, 1024, 8>(a, cluster, st);
+    }
+    return launch_big<T, 256, 16>(a, 1, st);
 }
 
 }  // namespace ytm
