@@ -27,11 +27,18 @@ from ._lib import AnswerArgs, LossArgs, check
 
 _TYPES = {torch.int32: _lib.YTM_I32, torch.float32: _lib.YTM_F32, torch.float16: _lib.YTM_F16,
           torch.bfloat16: _lib.YTM_BF16}
+_SUMS = tuple(_TYPES)
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_F32, _I32, _U8 = (torch.float32,), (torch.int32,), (torch.uint8,)
 _INDICES = (torch.int32, torch.int64)
+_I64 = torch.int64
+_f32 = torch.float32
+_empty = torch.empty
+_grad = torch.is_grad_enabled
+_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index; current_stream() takes 2 us for the same
 
 
-def _need(t, name: str, dim, types, device=None):
+def _need(t, name: str, dim: int, types, device=None):
     """Checks one tensor; returns it with contiguous rows."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
@@ -39,11 +46,11 @@ def _need(t, name: str, dim, types, device=None):
         raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in types)}, got {t.dtype}")
     if t.dim() != dim:
         raise ValueError(f"{name} must have {dim} dimension{'s' if dim > 1 else ''}, got {t.dim()}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device, got {t.device}")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
-    if t.requires_grad and torch.is_grad_enabled():
+    if t.requires_grad and _grad():
         raise ValueError(f"{name} requires grad: these operators do not record into autograd (detach it)")
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         t = t.contiguous()
@@ -57,29 +64,17 @@ def _vector(t, name: str, n: int, types, device):
     return t
 
 
-def _row_stride(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else 0
-
-
-def _stream(device):
-    return ct.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-class _on:
-    """The tensors' device as the current one, for the launch."""
-    __slots__ = ("idx", "ctx")
-
-    def __init__(self, device):
-        self.idx, self.ctx = device.index, None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.idx:
-            self.ctx = torch.cuda.device(self.idx)
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+def _call(f, what: str, device, *args) -> None:
+    """A library call with the tensors' device as the current one, on its
+    current stream."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = f(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
 def pack_allowed(allowed, k: int | None = None):
@@ -111,12 +106,10 @@ def q4_pack(weights: torch.Tensor, group: int = 64, scale_dtype: torch.dtype = t
         raise TypeError("scale_dtype must be float32, float16 or bfloat16")
     if C > 1 and w.stride(0) < K:
         w = w.contiguous()
-    packed = torch.empty((K, -(-C // 32) * 16), dtype=torch.uint8, device=w.device)
-    scales = torch.empty((K, -(-C // group)), dtype=scale_dtype, device=w.device)
-    with _on(w.device):
-        check(_lib.load().ytm_q4_pack(w.data_ptr(), _TYPES[w.dtype], w.stride(0) if C > 1 else K, C, K, group,
-                                      packed.data_ptr(), scales.data_ptr(), _TYPES[scale_dtype], _stream(w.device)),
-              "ytm_q4_pack")
+    packed = _empty(K, -(-C // 32) * 16, dtype=torch.uint8, device=w.device)
+    scales = _empty(K, -(-C // group), dtype=scale_dtype, device=w.device)
+    _call(_lib.load().ytm_q4_pack, "ytm_q4_pack", w.device, w.data_ptr(), _TYPES[w.dtype], w.stride(0) if C > 1 else K,
+          C, K, group, packed.data_ptr(), scales.data_ptr(), _TYPES[scale_dtype])
     return packed, scales
 
 
@@ -129,60 +122,57 @@ def q4_votes(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group:
     x: real activations [n, clauses] (float32, float16, bfloat16), or clause
     outputs as bits, int32 [n, ceil(clauses / 32)] (`CudaEngine.infer_fired`);
     with bits, `clauses` is needed.  bias: float32 [classes]."""
-    x = _need(x, "x", 2, (torch.int32,) + _FLOATS)
+    x = _need(x, "x", 2, _SUMS)
     dev = x.device
-    packed = _need(packed, "packed", 2, (torch.uint8,), dev)
+    packed = _need(packed, "packed", 2, _U8, dev)
     scales = _need(scales, "scales", 2, _FLOATS, dev)
-    bits = x.dtype == torch.int32
+    n, width = x.shape
+    K, row_bytes = packed.shape
+    bits = x.dtype is torch.int32
     if clauses is None:
         if bits:
             raise ValueError("clauses must be given with clause bits")
-        clauses = x.shape[1]
-    K = packed.shape[0]
+        clauses = width
     if clauses < 1 or K < 1:
         raise ValueError("needs at least one clause and one class")
     if group not in (32, 64, 128):
         raise ValueError("group must be 32, 64 or 128")
-    words = -(-clauses // 32)
-    if x.shape[1] != (words if bits else clauses):
-        raise ValueError(f"x has {x.shape[1]} columns, {clauses} clauses need {words if bits else clauses}")
-    if packed.shape[1] != words * 16 or not packed.is_contiguous():
+    words = (clauses + 31) // 32
+    if width != (words if bits else clauses):
+        raise ValueError(f"x has {width} columns, {clauses} clauses need {words if bits else clauses}")
+    if row_bytes != words * 16 or not packed.is_contiguous():
         raise ValueError(f"packed must be contiguous [classes, {words * 16}] for {clauses} clauses")
-    if scales.shape != (K, -(-clauses // group)) or not scales.is_contiguous():
+    if scales.shape != (K, (clauses + group - 1) // group) or not scales.is_contiguous():
         raise ValueError(f"scales must be contiguous [{K}, {-(-clauses // group)}]")
     if out_dtype not in _FLOATS:
         raise TypeError("out_dtype must be float32, float16 or bfloat16")
     if bias is not None:
-        bias = _vector(bias, "bias", K, (torch.float32,), dev)
-    n = x.shape[0]
-    y = torch.empty((n, K), dtype=out_dtype, device=dev)
+        bias = _vector(bias, "bias", K, _F32, dev)
+    y = _empty(n, K, dtype=out_dtype, device=dev)
     if n == 0:
         return y
     lib, x_type = _lib.load(), _lib.YTM_BITS if bits else _TYPES[x.dtype]
-    with _on(dev):
-        ws = torch.empty(lib.ytm_q4_votes_workspace_bytes(x_type, n, clauses, K, group), dtype=torch.uint8, device=dev)
-        check(lib.ytm_q4_votes(x.data_ptr(), x_type, _row_stride(x), n, clauses, packed.data_ptr(), scales.data_ptr(),
-                               _TYPES[scales.dtype], group, K, None if bias is None else bias.data_ptr(), y.data_ptr(),
-                               _TYPES[out_dtype], ws.data_ptr(), _stream(dev)), "ytm_q4_votes")
+    ws = _empty(lib.ytm_q4_votes_workspace_bytes(x_type, n, clauses, K, group), dtype=torch.uint8, device=dev)
+    _call(lib.ytm_q4_votes, "ytm_q4_votes", dev, x.data_ptr(), x_type, x.stride(0) if n > 1 else 0, n, clauses,
+          packed.data_ptr(), scales.data_ptr(), _TYPES[scales.dtype], group, K,
+          None if bias is None else bias.data_ptr(), y.data_ptr(), _TYPES[out_dtype], ws.data_ptr())
     return y
 
 
 # -------------------------------------------------------------- adjusted class sums
 
 def _allowed(allowed, n: int, k: int, device):
-    """(pointer, row stride, tensor) of allowed-class bit words."""
-    if allowed is None:
-        return None, 0, None
-    a = _need(allowed, "allowed", 2, (torch.int32,), device)
+    """Allowed-class bit words, checked."""
+    a = _need(allowed, "allowed", 2, _I32, device)
     if a.shape[1] != (k + 31) // 32 or a.shape[0] not in (1, n):
         raise ValueError(f"allowed must be int32 [{n} or 1, {(k + 31) // 32}], got {list(a.shape)}")
-    return a.data_ptr(), _row_stride(a), a
+    return a
 
 
 def _knob(v, name: str, n: int, device, positive: bool):
     """A number, or float32 [n]: (pointer, value for all rows, tensor)."""
     if isinstance(v, torch.Tensor):
-        t = _vector(v, name, n, (torch.float32,), device)
+        t = _vector(v, name, n, _F32, device)
         return t.data_ptr(), 0.0, t
     v = float(v)
     if positive and not v > 0.0:
@@ -211,34 +201,36 @@ def answer(cs: torch.Tensor, bias: torch.Tensor | None = None, allowed: torch.Te
     the largest z (NaN above all, as numpy's argmax), -1 where no class is
     allowed; logprob is log softmax(z) at the choice, -inf where no class is
     allowed."""
-    cs = _need(cs, "cs", 2, tuple(_TYPES))
+    cs = _need(cs, "cs", 2, _SUMS)
     n, k = cs.shape
     dev = cs.device
     if k < 1:
         raise ValueError("cs must have at least one class")
-    bias_stride = 0
+    bias_p = allowed_p = hist_p = lens_p = None
+    bias_stride = allowed_stride = hist_stride = hist_len = hist_64 = 0
     if bias is not None:
         if isinstance(bias, torch.Tensor) and bias.dim() == 2:
-            bias = _need(bias, "bias", 2, (torch.float32,), dev)
-            if tuple(bias.shape) != (n, k):
+            bias = _need(bias, "bias", 2, _F32, dev)
+            if bias.shape != (n, k):
                 raise ValueError(f"bias must be [{k}] or [{n}, {k}], got {list(bias.shape)}")
-            bias_stride = _row_stride(bias)
+            bias_stride = bias.stride(0) if n > 1 else 0
         else:
-            bias = _vector(bias, "bias", k, (torch.float32,), dev)
-    allowed_p, allowed_stride, allowed = _allowed(allowed, n, k, dev)
-    hist_p = lens_p = None
-    hist_stride = hist_len = hist_64 = 0
+            bias = _vector(bias, "bias", k, _F32, dev)
+        bias_p = bias.data_ptr()
+    if allowed is not None:
+        allowed = _allowed(allowed, n, k, dev)
+        allowed_p, allowed_stride = allowed.data_ptr(), allowed.stride(0) if allowed.shape[0] > 1 else 0
     if history is not None:
         history = _need(history, "history", 2, _INDICES, dev)
         if history.shape[0] != n:
             raise ValueError(f"history must have {n} rows, got {history.shape[0]}")
-        if lengths is not None:
-            lengths = _vector(lengths, "lengths", n, (torch.int32,), dev)
         hist_len = history.shape[1]
+        if lengths is not None:
+            lengths = _vector(lengths, "lengths", n, _I32, dev)
         if hist_len > 2 ** 31 - 1:
             raise ValueError("history must have fewer than 2^31 entries a row")
         if hist_len:
-            hist_p, hist_stride, hist_64 = history.data_ptr(), _row_stride(history), int(history.dtype == torch.int64)
+            hist_p, hist_stride, hist_64 = history.data_ptr(), history.stride(0) if n > 1 else 0, history.dtype is _I64
             if lengths is not None:
                 lens_p = lengths.data_ptr()
     elif lengths is not None:
@@ -247,15 +239,13 @@ def answer(cs: torch.Tensor, bias: torch.Tensor | None = None, allowed: torch.Te
     fre_p, fre, frequency = _knob(frequency, "frequency", n, dev, False)
     pre_p, pre, presence = _knob(presence, "presence", n, dev, False)
     tem_p, tem, temperature = _knob(temperature, "temperature", n, dev, True)
-    choice = torch.empty(n, dtype=torch.int64, device=dev)
-    logprob = torch.empty(n, dtype=torch.float32, device=dev)
-    z = torch.empty((n, k), dtype=torch.float32, device=dev) if adjusted else None
-    args = AnswerArgs(cs.data_ptr(), _row_stride(cs), n, k, _TYPES[cs.dtype],
-                      None if bias is None else bias.data_ptr(), bias_stride, allowed_p, allowed_stride,
-                      hist_p, hist_stride, hist_len, hist_64, lens_p, rep_p, fre_p, pre_p, tem_p, rep, fre, pre, tem,
-                      choice.data_ptr(), logprob.data_ptr(), None if z is None else z.data_ptr())
-    with _on(dev):
-        check(_lib.load().ytm_answer(ct.byref(args), _stream(dev)), "ytm_answer")
+    choice = _empty(n, dtype=_I64, device=dev)
+    logprob = _empty(n, dtype=_f32, device=dev)
+    z = _empty(n, k, dtype=_f32, device=dev) if adjusted else None
+    args = AnswerArgs(cs.data_ptr(), cs.stride(0) if n > 1 else 0, n, k, _TYPES[cs.dtype], bias_p, bias_stride, allowed_p,
+                      allowed_stride, hist_p, hist_stride, hist_len, hist_64, lens_p, rep_p, fre_p, pre_p, tem_p, rep,
+                      fre, pre, tem, choice.data_ptr(), logprob.data_ptr(), None if z is None else z.data_ptr())
+    _call(_lib.load().ytm_answer, "ytm_answer", dev, ct.byref(args))
     return choice, logprob, z
 
 
@@ -276,29 +266,38 @@ def class_loss(cs: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None
     and no gradient.  bias: float32 [k]; allowed as for `answer`; temperature:
     a positive number or float32 [1], whose value is not checked; weight:
     float32 [n]."""
-    cs = _need(cs, "cs", 2, tuple(_TYPES))
+    cs = _need(cs, "cs", 2, _SUMS)
     n, k = cs.shape
     dev = cs.device
     if k < 1:
         raise ValueError("cs must have at least one class")
     target = _vector(target, "target", n, _INDICES, dev)
+    bias_p = allowed_p = weight_p = dcs_p = dbias_p = ws_p = dcs = dbias = None
+    allowed_stride = 0
     if bias is not None:
-        bias = _vector(bias, "bias", k, (torch.float32,), dev)
-    allowed_p, allowed_stride, allowed = _allowed(allowed, n, k, dev)
+        bias = _vector(bias, "bias", k, _F32, dev)
+        bias_p = bias.data_ptr()
+    if allowed is not None:
+        allowed = _allowed(allowed, n, k, dev)
+        allowed_p, allowed_stride = allowed.data_ptr(), allowed.stride(0) if allowed.shape[0] > 1 else 0
     tem_p, tem, temperature = _knob(temperature, "temperature", 1, dev, True)
     if weight is not None:
-        weight = _vector(weight, "weight", n, (torch.float32,), dev)
-    lib = _lib.load()
-    loss = torch.empty(n, dtype=torch.float32, device=dev)
-    dcs = None if cs.dtype == torch.int32 else torch.empty((n, k), dtype=cs.dtype, device=dev)
-    dbias = None if bias is None else torch.empty(k, dtype=torch.float32, device=dev)
-    dtem = torch.empty(1, dtype=torch.float32, device=dev)
-    need = lib.ytm_class_loss_workspace_bytes(n, k, _TYPES[cs.dtype], _row_stride(cs))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    args = LossArgs(cs.data_ptr(), _row_stride(cs), n, k, _TYPES[cs.dtype], None if bias is None else bias.data_ptr(),
-                    allowed_p, allowed_stride, target.data_ptr(), None if weight is None else weight.data_ptr(), tem_p,
-                    tem, int(target.dtype == torch.int64), loss.data_ptr(), None if dcs is None else dcs.data_ptr(),
-                    None if dbias is None else dbias.data_ptr(), dtem.data_ptr())
-    with _on(dev):
-        check(lib.ytm_class_loss(ct.byref(args), None if ws is None else ws.data_ptr(), _stream(dev)), "ytm_class_loss")
+        weight = _vector(weight, "weight", n, _F32, dev)
+        weight_p = weight.data_ptr()
+    lib, cs_type, stride = _lib.load(), _TYPES[cs.dtype], cs.stride(0) if n > 1 else 0
+    loss = _empty(n, dtype=_f32, device=dev)
+    dtem = _empty(1, dtype=_f32, device=dev)
+    if cs_type != _lib.YTM_I32:
+        dcs = _empty(n, k, dtype=cs.dtype, device=dev)
+        dcs_p = dcs.data_ptr()
+    if bias is not None:
+        dbias = _empty(k, dtype=_f32, device=dev)
+        dbias_p = dbias.data_ptr()
+    need = lib.ytm_class_loss_workspace_bytes(n, k, cs_type, stride)
+    if need:
+        ws = _empty(need, dtype=torch.uint8, device=dev)
+        ws_p = ws.data_ptr()
+    args = LossArgs(cs.data_ptr(), stride, n, k, cs_type, bias_p, allowed_p, allowed_stride, target.data_ptr(), weight_p,
+                    tem_p, tem, target.dtype is _I64, loss.data_ptr(), dcs_p, dbias_p, dtem.data_ptr())
+    _call(lib.ytm_class_loss, "ytm_class_loss", dev, ct.byref(args), ws_p)
     return loss, dcs, dbias, dtem

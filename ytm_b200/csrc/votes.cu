@@ -2,6 +2,9 @@
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <limits.h>
+#include <string.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "elem.cuh"
@@ -588,7 +591,7 @@ struct Q4Plan {
     size_t smem;
 };
 
-static Q4Plan q4_plan(int64_t N, int64_t C, int64_t K, int x_type, int group) {
+static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group) {
     Q4Plan p = {};
     p.mode = x_type == YTM_BITS ? Q4_BITS : x_type == YTM_F32 || (N <= 2 && K >= 1024) ? Q4_DIGITS : x_type == YTM_F16 ? Q4_FP16 : Q4_BF16;
     p.parts = p.mode == Q4_DIGITS ? 4 : 1;
@@ -629,6 +632,31 @@ static Q4Plan q4_plan(int64_t N, int64_t C, int64_t K, int x_type, int group) {
     return p;
 }
 
+// The thread's last plan again if the sizes are the same: the workspace's size
+// and the call ask for it one after the other, and a server's calls are alike.
+static const Q4Plan &q4_plan(int64_t N, int64_t C, int64_t K, int x_type, int group) {
+    static thread_local int64_t of[6] = {-1, 0, 0, 0, 0, 0};
+    static thread_local Q4Plan plan;
+    const int64_t now[6] = {N, C, K, x_type, group, sm_count()};
+    if (memcmp(of, now, sizeof now)) {
+        plan = q4_plan_of(N, C, K, x_type, group);
+        memcpy(of, now, sizeof now);
+    }
+    return plan;
+}
+
+// Lets kernel f have `smem` bytes and clusters of 16, once for a device.
+template <typename F>
+static ytm_status allow_smem(F *f, int smem, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    ytm_status rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+    if (rc || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return rc;
+    if ((rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "q4 votes smem"))) return rc;
+    if ((rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "q4 votes cluster"))) return rc;
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return YTM_OK;
+}
+
 // cuTensorMapEncodeTiled, which the driver hands out by name.
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -647,12 +675,10 @@ static EncodeTiled encode_tiled() {
 
 template <Q4Mode MODE, int COLS, int GROUP>
 static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, dim3 grid, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
     auto *f = k_q4_votes<MODE, COLS, GROUP>;
-    ytm_status rc;
-    if ((rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem), "q4 votes smem")))
-        return rc;
-    if (p.cluster > 8 && (rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "q4 votes cluster")))
-        return rc;
+    ytm_status rc = allow_smem(f, 227 * 1024, done);
+    if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(Q4_THREADS);
@@ -731,7 +757,7 @@ ytm_status ytm_q4_pack(const void *weights, int32_t w_type, int64_t w_stride, in
 
 uint64_t ytm_q4_votes_workspace_bytes(int32_t x_type, int64_t N, int32_t C, int32_t K, int32_t group) {
     if (N <= 0 || check_q4(C, K, group, YTM_F32)) return 0;
-    const Q4Plan p = q4_plan(N, C, K, x_type, group);
+    const Q4Plan &p = q4_plan(N, C, K, x_type, group);
     return (uint64_t)p.z * p.xs_block;
 }
 
