@@ -19,7 +19,7 @@ NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-Xcompiler", "-fPIC", "-shared",
-    "--expt-relaxed-constexpr",
+    "--expt-relaxed-constexpr", "--threads", "0",
 ]
 
 
@@ -41,6 +41,36 @@ def sources() -> list[str]:
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
 
 
+BIND = os.path.join(HERE, "_answers.so")
+
+
+def _bind_stale() -> bool:
+    deps = [os.path.join(CSRC, "answers_bind.cpp"), os.path.join(HERE, "..", "include", "ytm.h"), LIB]
+    return not os.path.exists(BIND) or any(os.path.getmtime(d) > os.path.getmtime(BIND) for d in deps)
+
+
+def build_bind(force: bool = False, verbose: bool = False) -> str:
+    """The Python entry points of ytm_b200.answers over libytm.so."""
+    if not force and not _bind_stale():
+        return BIND
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", os.path.join(CSRC, "answers_bind.cpp"),
+           *("-I" + i for i in (*include_paths(), sysconfig.get_paths()["include"], cuda)), "-L" + torch_lib,
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-L" + HERE, "-l:libytm.so",
+           "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + torch_lib, "-o", BIND + ".tmp"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(BIND + ".tmp", BIND)
+    return BIND
+
+
 def _stale() -> bool:
     if not os.path.exists(LIB):
         return True
@@ -52,6 +82,7 @@ def _stale() -> bool:
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> str:
     if not force and not _stale():
+        build_bind(verbose=verbose)
         return LIB
     nvcc = os.environ.get("NVCC", "nvcc")
     tmp = LIB + ".tmp"
@@ -60,6 +91,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
+    build_bind(verbose=verbose)
     return LIB
 
 
