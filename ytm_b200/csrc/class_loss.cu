@@ -299,39 +299,11 @@ struct RowVecs {
     __device__ __forceinline__ RowVecs(const void *base, int64_t row_index, int64_t stride)
         : row((const T *)base + row_index * stride), off((int)((uintptr_t)row % 16 / sizeof(T))) {}
 
-    // Vectors first .. last lie inside the row, so that they can be moved whole.
-    __device__ __forceinline__ bool inside(int first, int last, int K) const {
-        return (first > 0 || (first == 0 && off == 0)) && (int64_t)(last + 1) * V <= (int64_t)off + K;
-    }
-
-    __device__ __forceinline__ uint4 load_whole(int i) const { return *(const uint4 *)(row - off + (int64_t)i * V); }
-    __device__ __forceinline__ void store_whole(int i, uint4 v) const { *(uint4 *)(row - off + (int64_t)i * V) = v; }
-
-    __device__ __forceinline__ uint4 load(int i, int K) const {
-        if (inside(i, i, K)) return load_whole(i);
-        if ((int64_t)i * V >= (int64_t)off + K) return make_uint4(0, 0, 0, 0);
-        alignas(16) T t[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int64_t k = (int64_t)i * V + j - off;
-            t[j] = k >= 0 && k < K ? row[k] : T(0.f);
-        }
-        return *(const uint4 *)t;
-    }
-
-    __device__ __forceinline__ void store(int i, int K, uint4 v) const {
-        if (inside(i, i, K)) {
-            store_whole(i, v);
-            return;
-        }
-        if ((int64_t)i * V >= (int64_t)off + K) return;
-        const T *t = (const T *)&v;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int64_t k = (int64_t)i * V + j - off;
-            if (k >= 0 && k < K) const_cast<T *>(row)[k] = t[j];
-        }
-    }
+    // Vectors first .. end - 1 lie inside the row; `slack` more classes must
+    // follow them.  The classes before and behind are taken one by one.
+    __device__ __forceinline__ int first() const { return off ? 1 : 0; }
+    __device__ __forceinline__ int end(int K, int slack = 0) const { return max(first(), (int)(((int64_t)off + K - slack) / V)); }
+    __device__ __forceinline__ const uint4 *at(int i) const { return (const uint4 *)(row - off + (int64_t)i * V); }
 };
 
 // Two fp32 operations in one instruction, on register pairs.
@@ -365,30 +337,21 @@ __device__ __forceinline__ F2 class_pair(const uint4 &raw, int q) {
     return pair(to_f32(v[2 * q]), to_f32(v[2 * q + 1]));
 }
 
-// Bits j: class k + j (of V) is there and allowed.
-template <int V, bool INSIDE>
-__device__ __forceinline__ uint32_t open_classes(const uint32_t *allowed, int k, int K) {
-    constexpr uint32_t ALL = (1u << V) - 1u;
-    uint32_t there = ALL;
-    if (!INSIDE) {
-        if (k >= K || k <= -V) return 0u;
-        if (k + V > K) there = (1u << (K - k)) - 1u;
-        if (k < 0) there &= ALL << -k;
-    }
-    if (!allowed) return there;
-    const int w = k >> 5;  // of a k below 0: the word before the first
-    const uint32_t lo = INSIDE || w >= 0 ? allowed[w] : 0u;
-    const uint32_t hi = (k & 31) + V > 32 && (INSIDE || (w + 1) * 32 < K) ? allowed[w + 1] : 0u;
-    return __funnelshift_r(lo, hi, k & 31) & there;
+// Bits j: class k + j (of V, all of them in the row) is allowed.
+template <int V>
+__device__ __forceinline__ uint32_t open_classes(const uint32_t *allowed, int k) {
+    if (!allowed) return ~0u;
+    const uint32_t *w = allowed + (k >> 5);
+    return __funnelshift_r(w[0], (k & 31) + V > 32 ? w[1] : 0u, k & 31);
 }
 
-// bias[k .. k + V) (0 where there is none), k = R below a multiple of four.
-template <int V, int R, bool INSIDE>
-__device__ __forceinline__ void load_bias(const float *bias, int k, int K, F2 (&b)[V / 2]) {
+// bias[k .. k + V), k = R below a multiple of four; reads up to R behind.
+template <int V, int R>
+__device__ __forceinline__ void load_bias(const float *bias, int k, F2 (&b)[V / 2]) {
     if (!bias) {
 #pragma unroll
         for (int q = 0; q < V / 2; ++q) b[q] = pair(0.f, 0.f);
-    } else if (INSIDE && (uintptr_t)bias % 16 == 0) {
+    } else if ((uintptr_t)bias % 16 == 0) {
         float f[V + 4];  // from the boundary at or below k
         const float *from = bias + (R ? k + R - 4 : k);
 #pragma unroll
@@ -397,17 +360,15 @@ __device__ __forceinline__ void load_bias(const float *bias, int k, int K, F2 (&
         for (int q = 0; q < V / 2; ++q) b[q] = pair(f[(R ? 4 - R : 0) + 2 * q], f[(R ? 4 - R : 0) + 2 * q + 1]);
     } else {
 #pragma unroll
-        for (int q = 0; q < V / 2; ++q)
-            b[q] = pair(k + 2 * q >= 0 && k + 2 * q < K ? bias[k + 2 * q] : 0.f,
-                        k + 2 * q + 1 >= 0 && k + 2 * q + 1 < K ? bias[k + 2 * q + 1] : 0.f);
+        for (int q = 0; q < V / 2; ++q) b[q] = pair(bias[k + 2 * q], bias[k + 2 * q + 1]);
     }
 }
 
-// (m, s, h) of `rounds` rounds of NVS * LB_THREADS vectors of one row: block
+// (m, s, h) of `rounds` rounds of NV * LB_THREADS vectors of one row: block
 // (part, row).
-template <typename T, int NVS>
+template <typename T, int NV>
 __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args a, LossStat *__restrict__ stats, int rounds) {
-    constexpr int V = RowVecs<T>::V, STEP = NVS * LB_THREADS;
+    constexpr int V = RowVecs<T>::V, STEP = NV * LB_THREADS;
     __shared__ LossStat warp_stat[LB_THREADS / 32];
     const int K = a.k;
     const int64_t n = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
@@ -417,78 +378,70 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
     const RowVecs<T> row(a.cs, n, a.cs_stride);
     const uint32_t *allowed = a.allowed ? a.allowed + n * a.allowed_stride : nullptr;
     LossStat st = {-INFINITY, 0.f, 0.f};
-    const auto round = [&](int i0, auto below, auto count, auto inside) {
-        constexpr int R = decltype(below)::value, NV = decltype(count)::value;
-        constexpr bool INSIDE = decltype(inside)::value;
-        uint4 raw[NV];
-        uint32_t open[NV];
+    const int first = row.first(), below = row.off & 3, end = row.end(K, below);  // the bias is read up to the next boundary
+    const auto stream = [&](auto r) {
+        constexpr int R = decltype(r)::value;
+        const int64_t from = (int64_t)blockIdx.x * rounds * STEP;
+        const int to = (int)min((int64_t)end, first + from + (int64_t)rounds * STEP);
+        for (int i0 = (int)min((int64_t)end, first + from) + (int)threadIdx.x; i0 - (int)threadIdx.x < to; i0 += STEP) {
+            uint4 raw[NV];
+            uint32_t open[NV];
+            F2 b[NV][V / 2];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = i0 + j * LB_THREADS + (int)threadIdx.x;
-            raw[j] = INSIDE ? row.load_whole(i) : row.load(i, K);
-            open[j] = open_classes<V, INSIDE>(allowed, i * V - row.off, K);
-        }
-        float z[NV][V], m = st.m;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            F2 b[V / 2];
-            load_bias<V, R, INSIDE>(a.bias, (i0 + j * LB_THREADS + (int)threadIdx.x) * V - row.off, K, b);
-#pragma unroll
-            for (int q = 0; q < V / 2; ++q) {
-                float x, y;
-                split(fma2(class_pair<T>(raw[j], q), c2, mul2(b[q], c2)), x, y);
-                z[j][2 * q] = open[j] & (1u << (2 * q)) ? x : -INFINITY;
-                z[j][2 * q + 1] = open[j] & (2u << (2 * q)) ? y : -INFINITY;
-                m = fmaxf(m, fmaxf(z[j][2 * q], z[j][2 * q + 1]));
+            for (int j = 0; j < NV; ++j) {
+                const int i = min(i0 + j * LB_THREADS, to - 1), k = i * V - row.off;
+                raw[j] = *row.at(i);
+                open[j] = open_classes<V>(allowed, k);
+                load_bias<V, R>(a.bias, k, b[j]);
+                if (i0 + j * LB_THREADS >= to) open[j] = 0;
             }
-        }
-        const float base = m == -INFINITY ? 0.f : -m;  // nothing yet: every e is 0
-        const float d = st.m == m ? 0.f : st.m - m, f = ex2(d);
-        F2 s = pair(f * st.s, 0.f), h = pair(f * fmaf(st.s, fmaxf(d, -1024.f), st.h), 0.f);
-        const F2 base2 = pair(base, base);
-        st.m = m;
+            float z[NV][V], m = st.m;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+            for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int q = 0; q < V / 2; ++q) {
-                float x, y;
-                split(add2(pair(z[j][2 * q], z[j][2 * q + 1]), base2), x, y);
-                const F2 e = pair(ex2(x), ex2(y));
-                s = add2(s, e);
-                h = fma2(e, pair(fmaxf(x, -1024.f), fmaxf(y, -1024.f)), h);  // 0 * -inf counts for nothing
-            }
-        float x, y;
-        split(s, x, y);
-        st.s = x + y;
-        split(h, x, y);
-        st.h = x + y;
-    };
-    const int vecs = (int)(((int64_t)row.off + K + V - 1) / V);
-    const int64_t first = (int64_t)blockIdx.x * rounds * STEP;
-    const int end = (int)min((int64_t)vecs, first + (int64_t)rounds * STEP);
-    const int warp_vec = threadIdx.x & ~31;
-    // a warp's vectors from i0 on, LB_THREADS apart, lie inside the row (and the
-    // bias up to the next boundary, to which it is read)
-    const auto warp_inside = [&](int i0, int count, int below) {
-        const int last = i0 + (count - 1) * LB_THREADS + warp_vec + 31;
-        return row.inside(i0 + warp_vec, last, K) && (int64_t)(last + 1) * V - row.off + below <= K;
-    };
-    const auto stream = [&](auto below) {
-        int i0 = (int)first;
-        for (; i0 + STEP <= end; i0 += STEP) {
-            if (warp_inside(i0, NVS, below)) round(i0, below, std::integral_constant<int, NVS>(), std::true_type());
-            else round(i0, below, std::integral_constant<int, NVS>(), std::false_type());
-        }
-        for (; i0 + warp_vec < end; i0 += LB_THREADS) {
-            if (warp_inside(i0, 1, below)) round(i0, below, std::integral_constant<int, 1>(), std::true_type());
-            else round(i0, below, std::integral_constant<int, 1>(), std::false_type());
+                for (int q = 0; q < V / 2; ++q) {
+                    float x, y;
+                    split(fma2(class_pair<T>(raw[j], q), c2, mul2(b[j][q], c2)), x, y);
+                    z[j][2 * q] = open[j] & (1u << (2 * q)) ? x : -INFINITY;
+                    z[j][2 * q + 1] = open[j] & (2u << (2 * q)) ? y : -INFINITY;
+                    m = fmaxf(m, fmaxf(z[j][2 * q], z[j][2 * q + 1]));
+                }
+            const float base = m == -INFINITY ? 0.f : -m;  // nothing yet: every e is 0
+            const float d = st.m == m ? 0.f : st.m - m, f = ex2(d);
+            F2 s = pair(f * st.s, 0.f), h = pair(f * fmaf(st.s, fmaxf(d, -1024.f), st.h), 0.f);
+            const F2 base2 = pair(base, base);
+            st.m = m;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int q = 0; q < V / 2; ++q) {
+                    float x, y;
+                    split(add2(pair(z[j][2 * q], z[j][2 * q + 1]), base2), x, y);
+                    const F2 e = pair(ex2(x), ex2(y));
+                    s = add2(s, e);
+                    h = fma2(e, pair(fmaxf(x, -1024.f), fmaxf(y, -1024.f)), h);  // 0 * -inf counts for nothing
+                }
+            float x, y;
+            split(s, x, y);
+            st.s = x + y;
+            split(h, x, y);
+            st.h = x + y;
         }
     };
-    switch (row.off & 3) {  // where the bias lies against the vectors: the same for the block
+    switch (below) {  // where the bias lies against the vectors: the same for the block
         case 0: stream(std::integral_constant<int, 0>()); break;
         case 1: stream(std::integral_constant<int, 1>()); break;
         case 2: stream(std::integral_constant<int, 2>()); break;
         default: stream(std::integral_constant<int, 3>()); break;
+    }
+    if (blockIdx.x == 0) {  // the classes before the first and behind the last vector
+        const int head = first * V - (first ? row.off : 0), tail = end * V - row.off;
+        const int k = (int)threadIdx.x < head ? (int)threadIdx.x : tail + ((int)threadIdx.x - head);
+        if (k < K && is_allowed(allowed, k)) {
+            const float z = loss_z(to_f32(row.row[k]), a.bias ? __fmul_rn(a.bias[k], c) : 0.f, c);
+            // z itself if it is no number, so that it reaches the sum
+            st = merge(st, {z, z == z ? (z == -INFINITY ? 0.f : 1.f) : z, 0.f});
+        }
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1)
@@ -510,7 +463,9 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
 // classes from row to row, with a period of 2, 4 or 8 rows: a chunk takes every
 // `period`-th row only, so that its threads keep their classes, and loads,
 // stores and sums of dbias need no shift.  Tile 0 writes the losses and the
-// chunk's part of the temperature's gradient.
+// chunk's part of the temperature's gradient, and takes the classes outside
+// the row's whole vectors; where the class sums' rows lie otherwise than the
+// gradients', all classes are taken one by one.
 constexpr int LB_ROWS = 128;  // rows of a chunk at most
 
 struct GradRow {
@@ -561,105 +516,122 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
         else if (a.dtemperature) *a.dtemperature = (float)(-dt * (double)LN2 * (double)rt);
     }
     if (!a.dcs && !a.dbias) return;
-    const int64_t row0 = min(n0, a.n - 1);
-    const RowVecs<T> in0(a.cs, row0, a.cs_stride), out0(a.dcs ? a.dcs : a.cs, row0, a.dcs ? K : a.cs_stride);
-    const bool same = in0.off == out0.off;  // else the vectors are those of the gradients
-    const int vec = (int)(blockIdx.x * LB_THREADS + threadIdx.x);
-    const int k0 = vec * V - out0.off, warp_k = k0 - lane * V;
-    const F2 c2 = pair(c, c);
-    F2 bc[V / 2], acc[V / 2];
-    load_bias<V, 0, false>(a.bias, k0, K, bc);
-#pragma unroll
-    for (int q = 0; q < V / 2; ++q) {
-        bc[q] = mul2(bc[q], c2);
-        acc[q] = pair(0.f, 0.f);
-    }
-    const uint32_t shared_open = open_classes<V, false>(a.allowed_stride ? nullptr : a.allowed, k0, K);
-    const int64_t in_step = (int64_t)period * a.cs_stride, out_step = (int64_t)period * K;
-    const uint32_t *mask_word = a.allowed_stride ? a.allowed + row0 * a.allowed_stride + (k0 >> 5) : nullptr;
+    float *const db = !a.dbias ? nullptr : chunks == 1 ? a.dbias : part.db + (int64_t)blockIdx.y * K;
+    const int64_t row0 = min(n0, a.n - 1), in_step = (int64_t)period * a.cs_stride, out_step = (int64_t)period * K;
     const int64_t mask_step = (int64_t)period * a.allowed_stride;
-    const bool straddle = (k0 & 31) + V > 32;
-    const auto stream = [&](auto inside) {
-        constexpr bool INSIDE = decltype(inside)::value;
-        RowVecs<T> in = in0;
-        [[maybe_unused]] RowVecs<T> out = out0;
-        const uint32_t *mask = mask_word;
-        for (int i0 = 0; i0 < count; i0 += U) {
-            uint4 raw[U];
-            uint32_t open[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                raw[u] = make_uint4(0, 0, 0, 0);
-                open[u] = shared_open;
-                if (i0 + u < count) {
-                    if (INSIDE) {
-                        raw[u] = in.load_whole(vec);
-                        if (a.allowed_stride) open[u] = __funnelshift_r(mask[0], straddle ? mask[1] : 0u, k0 & 31);
-                    } else {
-                        if (same) {
-                            raw[u] = in.load(vec, K);
-                        } else {
-                            T *t = (T *)&raw[u];
-#pragma unroll
-                            for (int j = 0; j < V; ++j) t[j] = k0 + j >= 0 && k0 + j < K ? in.row[k0 + j] : T(0.f);
-                        }
-                        if (a.allowed_stride) open[u] = open_classes<V, false>(mask - (k0 >> 5), k0, K);
-                    }
-                }
-                in.row += in_step;
-                mask += mask_step;
+    const uint32_t *const mask0 = a.allowed ? a.allowed + row0 * a.allowed_stride : nullptr;
+    const RowVecs<T> in0(a.cs, row0, a.cs_stride), out0(a.dcs ? a.dcs : a.cs, row0, a.dcs ? K : a.cs_stride);
+    // One class over the chunk's rows.
+    const auto column = [&](int k) {
+        const float bc = a.bias ? __fmul_rn(a.bias[k], c) : 0.f;
+        const T *in = in0.row + k;
+        const uint32_t *mask = mask0 ? mask0 + (k >> 5) : nullptr;
+        T *out = a.dcs ? (T *)a.dcs + row0 * (int64_t)K + k : nullptr;
+        float sum = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < count; ++i, in += in_step) {
+            const GradRow r = rows[i];
+            float d = 0.f;
+            if (r.y >= 0) {
+                if (!mask || (*mask >> (k & 31)) & 1u) d = ex2(loss_z(to_f32(*in), bc, c) - r.m) * r.f;
+                if (r.y == k) d -= r.wt;
+                sum += d;
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (i0 + u >= count) break;
-                const GradRow r = rows[i0 + u];
-                float d[V];
-                if (r.y >= 0) {
-                    const F2 m2 = pair(-r.m, -r.m), f2 = pair(r.f, r.f);
-#pragma unroll
-                    for (int q = 0; q < V / 2; ++q) {
-                        float x, y;
-                        split(add2(fma2(class_pair<T>(raw[u], q), c2, bc[q]), m2), x, y);
-                        x = open[u] & (1u << (2 * q)) ? ex2(x) : 0.f;
-                        y = open[u] & (2u << (2 * q)) ? ex2(y) : 0.f;
-                        split(mul2(pair(x, y), f2), d[2 * q], d[2 * q + 1]);
-                    }
-                    if (r.y >= warp_k && r.y - warp_k < 32 * V) {  // the label's class is this warp's
-#pragma unroll
-                        for (int j = 0; j < V; ++j)
-                            if (r.y - k0 == j) d[j] -= r.wt;
-                    }
-#pragma unroll
-                    for (int q = 0; q < V / 2; ++q) acc[q] = add2(acc[q], pair(d[2 * q], d[2 * q + 1]));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) d[j] = 0.f;
-                }
-                if constexpr (!std::is_integral<T>::value) {
-                    if (a.dcs) {
-                        alignas(16) T t[V];
-#pragma unroll
-                        for (int j = 0; j < V; ++j) t[j] = from_f32<T>(d[j]);
-                        const uint4 w = *(const uint4 *)t;
-                        if (INSIDE) out.store_whole(vec, w);
-                        else out.store(vec, K, w);
-                        out.row += out_step;
-                    }
+            if (mask) mask += mask_step;
+            if constexpr (!std::is_integral<T>::value) {
+                if (out) {
+                    *out = from_f32<T>(d);
+                    out += out_step;
                 }
             }
         }
+        if (db) db[k] = sum;
     };
-    if (same && out0.inside(vec - lane, vec - lane + 31, K)) stream(std::true_type());
-    else stream(std::false_type());
-    if (a.dbias) {
-        float *db = chunks == 1 ? a.dbias : part.db + (int64_t)blockIdx.y * K;
+    const int tile = blockIdx.x * LB_THREADS;
+    if (in0.off != out0.off) {
+        const int k1 = (int)min((int64_t)K, (int64_t)(tile + LB_THREADS) * V);
+        for (int k = tile * V + (int)threadIdx.x; k < k1; k += LB_THREADS) column(k);
+        return;
+    }
+    const int first = in0.first(), end = in0.end(K);
+    if (blockIdx.x == 0) {
+        const int head = first * V - (first ? in0.off : 0), tail = end * V - in0.off;
+        const int k = (int)threadIdx.x < head ? (int)threadIdx.x : tail + ((int)threadIdx.x - head);
+        if (threadIdx.x < 32 && k < K) column(k);
+    }
+    const int vec = first + tile + (int)threadIdx.x;
+    if (vec >= end) return;
+    const int k0 = vec * V - in0.off, warp_k = k0 - lane * V;
+    const F2 c2 = pair(c, c);
+    F2 bc[V / 2], acc[V / 2];
+#pragma unroll
+    for (int q = 0; q < V / 2; ++q) {
+        bc[q] = a.bias ? mul2(pair(a.bias[k0 + 2 * q], a.bias[k0 + 2 * q + 1]), c2) : pair(0.f, 0.f);
+        acc[q] = pair(0.f, 0.f);
+    }
+    const uint32_t shared_open = open_classes<V>(a.allowed_stride ? nullptr : a.allowed, k0);
+    const bool straddle = (k0 & 31) + V > 32;
+    const char *in = (const char *)in0.at(vec);
+    char *out = (char *)out0.at(vec);
+    const uint32_t *mask = mask0 + (k0 >> 5);
+    for (int i0 = 0; i0 < count; i0 += U) {
+        uint4 raw[U];
+        uint32_t open[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            raw[u] = make_uint4(0, 0, 0, 0);
+            open[u] = shared_open;
+            if (i0 + u < count) {
+                raw[u] = *(const uint4 *)in;
+                if (a.allowed_stride) open[u] = __funnelshift_r(mask[0], straddle ? mask[1] : 0u, k0 & 31);
+            }
+            in += in_step * (int64_t)sizeof(T);
+            mask += mask_step;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u >= count) break;
+            const GradRow r = rows[i0 + u];
+            float d[V];
+            if (r.y >= 0) {
+                const F2 m2 = pair(-r.m, -r.m), f2 = pair(r.f, r.f);
+#pragma unroll
+                for (int q = 0; q < V / 2; ++q) {
+                    float x, y;
+                    split(add2(fma2(class_pair<T>(raw[u], q), c2, bc[q]), m2), x, y);
+                    x = open[u] & (1u << (2 * q)) ? ex2(x) : 0.f;
+                    y = open[u] & (2u << (2 * q)) ? ex2(y) : 0.f;
+                    split(mul2(pair(x, y), f2), d[2 * q], d[2 * q + 1]);
+                }
+                if (r.y >= warp_k && r.y - warp_k < 32 * V) {  // the label's class is this warp's
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (r.y - k0 == j) d[j] -= r.wt;
+                }
+#pragma unroll
+                for (int q = 0; q < V / 2; ++q) acc[q] = add2(acc[q], pair(d[2 * q], d[2 * q + 1]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) d[j] = 0.f;
+            }
+            if constexpr (!std::is_integral<T>::value) {
+                if (a.dcs) {
+                    alignas(16) T t[V];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) t[j] = from_f32<T>(d[j]);
+                    *(uint4 *)out = *(const uint4 *)t;
+                    out += out_step * (int64_t)sizeof(T);
+                }
+            }
+        }
+    }
+    if (db) {
 #pragma unroll
         for (int q = 0; q < V / 2; ++q) {
-            const int k = k0 + 2 * q;
             float x, y;
             split(acc[q], x, y);
-            if (k >= 0 && k < K) db[k] = x;
-            if (k + 1 >= 0 && k + 1 < K) db[k + 1] = y;
+            db[k0 + 2 * q] = x;
+            db[k0 + 2 * q + 1] = y;
         }
     }
 }
@@ -723,7 +695,7 @@ static LossPlan loss_plan(int64_t n, int64_t k, int64_t elem, int64_t cs_stride)
     }
     p.big = true;
     // parts of a row until every SM has about eight blocks
-    const int64_t vecs = cdiv(k * elem, 16) + 1;  // a row off a boundary can reach into one more
+    const int64_t vecs = cdiv(k * elem, 16);
     p.nv = vecs <= LB_THREADS ? 1 : (int)elem;    // 16 classes of a thread in a round
     const int64_t rounds = cdiv(vecs, (int64_t)LB_THREADS * p.nv);
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(32, cdiv(sms * 4, n)));
@@ -776,7 +748,7 @@ static ytm_status launch_big(const ytm_loss_args &a, const LossPlan &p, const Lo
     else k_loss_stat<T, (int)sizeof(T)><<<grid, LB_THREADS, 0, st>>>(a, stats, p.rounds);
     ytm_status rc = launch_check("class loss statistics");
     if (rc) return rc;
-    const uint64_t vecs = cdiv((uint64_t)a.k * sizeof(T), 16) + (p.period > 1 || (uintptr_t)a.cs % 16 || (uintptr_t)a.dcs % 16);
+    const uint64_t vecs = cdiv((uint64_t)a.k * sizeof(T), 16);
     const unsigned tiles = a.dcs || a.dbias ? (unsigned)cdiv(vecs, LB_THREADS) : 1;
     return launch_after(k_loss_grad<T>, dim3(tiles, (unsigned)p.teams), LB_THREADS, st, "class loss", a, stats, p.parts,
                         p.chunk, p.period, part);
