@@ -570,24 +570,27 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
         acc[q] = pair(0.f, 0.f);
     }
     const uint32_t shared_open = open_classes<V>(a.allowed_stride ? nullptr : a.allowed, k0);
-    const bool straddle = (k0 & 31) + V > 32;
+    const bool straddle = (k0 & 31) + V > 32, masked = a.allowed_stride != 0;
     const char *in = (const char *)in0.at(vec);
     char *out = (char *)out0.at(vec);
     const uint32_t *mask = mask0 + (k0 >> 5);
     for (int i0 = 0; i0 < count; i0 += U) {
         uint4 raw[U];
-        uint32_t open[U];
+        uint32_t open[U], lo[U], hi[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < U; ++u) {  // loads only: a use between them would wait for each in turn
             raw[u] = make_uint4(0, 0, 0, 0);
-            open[u] = shared_open;
+            lo[u] = hi[u] = 0u;
             if (i0 + u < count) {
                 raw[u] = *(const uint4 *)in;
-                if (a.allowed_stride) open[u] = __funnelshift_r(mask[0], straddle ? mask[1] : 0u, k0 & 31);
+                if (masked) lo[u] = mask[0];
+                if (masked && straddle) hi[u] = mask[1];
             }
             in += in_step * (int64_t)sizeof(T);
             mask += mask_step;
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) open[u] = masked ? __funnelshift_r(lo[u], hi[u], k0 & 31) : shared_open;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (i0 + u >= count) break;
