@@ -32,9 +32,8 @@ struct Best {
 
 // Order of numpy's argmax: NaN above all numbers, the lowest class of equals.
 __device__ __forceinline__ bool above(float z, int k, float z2, int k2) {
-    const bool n = z != z, n2 = z2 != z2;
-    if (n || n2) return n && (!n2 || k < k2);
-    return z > z2 || (z == z2 && k < k2);
+    const bool n = z != z, n2 = z2 != z2, equal = n == n2 && (n || z == z2);
+    return (z > z2) | (n & !n2) | (equal & (k < k2));
 }
 
 __device__ __forceinline__ float exp_of(float x) {  // within a few steps and x's rounding
@@ -84,27 +83,31 @@ __device__ __forceinline__ double penalised(double v, uint32_t count, const Answ
     return v * (v > 0.0 ? o.rr : (double)o.r) - (double)o.f * (double)count - (double)o.p;
 }
 
-// The best of E classes of a thread and the others' sum.
+// The best of E classes of a thread (z: -inf where closed) and the others' sum.
 template <int E, typename K>
 __device__ __forceinline__ Best best_of(const float (&z)[E], uint32_t open, K class_of) {
-    Best b = {-INFINITY, INT_MAX, 0.f};
-    int at = -1;
+    float m = z[0];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        if (!((open >> e) & 1u)) continue;
-        if (at < 0 || z[e] > b.z || (z[e] != z[e] && b.z == b.z)) {
-            b.z = z[e];
-            at = e;
+    for (int e = 1; e < E; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(z[e]));
+    int at = 0;
+    float s = 0.f;
+    if (m > -INFINITY) {  // a number, and no closed class has it
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e) at = z[e] == m ? e : at;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float x = exp_of(z[e] - m);
+            s += e == at ? 0.f : x;
         }
-    }
-    if (at < 0) return b;
+    } else {  // nothing open, -inf everywhere, or a NaN
+        if (!open) return {-INFINITY, INT_MAX, 0.f};
+        at = -1;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float x = exp_of(z[e] - b.z);
-        if ((open >> e) & 1u && e != at) b.s += x;
+        for (int e = E - 1; e >= 0; --e)
+            if (((open >> e) & 1u) && (m == -INFINITY || z[e] != z[e])) at = e;
+        if (m != m || __popc(open) > 1) s = NAN;
     }
-    b.k = class_of(at);
-    return b;
+    return {m, class_of(at), s};
 }
 
 __device__ __forceinline__ void write_answer(const ytm_answer_args &a, int64_t n, const Best &b) {
@@ -118,19 +121,18 @@ constexpr int AN_THREADS = 256;
 // -------------------------------------------------- rows of few classes
 // TPR threads hold a row, E classes each, neighbouring lanes neighbouring classes.
 
-template <typename T, int TPR, int E>
+template <typename T, int TPR, int E, bool HIST>
 __global__ void __launch_bounds__(AN_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_answer_small(const ytm_answer_args a) {
     constexpr int ROWS = AN_THREADS / TPR;
     extern __shared__ uint32_t counts[];  // [ROWS][TPR * E], with a history
     const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR, K = a.k;
     uint32_t *const mine = counts + team * TPR * E;
-    uint32_t there = 0, shared_open = 0;
+    uint32_t shared_open = 0;
     float b[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int k = e * TPR + lane;
         b[e] = a.bias && k < K && !a.bias_stride ? a.bias[k] : 0.f;
-        if (k < K) there |= 1u << e;
         if (k < K && (a.allowed_stride || is_allowed(a.allowed, k))) shared_open |= 1u << e;
     }
     struct Row {
@@ -141,16 +143,20 @@ __global__ void __launch_bounds__(AN_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_an
     const auto fetch = [&](int64_t n0) {
         Row r;
         const int64_t n = clamped(n0 + team);
-        const T *cs = (const T *)a.cs + n * a.cs_stride;
+        const T *cs = (const T *)a.cs + n * a.cs_stride + lane;
         r.open = shared_open;
 #pragma unroll
-        for (int e = 0; e < E; ++e) r.v[e] = (there >> e) & 1u ? cs[e * TPR + lane] : T(0.f);
+        for (int e = 0; e < E; ++e) r.v[e] = e * TPR + lane < K ? cs[e * TPR] : T(0.f);
         if (a.allowed_stride) {
             const uint32_t *w = a.allowed + n * a.allowed_stride;
             uint32_t bits = 0;
+            constexpr int STEP = TPR < 32 ? 32 / TPR : 1;  // classes of a thread in a word
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if ((there >> e) & 1u) bits |= (w[(e * TPR + lane) >> 5] >> ((e * TPR + lane) & 31) & 1u) << e;
+            for (int e0 = 0; e0 < E; e0 += STEP) {
+                const uint32_t word = e0 * TPR < K ? w[e0 * TPR / 32] >> lane : 0u;
+#pragma unroll
+                for (int e = e0; e < E && e < e0 + STEP; ++e) bits |= (word >> ((e - e0) * TPR) & 1u) << e;
+            }
             r.open &= bits;
         }
         return r;
@@ -164,7 +170,7 @@ __global__ void __launch_bounds__(AN_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_an
         const bool live = n0 + team < a.n;
         const int64_t n = clamped(n0 + team);
         const AnswerRow o = answer_row(a, n);
-        if (a.history) {
+        if (HIST) {
             __syncwarp();
 #pragma unroll
             for (int e = 0; e < E; ++e) mine[e * TPR + lane] = 0;
@@ -175,24 +181,29 @@ __global__ void __launch_bounds__(AN_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_an
             }
             __syncwarp();
         }
+        if (a.bias_stride) {
+            const float *bias = a.bias + n * a.bias_stride + lane;
+#pragma unroll
+            for (int e = 0; e < E; ++e) b[e] = e * TPR + lane < K ? bias[e * TPR] : 0.f;
+        }
         float z[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             double v = to_f64(row.v[e]);
-            if (a.history) {
+            if (HIST) {
                 const uint32_t c = mine[e * TPR + lane];
                 if (c) v = penalised(v, c, o);
             }
-            if (a.bias) v += (double)(a.bias_stride ? ((there >> e) & 1u ? a.bias[n * a.bias_stride + e * TPR + lane] : 0.f) : b[e]);
-            z[e] = (row.open >> e) & 1u ? (float)(v * o.rt) : -INFINITY;
+            z[e] = row.open & (1u << e) ? (float)((v + (double)b[e]) * o.rt) : -INFINITY;
         }
         Best best = best_of(z, row.open, [&](int e) { return e * TPR + lane; });
         best = merge_lanes(best, TPR);
         if (!live) continue;
         if (a.adjusted) {
+            float *const out = a.adjusted + n * (int64_t)K + lane;
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if ((there >> e) & 1u) a.adjusted[n * (int64_t)K + e * TPR + lane] = z[e];
+                if (e * TPR + lane < K) out[e * TPR] = z[e];
         }
         if (lane == 0) write_answer(a, n, best);
     }
@@ -203,8 +214,8 @@ __global__ void __launch_bounds__(AN_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_an
 // Classes whose counts a block holds.
 constexpr int AN_COUNTS = 8192;
 
-template <typename T, int THREADS, int E>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : E == 16 ? 3 : 4) k_answer_big(const ytm_answer_args a, int cluster, int part) {
+template <typename T, int THREADS, int E, bool HIST>
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 4) k_answer_big(const ytm_answer_args a, int cluster, int part) {
     __shared__ Best warp_best[32], block_best;
     extern __shared__ uint32_t counts[];  // [AN_COUNTS], with a history
     const int tid = threadIdx.x;
@@ -218,7 +229,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : E == 16 ? 3 : 4
     Best best = {-INFINITY, INT_MAX, 0.f};
     for (int c0 = from; c0 < to; c0 += AN_COUNTS) {
         const int c1 = (int)min((int64_t)to, (int64_t)c0 + AN_COUNTS);
-        if (o.len) {
+        if (HIST) {
             __syncthreads();
             for (int i = tid; i < c1 - c0; i += THREADS) counts[i] = 0;
             __syncthreads();
@@ -231,27 +242,35 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : E == 16 ? 3 : 4
             float z[E], b[E];
             uint32_t open = 0;
             T v[E];
+            uint32_t word[E];
+            const T *in = cs + k0;
+            const float *bin = bias ? bias + k0 : nullptr;
+            const uint32_t *win = allowed ? allowed + (k0 >> 5) : nullptr;
+            // the tiles start at multiples of 32: a warp's bits are one word
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const int k = k0 + e * THREADS;
-                const bool there = k < c1;
-                v[e] = there ? cs[k] : T(0.f);
-                b[e] = there && bias ? bias[k] : 0.f;
-                // c0 and the tiles are multiples of 32: a warp's bits are one word
-                if (there) open |= (allowed ? allowed[k >> 5] >> (k & 31) & 1u : 1u) << e;
+                const bool there = k0 + e * THREADS < c1;
+                v[e] = there ? in[e * THREADS] : T(0.f);
+                b[e] = there && bin ? bin[e * THREADS] : 0.f;
+                word[e] = !there ? 0u : win ? win[e * (THREADS / 32)] : ~0u;
             }
-            if (o.len && k0 == c0 + tid) __syncthreads();  // the counts are there
+#pragma unroll
+            for (int e = 0; e < E; ++e) open |= (word[e] >> (k0 & 31) & 1u) << e;
+            if (HIST && k0 == c0 + tid) __syncthreads();  // the counts are there
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const int k = k0 + e * THREADS;
                 double x = to_f64(v[e]);
-                if (o.len && k < c1) {
-                    const uint32_t c = counts[k - c0];
+                if (HIST) {
+                    const uint32_t c = counts[k0 - c0 + e * THREADS];  // behind c1: not open
                     if (c) x = penalised(x, c, o);
                 }
-                if (bias) x += (double)b[e];
-                z[e] = (open >> e) & 1u ? (float)(x * o.rt) : -INFINITY;
-                if (a.adjusted && k < c1) a.adjusted[n * a.k + k] = z[e];
+                z[e] = open & (1u << e) ? (float)((x + (double)b[e]) * o.rt) : -INFINITY;
+            }
+            if (a.adjusted) {
+                float *const out = a.adjusted + n * a.k + k0;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (k0 + e * THREADS < c1) out[e * THREADS] = z[e];
             }
             best = merge(best, best_of(z, open, [&](int e) { return k0 + e * THREADS; }));
         }
@@ -280,7 +299,8 @@ template <typename T, int TPR, int E>
 static ytm_status launch_small(const ytm_answer_args &a, cudaStream_t st) {
     const int64_t rows = AN_THREADS / TPR;
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.n, rows), (int64_t)sm_count() * (E == 16 ? 2 : E == 8 ? 3 : 4));
-    k_answer_small<T, TPR, E><<<grid, AN_THREADS, a.history ? AN_THREADS * E * 4 : 0, st>>>(a);
+    if (a.history) k_answer_small<T, TPR, E, true><<<grid, AN_THREADS, AN_THREADS * E * 4, st>>>(a);
+    else k_answer_small<T, TPR, E, false><<<grid, AN_THREADS, 0, st>>>(a);
     return launch_check("answer");
 }
 
@@ -299,7 +319,7 @@ static ytm_status launch_big(const ytm_answer_args &a, int cluster, cudaStream_t
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    auto *f = k_answer_big<T, THREADS, E>;
+    auto *f = a.history ? k_answer_big<T, THREADS, E, true> : k_answer_big<T, THREADS, E, false>;
     ytm_status rc;
     if (cluster > 8 && (rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "answer cluster")))
         return rc;
@@ -314,14 +334,13 @@ static ytm_status launch_answer(const ytm_answer_args &a, cudaStream_t st) {
     if (a.k <= 256) return launch_small<T, 16, 16>(a, st);
     if (a.k <= 512) return launch_small<T, 32, 16>(a, st);
     if (a.k <= 1024) return launch_big<T, 256, 4>(a, 1, st);
-    if (a.k <= 2048) return launch_big<T, 256, 8>(a, 1, st);
     // few rows: wide blocks, and clusters of them while every block has an SM
-    if (a.n <= sm_count()) {
+    if (a.k > 2048 && a.n <= sm_count()) {
         int cluster = 1;
         while (cluster < 16 && a.n * cluster * 2 <= sm_count() && a.k > cluster * 8192) cluster *= 2;
         return launch_big<T, 1024, 8>(a, cluster, st);
     }
-    return launch_big<T, 256, 16>(a, 1, st);
+    return launch_big<T, 256, 8>(a, 1, st);
 }
 
 }  // namespace ytm
