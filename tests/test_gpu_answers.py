@@ -198,7 +198,10 @@ def check_answer(got, cst, kw):
     (1, 1, 0, None, None), (1, 2, 1, None, "class"), (3, 10, 5, "row", "class"), (7, 31, 0, "all", "row"),
     (64, 100, 33, "row", None), (5, 257, 40, None, "row"), (33, 1000, 100, "all", "class"), (2, 1025, 0, "row", "row"),
     (3, 4099, 700, "row", "class"), (1, 8193, 9000, "all", None), (2, 40001, 300, "row", "class"),
-    (1, 131072, 2000, "row", "class"), (200, 3, 2, None, "class")])
+    (1, 131072, 2000, "row", "class"), (200, 3, 2, None, "class"),
+    # clusters without a history, blocks of many tiles, more than fit one count
+    (1, 131072, 0, None, "class"), (2, 70001, 0, "row", None), (160, 9000, 0, None, None), (150, 20000, 30, "row", "class"),
+    (1, 300001, 50, None, None)])
 def test_answer(n, k, hist, mask, bias, dt):
     seed = n + k + (0 if dt == "i32" else len(dt))
     cst, kw, kt = answer_inputs(n, k, dt, hist, mask, bias, seed=seed)

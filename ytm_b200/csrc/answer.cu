@@ -211,13 +211,13 @@ __global__ void __launch_bounds__(AN_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_an
 
 // -------------------------------------------------- rows of many classes
 
-// Classes whose counts a block holds.
-constexpr int AN_COUNTS = 8192;
+// Classes whose counts a block holds at most; a multiple of every tile.
+constexpr int AN_COUNTS = 16384;
 
 template <typename T, int THREADS, int E, bool HIST>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 4) k_answer_big(const ytm_answer_args a, int cluster, int part) {
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 4) k_answer_big(const ytm_answer_args a, int cluster, int part, int hold) {
     __shared__ Best warp_best[32], block_best;
-    extern __shared__ uint32_t counts[];  // [AN_COUNTS], with a history
+    extern __shared__ uint32_t counts[];  // [hold], with a history
     const int tid = threadIdx.x;
     const int64_t n = blockIdx.x / cluster;
     const int rank = (int)(blockIdx.x % cluster);
@@ -227,17 +227,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 4) k_answer_big
     const uint32_t *allowed = a.allowed ? a.allowed + n * a.allowed_stride : nullptr;
     const AnswerRow o = answer_row(a, n);
     Best best = {-INFINITY, INT_MAX, 0.f};
-    for (int c0 = from; c0 < to; c0 += AN_COUNTS) {
-        const int c1 = (int)min((int64_t)to, (int64_t)c0 + AN_COUNTS);
-        if (HIST) {
-            __syncthreads();
-            for (int i = tid; i < c1 - c0; i += THREADS) counts[i] = 0;
-            __syncthreads();
-            for (int64_t i = tid; i < o.len; i += THREADS) {
-                const int64_t h = index_at(a.history, a.history_64, n * a.history_stride + i) - c0;
-                if (h >= 0 && h < c1 - c0) atomicAdd(&counts[h], 1u);
-            }
-        }
+    for (int64_t c = from; c < to; c += hold) {
+        const int c0 = (int)c, c1 = (int)min((int64_t)to, c + hold);
         for (int k0 = c0 + tid; k0 - tid < c1; k0 += THREADS * E) {
             float z[E], b[E];
             uint32_t open = 0;
@@ -256,7 +247,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 4) k_answer_big
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) open |= (word[e] >> (k0 & 31) & 1u) << e;
-            if (HIST && k0 == c0 + tid) __syncthreads();  // the counts are there
+            if (HIST && k0 == c0 + tid) {  // count, while the first tile is on its way
+                __syncthreads();
+                for (int i = tid; i < c1 - c0; i += THREADS) counts[i] = 0;
+                __syncthreads();
+                for (int64_t i = tid; i < o.len; i += THREADS) {
+                    const int64_t h = index_at(a.history, a.history_64, n * a.history_stride + i) - c0;
+                    if (h >= 0 && h < c1 - c0) atomicAdd(&counts[h], 1u);
+                }
+                __syncthreads();
+            }
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 double x = to_f64(v[e]);
@@ -308,10 +308,14 @@ template <typename T, int THREADS, int E>
 static ytm_status launch_big(const ytm_answer_args &a, int cluster, cudaStream_t st) {
     if (a.n * cluster > INT_MAX) return fail(YTM_ERR_UNSUPPORTED, "answer: too many rows for one call");
     const int part = (int)(cdiv(cdiv(a.k, cluster), 32) * 32);
+    // counts of whole tiles; narrow blocks hold fewer, so that four fit an SM
+    const int tile = THREADS * E, most = THREADS == 1024 ? AN_COUNTS : AN_COUNTS / 2;
+    const int64_t tiles = (int64_t)cdiv(part, tile) * tile;
+    const int hold = (int)std::min<int64_t>(a.history ? most : tiles, tiles);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.n * cluster));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = a.history ? AN_COUNTS * 4 : 0;
+    cfg.dynamicSmemBytes = a.history ? hold * 4 : 0;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -323,7 +327,10 @@ static ytm_status launch_big(const ytm_answer_args &a, int cluster, cudaStream_t
     ytm_status rc;
     if (cluster > 8 && (rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "answer cluster")))
         return rc;
-    return cuda_check(cudaLaunchKernelEx(&cfg, f, a, cluster, part), "answer");
+    if (cfg.dynamicSmemBytes > 48 * 1024 &&
+        (rc = cuda_check(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, AN_COUNTS * 4), "answer smem")))
+        return rc;
+    return cuda_check(cudaLaunchKernelEx(&cfg, f, a, cluster, part, hold), "answer");
 }
 
 template <typename T>
