@@ -63,106 +63,93 @@ struct LossPart {
     double *dt;
 };
 
+// Two fp32 operations in one instruction, on register pairs.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair(float x, float y) {
+    F2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ void split(F2 a, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
 // -------------------------------------------------- rows of few classes
-// TPR threads hold a row, 4 * NV classes each: vectors of four where the rows
-// are 16-byte (8-byte for 16-bit types) aligned, else neighbouring lanes take
-// neighbouring classes.
+// TPR threads hold a row, E classes each (e TPR + lane), in pairs for the paired
+// arithmetic.  The label's class is not looked for among them: the lane that
+// holds it adds the row's weight to its own sum in shared memory and stores the
+// class's gradient once more.
 
 constexpr int LS_THREADS = 256;
 
-template <int TPR, int NV, bool VEC>
-__device__ __forceinline__ int small_class(int lane, int j, int i) {
-    return VEC ? (j * TPR + lane) * 4 + i : (j * 4 + i) * TPR + lane;
-}
-
-// Bits i = 0..3: class (j, i) is there and allowed.
-template <int TPR, int NV, bool VEC>
-__device__ __forceinline__ uint32_t small_open(const uint32_t *row, int lane, int j, int K) {
-    uint32_t o = 0;
-    if constexpr (VEC) {  // four neighbours: bits of one word
-        const int k = small_class<TPR, NV, VEC>(lane, j, 0);
-        if (k < K) o = (row ? row[k >> 5] >> (k & 31) : ~0u) & (k + 4 <= K ? 15u : (1u << (K - k)) - 1u);
-    } else if constexpr (TPR <= 8) {  // the team's 4 * TPR classes: bits of one word
-        const int k = small_class<TPR, NV, VEC>(0, j, 0);
-        const uint32_t w = k < K ? (row ? row[k >> 5] >> (k & 31) : ~0u) : 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (small_class<TPR, NV, VEC>(lane, j, i) < K) o |= ((w >> (i * TPR + lane)) & 1u) << i;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = small_class<TPR, NV, VEC>(lane, j, i);
-            if (k < K && is_allowed(row, k)) o |= 1u << i;
-        }
-    }
-    return o;
-}
-
-template <typename T>
-struct alignas(4 * sizeof(T)) Vec4 {
-    T v[4];
-};
-
-template <typename T, int TPR, int NV, bool VEC>
-__global__ void __launch_bounds__(LS_THREADS, NV >= 4 ? 2 : NV == 2 ? 3 : 4) k_loss_small(const ytm_loss_args a, const LossPart part) {
-    constexpr int ROWS = LS_THREADS / TPR;
-    extern __shared__ float red[];  // [ROWS][4 * NV * TPR]
+template <typename T, int TPR, int E>
+__global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_loss_small(const ytm_loss_args a, const LossPart part) {
+    constexpr int ROWS = LS_THREADS / TPR, SLOTS = TPR * E;
+    extern __shared__ float red[];  // [ROWS][SLOTS]: the labels' weights, at the end dbias of the teams
     __shared__ double red_dt[LS_THREADS / 32];
     const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR, K = a.k;
+    float *const mine = red + team * SLOTS + lane;
     const float rt = loss_rt(a), c = rt * LOG2E;
-    float b[NV][4], acc[NV][4];
-    uint32_t shared_open = 0;  // bit 4 j + i
+    const F2 c2 = pair(c, c);
+    F2 bc[E / 2], acc[E / 2];
+    uint32_t shared_open = 0;
+    const uint32_t *const shared_mask = a.allowed_stride ? nullptr : a.allowed;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        shared_open |= small_open<TPR, NV, VEC>(a.allowed_stride ? nullptr : a.allowed, lane, j, K) << (4 * j);
+    for (int e = 0; e < E; ++e) {
+        const int k = e * TPR + lane;
+        if (k < K && is_allowed(shared_mask, k)) shared_open |= 1u << e;
+        mine[e * TPR] = 0.f;
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = small_class<TPR, NV, VEC>(lane, j, i);
-            b[j][i] = a.bias && k < K ? __fmul_rn(a.bias[k], c) : 0.f;
-            acc[j][i] = 0.f;
-        }
+    for (int q = 0; q < E / 2; ++q) {
+        const int k = 2 * q * TPR + lane;
+        bc[q] = pair(a.bias && k < K ? __fmul_rn(a.bias[k], c) : 0.f, a.bias && k + TPR < K ? __fmul_rn(a.bias[k + TPR], c) : 0.f);
+        acc[q] = pair(0.f, 0.f);
     }
     // A row's loads are issued a round ahead, and its label's two rounds ahead,
     // so that the label's class sum, which waits for the label, comes in time.
-    const auto clamped = [&](int64_t n) { return n < a.n ? n : a.n - 1; };
     struct Row {
-        Vec4<T> v[NV];
+        T v[E];
         uint32_t open;
         T vy;
         float by;
         LossLabel label;
     };
-    const auto fetch = [&](int64_t n0, const LossLabel &label) {
+    const auto clamped = [&](int64_t n) { return n < a.n ? n : a.n - 1; };
+    const auto fetch = [&](int64_t n, const LossLabel &label) {
         Row r;
-        const int64_t n = clamped(n0 + team);
-        const T *cs = (const T *)a.cs + n * a.cs_stride;
+        const T *row = (const T *)a.cs + n * a.cs_stride, *cs = row + lane;
         r.open = shared_open;
         r.label = label;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            if (VEC) {
-                const int k = small_class<TPR, NV, VEC>(lane, j, 0);
-                if (k + 4 <= K) {
-                    if constexpr (sizeof(T) == 4) *(uint4 *)&r.v[j] = *(const uint4 *)(cs + k);
-                    else *(uint2 *)&r.v[j] = *(const uint2 *)(cs + k);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) r.v[j].v[i] = cs[min(k + i, K - 1)];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) r.v[j].v[i] = cs[min(small_class<TPR, NV, VEC>(lane, j, i), K - 1)];
-            }
-        }
+        for (int e = 0; e < E; ++e) r.v[e] = e * TPR + lane < K ? cs[e * TPR] : T(0.f);
         if (a.allowed_stride) {
+            const uint32_t *w = a.allowed + n * a.allowed_stride;
             uint32_t bits = 0;
+            constexpr int STEP = TPR < 32 ? 32 / TPR : 1;  // classes of a thread in a word
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
-                bits |= small_open<TPR, NV, VEC>(a.allowed + n * a.allowed_stride, lane, j, K) << (4 * j);
+            for (int e0 = 0; e0 < E; e0 += STEP) {
+                const uint32_t word = e0 * TPR < K ? w[e0 * TPR / 32] >> lane : 0u;
+#pragma unroll
+                for (int e = e0; e < E && e < e0 + STEP; ++e) bits |= (word >> ((e - e0) * TPR) & 1u) << e;
+            }
             r.open &= bits;
         }
         const int y = max(label.y, 0);
-        r.vy = cs[y];
+        r.vy = row[y];
         r.by = a.bias ? __fmul_rn(a.bias[y], c) : 0.f;
         return r;
     };
@@ -170,86 +157,89 @@ __global__ void __launch_bounds__(LS_THREADS, NV >= 4 ? 2 : NV == 2 ? 3 : 4) k_l
     const int64_t step = (int64_t)gridDim.x * ROWS;
     int64_t n0 = (int64_t)blockIdx.x * ROWS;
     LossLabel label1 = loss_label(a, clamped(n0 + step + team));
-    Row next = fetch(n0, loss_label(a, clamped(n0 + team)));
+    Row next = fetch(clamped(n0 + team), loss_label(a, clamped(n0 + team)));
     for (; n0 < a.n; n0 += step) {
         const Row row = next;
         if (n0 + step < a.n) {
-            next = fetch(n0 + step, label1);
+            next = fetch(clamped(n0 + step + team), label1);
             label1 = loss_label(a, clamped(n0 + 2 * step + team));
         }
         const bool live = n0 + team < a.n;
         const int64_t n = clamped(n0 + team);
-        float z[NV][4], m = -INFINITY;
+        float z[E], m = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                z[j][i] = (row.open >> (4 * j + i)) & 1u
-                              ? loss_z(to_f32(row.v[j].v[i]), b[j][i], c)
-                              : -INFINITY;
-                m = fmaxf(m, z[j][i]);
-            }
+        for (int q = 0; q < E / 2; ++q) {
+            float x, y;
+            split(fma2(pair(to_f32(row.v[2 * q]), to_f32(row.v[2 * q + 1])), c2, bc[q]), x, y);
+            z[2 * q] = row.open & (1u << (2 * q)) ? x : -INFINITY;
+            z[2 * q + 1] = row.open & (2u << (2 * q)) ? y : -INFINITY;
+            m = fmaxf(m, fmaxf(z[2 * q], z[2 * q + 1]));
+        }
 #pragma unroll
         for (int d = TPR / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-        float s = 0.f, h = 0.f;
+        F2 s2 = pair(0.f, 0.f), h2 = s2;
+        const F2 m2 = pair(-m, -m);
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = z[j][i] - m;
-                z[j][i] = ex2(x);
-                s += z[j][i];
-                h = fmaf(z[j][i], fmaxf(x, -1024.f), h);  // 0 * -inf counts for nothing
-            }
+        for (int q = 0; q < E / 2; ++q) {
+            float x, y;
+            split(add2(pair(z[2 * q], z[2 * q + 1]), m2), x, y);
+            z[2 * q] = ex2(x);
+            z[2 * q + 1] = ex2(y);
+            const F2 e2 = pair(z[2 * q], z[2 * q + 1]);
+            s2 = add2(s2, e2);
+            h2 = fma2(e2, pair(fmaxf(x, -1024.f), fmaxf(y, -1024.f)), h2);  // 0 * -inf counts for nothing
+        }
+        float s, h, t;
+        split(s2, s, t);
+        s += t;
+        split(h2, h, t);
+        h += t;
 #pragma unroll
         for (int d = TPR / 2; d; d >>= 1) {
             s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
             h += __shfl_xor_sync(0xFFFFFFFFu, h, d);
         }
         const bool use = live && row.label.open;
-        const float wt = row.label.w * rt, f = wt / s;
-        T *dcs = (T *)a.dcs + n * (int64_t)K;
+        const float wt = row.label.w * rt, f = wt / s, zy = loss_z(to_f32(row.vy), row.by, c);
+        if (use) {
+            const F2 f2 = pair(f, f);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float d = z[j][i] * f;
-                if (small_class<TPR, NV, VEC>(lane, j, i) == row.label.y) d -= wt;
-                z[j][i] = use ? d : 0.f;
-                acc[j][i] += z[j][i];
+            for (int q = 0; q < E / 2; ++q) {
+                const F2 d2 = mul2(pair(z[2 * q], z[2 * q + 1]), f2);
+                acc[q] = add2(acc[q], d2);
+                split(d2, z[2 * q], z[2 * q + 1]);
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) z[e] = 0.f;
+        }
+        if constexpr (!std::is_integral<T>::value) {
+            if (a.dcs && live) {
+                T *const out = (T *)a.dcs + n * (int64_t)K + lane;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e * TPR + lane < K) out[e * TPR] = from_f32<T>(z[e]);
+            }
+        }
+        if (use && row.label.y % TPR == lane) {
+            mine[row.label.y - lane] += wt;
             if constexpr (!std::is_integral<T>::value) {
-                if (a.dcs && live) {
-                    const int k = small_class<TPR, NV, VEC>(lane, j, 0);
-                    Vec4<T> out;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) out.v[i] = from_f32<T>(z[j][i]);
-                    if (VEC && k + 4 <= K) {
-                        if constexpr (sizeof(T) == 4) *(uint4 *)(dcs + k) = *(uint4 *)&out;
-                        else *(uint2 *)(dcs + k) = *(uint2 *)&out;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int ki = small_class<TPR, NV, VEC>(lane, j, i);
-                            if (ki < K) dcs[ki] = out.v[i];
-                        }
-                    }
-                }
+                if (a.dcs) ((T *)a.dcs)[n * (int64_t)K + row.label.y] = from_f32<T>(ex2(zy - m) * f - wt);
             }
         }
         if (lane == 0 && live) {
-            const float w = row.label.w, gap = loss_z(to_f32(row.vy), row.by, c) - m;
+            const float w = row.label.w, gap = zy - m;
             a.loss[n] = use ? w * (logf(s) - gap * LN2) : row.label.y >= 0 ? w * INFINITY : 0.f;
             if (use) dt += (double)w * (double)(h / s - gap);
         }
     }
     // the block's sums, teams in order
-    constexpr int SLOTS = 4 * NV * TPR;
-    if (a.dbias) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) red[team * SLOTS + small_class<TPR, NV, VEC>(lane, j, i)] = acc[j][i];
+    for (int q = 0; q < E / 2; ++q) {
+        float x, y;
+        split(acc[q], x, y);
+        mine[2 * q * TPR] = x - mine[2 * q * TPR];
+        mine[(2 * q + 1) * TPR] = y - mine[(2 * q + 1) * TPR];
     }
     for (int d = 16; d; d >>= 1) dt += __shfl_xor_sync(0xFFFFFFFFu, dt, d);
     if ((threadIdx.x & 31) == 0) red_dt[threadIdx.x >> 5] = dt;
@@ -305,30 +295,6 @@ struct RowVecs {
     __device__ __forceinline__ int end(int K, int slack = 0) const { return max(first(), (int)(((int64_t)off + K - slack) / V)); }
     __device__ __forceinline__ const uint4 *at(int i) const { return (const uint4 *)(row - off + (int64_t)i * V); }
 };
-
-// Two fp32 operations in one instruction, on register pairs.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 pair(float x, float y) {
-    F2 d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-    return d;
-}
-__device__ __forceinline__ void split(F2 a, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a)); }
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-    F2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-    F2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
 
 // Classes 2 q and 2 q + 1 of a vector.
 template <typename T>
@@ -677,7 +643,8 @@ __global__ void __launch_bounds__(1024) k_loss_join(const ytm_loss_args a, const
 // How a call is cut: which kernels, and how many teams' parts there are to join.
 struct LossPlan {
     bool big;
-    int tpr, nv;  // threads of a row (small), vectors of a thread (small: of four classes; big: in a round)
+    int tpr, e;   // small: threads of a row, classes of a thread
+    int nv;       // big: vectors of a thread in a round
     int parts, rounds, chunk, period;  // big: parts of a row, rounds of a part, rows of a chunk and their distance
     int64_t teams;             // blocks (small) or chunks (big)
 };
@@ -689,10 +656,10 @@ static LossPlan loss_plan(int64_t n, int64_t k, int64_t elem, int64_t cs_stride)
     const int64_t sms = sm_count();
     if (k <= 512) {
         p.tpr = k <= 16 ? 4 : k <= 128 ? 8 : k <= 256 ? 16 : 32;
-        p.nv = k <= 32 ? 1 : k <= 64 ? 2 : 4;
+        p.e = k <= 32 ? 4 : k <= 64 ? 8 : 16;
         const int64_t rows = LS_THREADS / p.tpr;
         // up to four rounds of one block cost less than joining blocks
-        p.teams = n <= 4 * rows ? 1 : std::min<int64_t>(cdiv(n, rows), sms * (p.nv >= 4 ? 2 : 4));
+        p.teams = n <= 4 * rows ? 1 : std::min<int64_t>(cdiv(n, rows), sms * (p.e == 16 ? 2 : p.e == 8 ? 3 : 4));
         p.teams = std::max<int64_t>(p.teams, cdiv(n, rows * LOSS_CHAIN));
         return p;
     }
@@ -757,27 +724,21 @@ static ytm_status launch_big(const ytm_loss_args &a, const LossPlan &p, const Lo
                         p.chunk, p.period, part);
 }
 
-template <typename T, int TPR, int NV>
-static ytm_status launch_small(const ytm_loss_args &a, const LossPlan &p, const LossPart &part, bool vec, cudaStream_t st) {
-    const size_t smem = (size_t)LS_THREADS * NV * 16;
-    if (vec) k_loss_small<T, TPR, NV, true><<<(unsigned)p.teams, LS_THREADS, smem, st>>>(a, part);
-    else k_loss_small<T, TPR, NV, false><<<(unsigned)p.teams, LS_THREADS, smem, st>>>(a, part);
+template <typename T, int TPR, int E>
+static ytm_status launch_small(const ytm_loss_args &a, const LossPlan &p, const LossPart &part, cudaStream_t st) {
+    k_loss_small<T, TPR, E><<<(unsigned)p.teams, LS_THREADS, LS_THREADS * E * 4, st>>>(a, part);
     return launch_check("class loss");
 }
 
 template <typename T>
 static ytm_status launch_loss(const ytm_loss_args &a, const LossPlan &p, const LossPart &part, LossStat *stats, cudaStream_t st) {
     if (p.big) return launch_big<T>(a, p, part, stats, st);
-    // vectors of four classes
-    const uint64_t step = 4 * sizeof(T);
-    const bool vec = (uintptr_t)a.cs % step == 0 && a.cs_stride * sizeof(T) % step == 0 &&
-                     (!a.dcs || ((uintptr_t)a.dcs % step == 0 && (uint64_t)a.k * sizeof(T) % step == 0));
-    if (p.tpr == 4) return launch_small<T, 4, 1>(a, p, part, vec, st);
-    if (p.tpr == 8 && p.nv == 1) return launch_small<T, 8, 1>(a, p, part, vec, st);
-    if (p.tpr == 8 && p.nv == 2) return launch_small<T, 8, 2>(a, p, part, vec, st);
-    if (p.tpr == 8) return launch_small<T, 8, 4>(a, p, part, vec, st);
-    if (p.tpr == 16) return launch_small<T, 16, 4>(a, p, part, vec, st);
-    return launch_small<T, 32, 4>(a, p, part, vec, st);
+    if (p.tpr == 4) return launch_small<T, 4, 4>(a, p, part, st);
+    if (p.tpr == 8 && p.e == 4) return launch_small<T, 8, 4>(a, p, part, st);
+    if (p.tpr == 8 && p.e == 8) return launch_small<T, 8, 8>(a, p, part, st);
+    if (p.tpr == 8) return launch_small<T, 8, 16>(a, p, part, st);
+    if (p.tpr == 16) return launch_small<T, 16, 16>(a, p, part, st);
+    return launch_small<T, 32, 16>(a, p, part, st);
 }
 
 }  // namespace ytm
