@@ -322,7 +322,7 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 
 // COLS: the columns of a block, padded to a multiple of 8.
 template <Q4Mode MODE, int COLS, int GROUP>
-__global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS == 16 ? 2 : 1) k_q4_votes(const Q4Args a, const __grid_constant__ CUtensorMap weights) {
+__global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS <= 32 ? 2 : 1) k_q4_votes(const Q4Args a, const __grid_constant__ CUtensorMap weights) {
     constexpr int NT = COLS / 8, SEG_BYTES = q4_seg_bytes(MODE, COLS, GROUP);
     extern __shared__ __align__(1024) char smem[];  // weights, activations; barriers at the end
     uint64_t *const bars = (uint64_t *)(smem + a.bars_at);
@@ -599,7 +599,7 @@ static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group)
     p.samples = (int)std::min(N, most);
     p.z = std::min<int64_t>(cdiv(N, most), 65535);
     const int used = p.samples * p.parts;
-    p.cols = used <= 8 ? 8 : used <= 16 ? 16 : used <= 32 ? 32 : used <= 48 ? 48 : 64;
+    p.cols = used <= 32 ? (used + 7) / 8 * 8 : used <= 48 ? 48 : 64;
     const int seg_bytes = q4_seg_bytes(p.mode, p.cols, group);
     const int64_t sms = sm_count();
     const int nt = p.cols / 8;
@@ -610,7 +610,7 @@ static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group)
         const size_t smem = std::max<size_t>(Q4_STAGES * (Q4_STAGE_BYTES + (size_t)seg_bytes * wk), red) + Q4_BARS;
         if (smem > 227 * 1024) continue;
         const int64_t tiles = cdiv(K, 16 * wm) * p.z, stages = cdiv(C, Q4_SEG * wk);
-        const int64_t held = std::min<int64_t>(nt == 1 ? 3 : nt == 2 ? 2 : 1, 227 * 1024 / (smem + 1024));  // blocks of an SM
+        const int64_t held = std::min<int64_t>(nt == 1 ? 3 : nt <= 4 ? 2 : 1, 227 * 1024 / (smem + 1024));  // blocks of an SM
         for (int cl = 1; cl <= 16 && (cl == 1 || cl <= stages); cl *= 2) {
             const int64_t place = cl == 16 ? sms * 3 / 4 : cl == 8 ? sms * 6 / 7 : sms;  // SMs that such clusters reach
             const int64_t rounds = tiles * cl / (place * held), rest = tiles * cl % (place * held);
@@ -711,6 +711,7 @@ static ytm_status launch_q4(const Q4XArgs &xa, unsigned x_blocks, const Q4Args &
     switch (p.cols) {
         case 8: return launch_q4<MODE, 8>(a, p, map, group, grid, st);
         case 16: return launch_q4<MODE, 16>(a, p, map, group, grid, st);
+        case 24: return launch_q4<MODE, 24>(a, p, map, group, grid, st);
         case 32: return launch_q4<MODE, 32>(a, p, map, group, grid, st);
         case 48: return launch_q4<MODE, 48>(a, p, map, group, grid, st);
         default: return launch_q4<MODE, 64>(a, p, map, group, grid, st);
