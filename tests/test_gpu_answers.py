@@ -136,6 +136,36 @@ def test_votes_of_no_samples_and_infinite_activations():
     assert (np.abs(y / (0.5 * f64(big)[0, 0]) - 1) <= 4 * U).all()
 
 
+@pytest.mark.parametrize("n,c,k,x,group,scale", [(1, 16384, 32768, "bf16", 32, "f32"), (1, 16384, 20011, "f32", 128, "f16"),
+                                                 (2, 8192, 30000, "f16", 64, "bf16"), (7, 8192, 20000, "bf16", 32, "f32"),
+                                                 (1, 16384, 30000, "bits", 64, "f32")])
+def test_votes_again_and_again(n, c, k, x, group, scale):
+    """Streams of many stages over all SMs, call after call on two inputs: a
+    stage that is copied over before it is read shows as another result, once
+    in some hundred calls."""
+    sets = []
+    for seed in (1, 2):
+        torch.manual_seed(seed)
+        words = -(-c // 32)
+        packed = torch.randint(0, 256, (k, words * 16), dtype=torch.uint8, device="cuda")
+        scales = (torch.rand(k, -(-c // group), device="cuda") + 0.1).to(DT[scale])
+        xt = torch.randint(-2 ** 31, 2 ** 31 - 1, (n, words), device="cuda").to(torch.int32) if x == "bits" \
+            else torch.randn(n, c, device="cuda").to(DT[x])
+        sets.append((xt, packed, scales))
+    want = [answers.q4_votes(*s, group, clauses=c) for s in sets]
+    other = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(400):
+        for s, w in zip(sets, want):
+            other += (answers.q4_votes(*s, group, clauses=c) != w).sum()
+    assert other.item() == 0
+    for (xt, packed, scales), w in zip(sets, want):
+        rows = torch.randint(0, k, (64,), device="cuda")
+        q = nibbles(packed[rows].cpu().numpy(), c).astype(np.int64) - 8
+        xw = xt.cpu().numpy()
+        xv = f64(xt) if x != "bits" else ((xw.view(np.uint32)[:, np.arange(c) // 32] >> (np.arange(c) % 32)) & 1).astype(np.float64)
+        check_votes(w[:, rows], xv, q, scales[rows], group, np.zeros(64), "f32", c)
+
+
 # ------------------------------------------------------------------- answer
 
 def answer_inputs(n, k, dt, hist, mask, bias, seed=0, knobs=True):
