@@ -122,6 +122,12 @@ def test_votes_strides_and_alignment(x):
     check_votes(y, xv, q[5:20], scales[5:20], group, bias[5:20], "f32", c)
 
 
+def test_votes_of_more_samples_than_one_launch_takes():
+    n, c, k = 530001, 33, 2  # blocks of eight fp32 samples, 65,535 of them a launch
+    xt, xv, packed, q, scales, bias = votes_inputs(n, c, k, "f32", 32, "f32")
+    check_votes(answers.q4_votes(xt, packed, scales, 32, bias=dev(bias)), xv, q, scales, 32, bias, "f32", c)
+
+
 def test_votes_of_no_samples_and_infinite_activations():
     xt, xv, packed, q, scales, bias = votes_inputs(4, 100, 20, "f32", 64, "f32")
     assert answers.q4_votes(xt[:0], packed, scales, 64).shape == (0, 20)
@@ -161,8 +167,10 @@ def test_votes_again_and_again(n, c, k, x, group, scale):
     for (xt, packed, scales), w in zip(sets, want):
         rows = torch.randint(0, k, (64,), device="cuda")
         q = nibbles(packed[rows].cpu().numpy(), c).astype(np.int64) - 8
-        xw = xt.cpu().numpy()
-        xv = f64(xt) if x != "bits" else ((xw.view(np.uint32)[:, np.arange(c) // 32] >> (np.arange(c) % 32)) & 1).astype(np.float64)
+        if x == "bits":
+            xv = ((xt.cpu().numpy().view(np.uint32)[:, np.arange(c) // 32] >> (np.arange(c) % 32)) & 1).astype(np.float64)
+        else:
+            xv = f64(xt)
         check_votes(w[:, rows], xv, q, scales[rows], group, np.zeros(64), "f32", c)
 
 
