@@ -50,6 +50,7 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
                dict(g=16), dict(K=0), dict(y=None), dict(yt=0), dict(x=None), dict(s=None), dict(ws=None), dict(ws=ct.c_void_p(8))):
         assert votes(**kw) == 1, kw
     assert votes(N=0) == 0
+    assert votes(K=(1 << 30) + 1) == 3 and votes(C=(1 << 30) + 1) == 3
     good = dict(cs=16, cs_stride=4, n=1, k=4, cs_type=0)
     for kw in (dict(k=0), dict(n=-1), dict(cs_type=4), dict(cs=None), dict(cs_stride=-1), dict(bias_stride=-1),
                dict(allowed_stride=-1), dict(history_len=-1), dict(lengths=16)):
@@ -62,7 +63,8 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
         assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, **kw})), one, None) == 1, kw
     assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "n": 100000})), None, None) == 1
     assert lib.ytm_class_loss_workspace_bytes(100000, 4, 1, 4) > 0
-    assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "k": 5000, "n": 1 << 27})), one, None) == 3
+    assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "n": 1 << 31})), one, None) == 3
+    assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "k": (1 << 30) + 1})), one, None) == 3
     assert lib.ytm_class_loss(None, one, None) == 1
     assert lib.ytm_class_loss(ct.byref(_lib.LossArgs(**{**good, "n": 0})), None, None) == 0
     assert lib.ytm_class_loss_workspace_bytes(-1, 4, 1, 4) == 0

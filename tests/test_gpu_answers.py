@@ -10,7 +10,7 @@ import torch
 from oracle import oracle as O
 from tests.answers_ref import nibbles, ref_answer, ref_loss, ref_pack, ref_votes
 from ytm_b200 import _lib, answers
-from ytm_b200.cutm import MultiClassTM
+from ytm_b200.cutm import MultiClassTM, MultiOutputTM
 from ytm_b200.engine import CudaEngine
 
 pytestmark = pytest.mark.gpu
@@ -448,6 +448,56 @@ def test_class_loss_values_under_the_mask_and_unusual_rows():
     assert abs(loss.item() - want[0][0]) <= 8 * U * 4 and (dcs[0, 3:] == 0).all() and np.isfinite(dt.item())
 
 
+@pytest.mark.parametrize("k", [12, 300, 1000, 5003])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_class_loss_of_the_types_lowest_values(k, dt):
+    """A row of nothing but the lowest value is uniform; a label there has a
+    finite loss while others are ordinary; the largest value does no harm."""
+    tt = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dt]
+    low, high = torch.finfo(tt).min, torch.finfo(tt).max
+    cs = torch.zeros(5, k, dtype=tt, device="cuda")
+    cs[0] = low
+    cs[1, 3:] = low
+    cs[2, 5] = low
+    cs[3, 7] = high
+    cs[4] = high
+    y = np.array([1, 0, 5, 7, k - 1])
+    loss, dcs, _, _ = answers.class_loss(cs, dev(y))
+    # less the row's largest, which changes no loss: beside 3e38 even 64 bits lose log k
+    want = ref_loss(f64(cs) - f64(cs).max(1, keepdims=True), y, temperature=1.0)
+    # log k by the sum's chain, the lowest value by four roundings
+    tol = 16 * U * np.abs(want[0]) + (k / 32 + 64) * 4 * U
+    assert np.isfinite(f64(loss)).all() and (np.abs(f64(loss) - want[0]) <= tol).all()
+    # p by ex2 and the sum's chain, its rounding to the type
+    tol = (np.abs(want[1]) + 1 / k) * (k / 32 + 72) * 4 * U
+    assert (np.abs(f64(dcs) - want[1]) <= tol + half_step(tt, np.abs(want[1]) + tol)).all()
+
+
+@pytest.mark.parametrize("k", [40, 1030])
+def test_class_loss_of_an_infinite_temperature_is_uniform(k):
+    rng = np.random.default_rng(1)
+    a = rng.random((7, k)) < 0.5
+    a[:, 0] = True
+    cs = dev(rng.normal(size=(7, k)).astype(np.float32) * 1e4)
+    loss, dcs, _, dt = answers.class_loss(cs, dev(np.zeros(7, np.int64)), allowed=answers.pack_allowed(a).cuda(), temperature=float("inf"))
+    assert (np.abs(f64(loss) - np.log(a.sum(1))) <= 64 * U).all() and (dcs == 0).all() and dt.item() == 0
+
+
+def test_class_loss_of_more_chunks_than_one_grid_dimension():
+    """Nine million rows of one memory; every row's loss is its label's."""
+    n, k = 9_000_001, 513
+    cs = dev(np.arange(k, dtype=np.int32)[None] % 7).expand(n, k)
+    y = torch.arange(n, device="cuda") % k
+    loss, dcs, db, dt = answers.class_loss(cs, y, bias=torch.zeros(k, device="cuda"))
+    z = np.arange(k) % 7
+    lse = np.log(np.exp(z.astype(np.float64)).sum())
+    # ex2 and the sum's chain of 513 terms over 256 threads
+    assert (loss - dev((lse - z).astype(np.float32))[y]).abs().max().item() <= 64 * U
+    want = n * np.exp(z - lse) - np.bincount(np.arange(n) % k, minlength=k)
+    # chunks of 128 rows in fp32, joined in 64 bits: (128 + 64) roundings of the sums' parts
+    assert (np.abs(f64(db) - want) <= 192 * U * (n * np.exp(z - lse) + n / k + 1)).all()
+
+
 def test_class_loss_gradients_against_differences():
     """Central differences of the 64-bit loss (h = 1e-5: error about 1e-9), and
     the kernel's fp32 error as in check_loss, here below 1e-5 of the weights."""
@@ -485,7 +535,7 @@ def test_refusals():
         lambda: answers.answer(z, history=torch.zeros((2, 4), dtype=torch.int64, device="cuda")),
         lambda: answers.answer(z, history=torch.zeros((3, 4), device="cuda")),
         lambda: answers.answer(z, history=torch.zeros((3, 4), dtype=torch.int64, device="cuda"), lengths=i),
-        lambda: answers.answer(z, temperature=0.0),
+        lambda: answers.answer(z, temperature=0.0), lambda: answers.answer(z, temperature=1e-50),
         lambda: answers.answer(z, temperature=float("nan")),
         lambda: answers.answer(z, repetition=-1.0),
         lambda: answers.answer(z, presence=torch.zeros(2, device="cuda")),
@@ -652,3 +702,18 @@ def test_model_path_from_packed_votes_to_answers():
     tm.fit(X, y, batch_size=8)  # the packed copy stays as it was
     votes2 = tm.pack_votes(group=32)
     assert votes2.packed.data_ptr() != votes.packed.data_ptr()
+
+
+def test_multi_output_scores_from_packed_votes():
+    rng = np.random.default_rng(6)
+    X = (rng.random((40, 64)) < 0.4).astype(np.uint32)
+    Y = (rng.random((40, 3)) < 0.5).astype(np.uint32)
+    tm = MultiOutputTM(number_of_clauses_per_class=20, T=15, s=4.0, dim=(8, 8, 1), n_classes=3, seed=2)
+    tm.fit(X, Y)
+    votes = tm.pack_votes(group=64)
+    full, cs = tm.score(X, False), tm.score(X, False, votes=votes)
+    # rounding a weight moves it by at most half a scale
+    assert (np.abs(cs - full) <= 64 * f64(votes.scales).sum(1) / 2 + 1e-3).all()
+    preds, cs2 = tm.predict(X, votes=votes)
+    np.testing.assert_array_equal(cs2, cs)
+    np.testing.assert_array_equal(preds, (cs >= 0).astype(np.uint32))

@@ -1,12 +1,14 @@
 // class_loss.cu — cross entropy of biased, masked, tempered class sums with
 // its gradients.
 //
-// In units of log2 e: with c = log2(e) / t and z = (v + b) c (allowed classes),
-//   e_k = 2^(z_k - m), s = sum e, h = sum e (z - m)         (m = max z)
-//   loss = w (ln s - (z_y - m) ln 2)
+// With u = v + b (allowed classes), m = max u and c = log2(e) / t,
+//   x_k = (u_k - m) c, e_k = 2^x_k, s = sum e, h = sum e x
+//   loss = w (ln s - (u_y - m) / t)
 //   dcs_k = (w / t) (e_k / s - 1[k = y]),  dbias = sum_n dcs
-//   dt = -(ln 2 / t) sum_n w (h / s - (z_y - m))
-// so that h gives the temperature's gradient without another look at z.
+//   dt = -(ln 2 / t) sum_n w (h / s - x_y)
+// so that h gives the temperature's gradient without another look at u.  The
+// factor comes after the difference: a row of the type's lowest value, whose
+// product with c has left the type, keeps its u - m = 0.
 //
 // Rows of up to 512 classes stay in the registers of 4 to 32 threads between
 // the sum and the gradient (k_loss_small).  Longer rows take two streams over
@@ -14,6 +16,7 @@
 // k_loss_grad, whose threads keep their classes over a chunk of rows.  Both
 // kernels sum dbias in registers and leave one part per team or chunk, which
 // k_loss_join adds in a fixed order.
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
@@ -32,9 +35,10 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// z, with bc = b c; the same operations for every use of a class's z, so that
-// the largest class's exponent is 0 exactly.
-__device__ __forceinline__ float loss_z(float v, float bc, float c) { return __fmaf_rn(v, c, bc); }
+// u and x, the same operations for every use of a class's, so that the largest
+// class's x is 0 exactly.
+__device__ __forceinline__ float loss_u(float v, float b) { return __fadd_rn(v, b); }
+__device__ __forceinline__ float loss_x(float u, float m, float c) { return __fmul_rn(__fsub_rn(u, m), c); }
 
 // A row's label, weight and label's mask bit.  y < 0: the row counts for
 // nothing; open: it has a gradient.
@@ -56,6 +60,8 @@ __device__ __forceinline__ LossLabel loss_label(const ytm_loss_args &a, int64_t 
 __device__ __forceinline__ float loss_rt(const ytm_loss_args &a) {
     return 1.f / (a.temperature ? *a.temperature : a.temperature_all);
 }
+// Not 0, so that a masked class's -inf stays one under an infinite temperature.
+__device__ __forceinline__ float loss_c(float rt) { return fmaxf(rt * LOG2E, FLT_MIN); }
 
 // Partial sums of the teams or chunks: dbias [G][k], dt / (-ln 2 / t) [G].
 struct LossPart {
@@ -102,9 +108,9 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
     __shared__ double red_dt[LS_THREADS / 32];
     const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR, K = a.k;
     float *const mine = red + team * SLOTS + lane;
-    const float rt = loss_rt(a), c = rt * LOG2E;
+    const float rt = loss_rt(a), c = loss_c(rt);
     const F2 c2 = pair(c, c);
-    F2 bc[E / 2], acc[E / 2];
+    F2 b[E / 2], acc[E / 2];
     uint32_t shared_open = 0;
     const uint32_t *const shared_mask = a.allowed_stride ? nullptr : a.allowed;
 #pragma unroll
@@ -116,7 +122,7 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
 #pragma unroll
     for (int q = 0; q < E / 2; ++q) {
         const int k = 2 * q * TPR + lane;
-        bc[q] = pair(a.bias && k < K ? __fmul_rn(a.bias[k], c) : 0.f, a.bias && k + TPR < K ? __fmul_rn(a.bias[k + TPR], c) : 0.f);
+        b[q] = pair(a.bias && k < K ? a.bias[k] : 0.f, a.bias && k + TPR < K ? a.bias[k + TPR] : 0.f);
         acc[q] = pair(0.f, 0.f);
     }
     // A row's loads are issued a round ahead, and its label's two rounds ahead,
@@ -150,7 +156,7 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
         }
         const int y = max(label.y, 0);
         r.vy = row[y];
-        r.by = a.bias ? __fmul_rn(a.bias[y], c) : 0.f;
+        r.by = a.bias ? a.bias[y] : 0.f;
         return r;
     };
     double dt = 0.0;
@@ -170,7 +176,7 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
 #pragma unroll
         for (int q = 0; q < E / 2; ++q) {
             float x, y;
-            split(fma2(pair(to_f32(row.v[2 * q]), to_f32(row.v[2 * q + 1])), c2, bc[q]), x, y);
+            split(add2(pair(to_f32(row.v[2 * q]), to_f32(row.v[2 * q + 1])), b[q]), x, y);
             z[2 * q] = row.open & (1u << (2 * q)) ? x : -INFINITY;
             z[2 * q + 1] = row.open & (2u << (2 * q)) ? y : -INFINITY;
             m = fmaxf(m, fmaxf(z[2 * q], z[2 * q + 1]));
@@ -182,7 +188,7 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
 #pragma unroll
         for (int q = 0; q < E / 2; ++q) {
             float x, y;
-            split(add2(pair(z[2 * q], z[2 * q + 1]), m2), x, y);
+            split(mul2(add2(pair(z[2 * q], z[2 * q + 1]), m2), c2), x, y);
             z[2 * q] = ex2(x);
             z[2 * q + 1] = ex2(y);
             const F2 e2 = pair(z[2 * q], z[2 * q + 1]);
@@ -200,7 +206,7 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
             h += __shfl_xor_sync(0xFFFFFFFFu, h, d);
         }
         const bool use = live && row.label.open;
-        const float wt = row.label.w * rt, f = wt / s, zy = loss_z(to_f32(row.vy), row.by, c);
+        const float wt = row.label.w * rt, f = wt / s, uy = loss_u(to_f32(row.vy), row.by);
         if (use) {
             const F2 f2 = pair(f, f);
 #pragma unroll
@@ -224,13 +230,13 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
         if (use && row.label.y % TPR == lane) {
             mine[row.label.y - lane] += wt;
             if constexpr (!std::is_integral<T>::value) {
-                if (a.dcs) ((T *)a.dcs)[n * (int64_t)K + row.label.y] = from_f32<T>(ex2(zy - m) * f - wt);
+                if (a.dcs) ((T *)a.dcs)[n * (int64_t)K + row.label.y] = from_f32<T>(ex2(loss_x(uy, m, c)) * f - wt);
             }
         }
         if (lane == 0 && live) {
-            const float w = row.label.w, gap = zy - m;
-            a.loss[n] = use ? w * (logf(s) - gap * LN2) : row.label.y >= 0 ? w * INFINITY : 0.f;
-            if (use) dt += (double)w * (double)(h / s - gap);
+            const float w = row.label.w, gap = uy - m;
+            a.loss[n] = use ? w * (logf(s) - gap * rt) : row.label.y >= 0 ? w * INFINITY : 0.f;
+            if (use) dt += (double)w * ((double)(h / s) - (double)gap * (double)c);
         }
     }
     // the block's sums, teams in order
@@ -264,10 +270,10 @@ struct LossStat {
     float m, s, h;
 };
 
-__device__ __forceinline__ LossStat merge(const LossStat &a, const LossStat &b) {
+__device__ __forceinline__ LossStat merge(const LossStat &a, const LossStat &b, float c) {
     const float m = fmaxf(a.m, b.m);
     // a.m == m: the factor is 1 also where both are infinite
-    const float da = a.m == m ? 0.f : a.m - m, db = b.m == m ? 0.f : b.m - m;
+    const float da = a.m == m ? 0.f : loss_x(a.m, m, c), db = b.m == m ? 0.f : loss_x(b.m, m, c);
     const float fa = ex2(da), fb = ex2(db);
     // separate roundings: merge(a, b) == merge(b, a), so all lanes of an
     // exchange end with the same bits
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
     const int K = a.k;
     const int64_t n = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
     if (n >= a.n) return;
-    const float c = loss_rt(a) * LOG2E;
+    const float c = loss_c(loss_rt(a));
     const F2 c2 = pair(c, c);
     const RowVecs<T> row(a.cs, n, a.cs_stride);
     const uint32_t *allowed = a.allowed ? a.allowed + n * a.allowed_stride : nullptr;
@@ -367,13 +373,13 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
 #pragma unroll
                 for (int q = 0; q < V / 2; ++q) {
                     float x, y;
-                    split(fma2(class_pair<T>(raw[j], q), c2, mul2(b[j][q], c2)), x, y);
+                    split(add2(class_pair<T>(raw[j], q), b[j][q]), x, y);
                     z[j][2 * q] = open[j] & (1u << (2 * q)) ? x : -INFINITY;
                     z[j][2 * q + 1] = open[j] & (2u << (2 * q)) ? y : -INFINITY;
                     m = fmaxf(m, fmaxf(z[j][2 * q], z[j][2 * q + 1]));
                 }
             const float base = m == -INFINITY ? 0.f : -m;  // nothing yet: every e is 0
-            const float d = st.m == m ? 0.f : st.m - m, f = ex2(d);
+            const float d = st.m == m ? 0.f : loss_x(st.m, m, c), f = ex2(d);
             F2 s = pair(f * st.s, 0.f), h = pair(f * fmaf(st.s, fmaxf(d, -1024.f), st.h), 0.f);
             const F2 base2 = pair(base, base);
             st.m = m;
@@ -382,7 +388,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
 #pragma unroll
                 for (int q = 0; q < V / 2; ++q) {
                     float x, y;
-                    split(add2(pair(z[j][2 * q], z[j][2 * q + 1]), base2), x, y);
+                    split(mul2(add2(pair(z[j][2 * q], z[j][2 * q + 1]), base2), c2), x, y);
                     const F2 e = pair(ex2(x), ex2(y));
                     s = add2(s, e);
                     h = fma2(e, pair(fmaxf(x, -1024.f), fmaxf(y, -1024.f)), h);  // 0 * -inf counts for nothing
@@ -404,15 +410,15 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
         const int head = first * V - (first ? row.off : 0), tail = end * V - row.off;
         const int k = (int)threadIdx.x < head ? (int)threadIdx.x : tail + ((int)threadIdx.x - head);
         if (k < K && is_allowed(allowed, k)) {
-            const float z = loss_z(to_f32(row.row[k]), a.bias ? __fmul_rn(a.bias[k], c) : 0.f, c);
-            // z itself if it is no number, so that it reaches the sum
-            st = merge(st, {z, z == z ? (z == -INFINITY ? 0.f : 1.f) : z, 0.f});
+            const float u = loss_u(to_f32(row.row[k]), a.bias ? a.bias[k] : 0.f);
+            // u itself if it is no number, so that it reaches the sum
+            st = merge(st, {u, u == u ? (u == -INFINITY ? 0.f : 1.f) : u, 0.f}, c);
         }
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1)
         st = merge(st, {__shfl_xor_sync(0xFFFFFFFFu, st.m, d), __shfl_xor_sync(0xFFFFFFFFu, st.s, d),
-                        __shfl_xor_sync(0xFFFFFFFFu, st.h, d)});
+                        __shfl_xor_sync(0xFFFFFFFFu, st.h, d)}, c);
     if ((threadIdx.x & 31) == 0) warp_stat[threadIdx.x >> 5] = st;
     __syncthreads();
     if (threadIdx.x >= 32) return;
@@ -420,7 +426,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
 #pragma unroll
     for (int d = LB_THREADS / 64; d; d >>= 1)
         st = merge(st, {__shfl_xor_sync(0xFFFFFFFFu, st.m, d), __shfl_xor_sync(0xFFFFFFFFu, st.s, d),
-                        __shfl_xor_sync(0xFFFFFFFFu, st.h, d)});
+                        __shfl_xor_sync(0xFFFFFFFFu, st.h, d)}, c);
     if (threadIdx.x == 0) stats[n * gridDim.x + blockIdx.x] = st;
 }
 
@@ -435,21 +441,23 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
 constexpr int LB_ROWS = 128;  // rows of a chunk at most
 
 struct GradRow {
-    float m, f, wt;  // z of the largest class, w / (t s), w / t
+    float m, f, wt;  // u of the largest class, w / (t s), w / t
     int y;           // -1: no gradient
 };
 
 template <typename T>
 __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args a, const LossStat *__restrict__ stats,
-                                                             int parts, int chunk, int period, const LossPart part) {
+                                                             int parts, int chunks, int chunk, int period, const LossPart part) {
     constexpr int V = RowVecs<T>::V, U = 4;
     __shared__ GradRow rows[LB_ROWS];
     __shared__ double red_dt[LB_THREADS / 32];
     cudaGridDependencySynchronize();
-    const int K = a.k, chunks = gridDim.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t n0 = blockIdx.y % period + (int64_t)(blockIdx.y / period) * chunk * period;  // the chunk's rows: n0 + i * period
+    const int K = a.k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int id = (int)(blockIdx.y + blockIdx.z * gridDim.y);  // of the chunk
+    if (id >= chunks) return;
+    const int64_t n0 = id % period + (int64_t)(id / period) * chunk * period;  // the chunk's rows: n0 + i * period
     const int count = n0 < a.n ? (int)min((int64_t)chunk, (a.n - n0 + period - 1) / period) : 0;
-    const float rt = loss_rt(a), c = rt * LOG2E;
+    const float rt = loss_rt(a), c = loss_c(rt);
     double dt = 0.0;
     for (int i = threadIdx.x; i < count; i += LB_THREADS) {
         const int64_t n = n0 + (int64_t)i * period;
@@ -458,13 +466,12 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
         float loss = label.y >= 0 ? label.w * INFINITY : 0.f;
         if (label.open) {
             LossStat st = stats[n * parts];
-            for (int j = 1; j < parts; ++j) st = merge(st, stats[n * parts + j]);
+            for (int j = 1; j < parts; ++j) st = merge(st, stats[n * parts + j], c);
             r = {st.m, label.w * rt / st.s, label.w * rt, label.y};
             if (blockIdx.x == 0) {
-                const float gap = loss_z(to_f32(((const T *)a.cs)[n * a.cs_stride + label.y]),
-                                         a.bias ? __fmul_rn(a.bias[label.y], c) : 0.f, c) - st.m;
-                loss = label.w * (logf(st.s) - gap * LN2);
-                dt += (double)label.w * (double)(st.h / st.s - gap);
+                const float gap = loss_u(to_f32(((const T *)a.cs)[n * a.cs_stride + label.y]), a.bias ? a.bias[label.y] : 0.f) - st.m;
+                loss = label.w * (logf(st.s) - gap * rt);
+                dt += (double)label.w * ((double)(st.h / st.s) - (double)gap * (double)c);
             }
         }
         rows[i] = r;
@@ -478,18 +485,18 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         for (int i = 1; i < LB_THREADS / 32; ++i) dt += red_dt[i];
-        if (chunks > 1) part.dt[blockIdx.y] = dt;
+        if (chunks > 1) part.dt[id] = dt;
         else if (a.dtemperature) *a.dtemperature = (float)(-dt * (double)LN2 * (double)rt);
     }
     if (!a.dcs && !a.dbias) return;
-    float *const db = !a.dbias ? nullptr : chunks == 1 ? a.dbias : part.db + (int64_t)blockIdx.y * K;
+    float *const db = !a.dbias ? nullptr : chunks == 1 ? a.dbias : part.db + (int64_t)id * K;
     const int64_t row0 = min(n0, a.n - 1), in_step = (int64_t)period * a.cs_stride, out_step = (int64_t)period * K;
     const int64_t mask_step = (int64_t)period * a.allowed_stride;
     const uint32_t *const mask0 = a.allowed ? a.allowed + row0 * a.allowed_stride : nullptr;
     const RowVecs<T> in0(a.cs, row0, a.cs_stride), out0(a.dcs ? a.dcs : a.cs, row0, a.dcs ? K : a.cs_stride);
     // One class over the chunk's rows.
     const auto column = [&](int k) {
-        const float bc = a.bias ? __fmul_rn(a.bias[k], c) : 0.f;
+        const float b = a.bias ? a.bias[k] : 0.f;
         const T *in = in0.row + k;
         const uint32_t *mask = mask0 ? mask0 + (k >> 5) : nullptr;
         T *out = a.dcs ? (T *)a.dcs + row0 * (int64_t)K + k : nullptr;
@@ -499,7 +506,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
             const GradRow r = rows[i];
             float d = 0.f;
             if (r.y >= 0) {
-                if (!mask || (*mask >> (k & 31)) & 1u) d = ex2(loss_z(to_f32(*in), bc, c) - r.m) * r.f;
+                if (!mask || (*mask >> (k & 31)) & 1u) d = ex2(loss_x(loss_u(to_f32(*in), b), r.m, c)) * r.f;
                 if (r.y == k) d -= r.wt;
                 sum += d;
             }
@@ -529,10 +536,10 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
     if (vec >= end) return;
     const int k0 = vec * V - in0.off, warp_k = k0 - lane * V;
     const F2 c2 = pair(c, c);
-    F2 bc[V / 2], acc[V / 2];
+    F2 b[V / 2], acc[V / 2];
 #pragma unroll
     for (int q = 0; q < V / 2; ++q) {
-        bc[q] = a.bias ? mul2(pair(a.bias[k0 + 2 * q], a.bias[k0 + 2 * q + 1]), c2) : pair(0.f, 0.f);
+        b[q] = a.bias ? pair(a.bias[k0 + 2 * q], a.bias[k0 + 2 * q + 1]) : pair(0.f, 0.f);
         acc[q] = pair(0.f, 0.f);
     }
     const uint32_t shared_open = open_classes<V>(a.allowed_stride ? nullptr : a.allowed, k0);
@@ -567,7 +574,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
 #pragma unroll
                 for (int q = 0; q < V / 2; ++q) {
                     float x, y;
-                    split(add2(fma2(class_pair<T>(raw[u], q), c2, bc[q]), m2), x, y);
+                    split(mul2(add2(add2(class_pair<T>(raw[u], q), b[q]), m2), c2), x, y);
                     x = open[u] & (1u << (2 * q)) ? ex2(x) : 0.f;
                     y = open[u] & (2u << (2 * q)) ? ex2(y) : 0.f;
                     split(mul2(pair(x, y), f2), d[2 * q], d[2 * q + 1]);
@@ -720,7 +727,8 @@ static ytm_status launch_big(const ytm_loss_args &a, const LossPlan &p, const Lo
     if (rc) return rc;
     const uint64_t vecs = cdiv((uint64_t)a.k * sizeof(T), 16);
     const unsigned tiles = a.dcs || a.dbias ? (unsigned)cdiv(vecs, LB_THREADS) : 1;
-    return launch_after(k_loss_grad<T>, dim3(tiles, (unsigned)p.teams), LB_THREADS, st, "class loss", a, stats, p.parts,
+    const unsigned cz = (unsigned)cdiv(p.teams, 65535), cy = (unsigned)cdiv(p.teams, cz);
+    return launch_after(k_loss_grad<T>, dim3(tiles, cy, cz), LB_THREADS, st, "class loss", a, stats, p.parts, (int)p.teams,
                         p.chunk, p.period, part);
 }
 
@@ -769,7 +777,6 @@ ytm_status ytm_class_loss(const ytm_loss_args *args, void *workspace, void *stre
     }
     const LossPlan p = loss_plan(a.n, a.k, type_bytes(a.cs_type), a.cs_stride);
     const LossWs ws = loss_ws(p, a.n, a.k);
-    if (p.teams > (p.big ? 65535 : INT_MAX)) return fail(YTM_ERR_UNSUPPORTED, "class loss: too many rows for one call");
     if (!a.cs || !a.target || !a.loss || (ws.total && !workspace)) return fail(YTM_ERR_ARG, "null pointer");
     const LossPart part = {(float *)((char *)workspace + ws.db), (double *)workspace};
     LossStat *stats = (LossStat *)((char *)workspace + ws.stats);
