@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cfloat>
 #include <string>
 
 #include "../../include/ytm.h"
@@ -110,8 +111,13 @@ Knob knob(PyObject *o, const char *name, int64_t n, const Tensor &with, bool pos
     }
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw Error{nullptr, ""};
-    if (positive && !(v > 0.0)) value_error(std::string(name) + " must be positive, got " + std::to_string(v));
     k.all = (float)v;
+    // below the smallest normal number the reciprocal leaves the type
+    if (positive && !(k.all >= FLT_MIN)) {
+        char text[32];
+        PyOS_snprintf(text, sizeof text, "%g", v);
+        value_error(std::string(name) + " must be positive (at least 2^-126), got " + text);
+    }
     return k;
 }
 

@@ -257,15 +257,19 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok;
 }
-__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volatile int &failed) {
+__device__ __noinline__ bool bar_try_long(uint32_t bar, uint32_t parity) {
     uint64_t start, now;
-    if (failed) return false;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(start));
     for (int i = 0; i < (1 << 24); ++i) {
         if (bar_try(bar, parity)) return true;
         asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
         if (now - start > 2000000000ull) break;
     }
+    return false;
+}
+__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volatile int &failed) {
+    if (failed) return false;
+    if (bar_try_long(bar, parity)) return true;
     failed = 1;
     return false;
 }
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS <= 32 ? 2 : 1
     constexpr int NT = COLS / 8, SEG_BYTES = q4_seg_bytes(MODE, COLS, GROUP);
     extern __shared__ __align__(1024) char smem[];  // weights, activations; barriers at the end
     uint64_t *const bars = (uint64_t *)(smem + a.bars_at);
-    volatile int &failed = *(int *)(bars + 2 * Q4_STAGES);
+    volatile int &failed = *(int *)(bars + 2 * Q4_STAGES), &copied = *((int *)(bars + 2 * Q4_STAGES) + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int WK = 1 << a.log_wk, WM = Q4_WARPS >> a.log_wk;
     const int rank = a.cluster > 1 ? (int)cg::this_cluster().block_rank() : 0;
@@ -376,12 +380,14 @@ __global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS <= 32 ? 2 : 1
             // the weights do not wait for k_q4_x
             for (int s = 0; s < min(count, Q4_STAGES); ++s) copy_weights(s);
             asm volatile("griddepcontrol.wait;" ::: "memory");
-            for (int s = 0; s < min(count, Q4_STAGES); ++s) copy_x(s);
-            for (int s = Q4_STAGES; s < count; ++s) {
+            int s = 0;
+            for (; s < min(count, Q4_STAGES); ++s) copy_x(s);
+            for (; s < count; ++s) {
                 if (!bar_wait(empty + 8 * (s % Q4_STAGES), (s / Q4_STAGES - 1) & 1, failed)) break;
                 copy_weights(s);
                 copy_x(s);
             }
+            copied = s;
         }
     } else {
         // scales: lane t of a class holds groups t, t + 4, ... of a stage; the
@@ -545,6 +551,13 @@ __global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS <= 32 ? 2 : 1
         }
     }
     __syncthreads();  // all stages have been read
+    if (failed) {  // copies may still be on their way: the memory is not used again, nor given back, before them
+        if (tid < Q4_STAGES && tid < copied) {
+            const int s = copied - 1 - tid;
+            bar_try_long(full + 8 * (s % Q4_STAGES), (s / Q4_STAGES) & 1);
+        }
+        __syncthreads();
+    }
     // sums of the warps along the clauses and of the parts of an activation
     float *red = (float *)smem;                      // [warp][16][COLS]
     float *mine = red + Q4_WARPS * 16 * COLS;        // [samples][16 * WM]
@@ -620,7 +633,7 @@ static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group)
         const size_t smem = std::max<size_t>(Q4_STAGES * (Q4_STAGE_BYTES + (size_t)seg_bytes * wk), red) + Q4_BARS;
         if (smem > 227 * 1024) continue;
         const int64_t tiles = cdiv(K, 16 * wm) * p.z, stages = cdiv(C, Q4_SEG * wk);
-        const int64_t held = std::min<int64_t>(nt == 1 ? 3 : nt <= 4 ? 2 : 1, 227 * 1024 / (smem + 1024));  // blocks of an SM
+        const int64_t held = std::max<int64_t>(1, std::min<int64_t>(nt == 1 ? 3 : nt <= 4 ? 2 : 1, 227 * 1024 / (smem + 1024)));  // blocks of an SM
         for (int cl = 1; cl <= 16 && (cl == 1 || cl <= stages); cl *= 2) {
             const int64_t place = cl == 16 ? sms * 3 / 4 : cl == 8 ? sms * 6 / 7 : sms;  // SMs that such clusters reach
             const int64_t rounds = tiles * cl / (place * held), rest = tiles * cl % (place * held);
@@ -730,7 +743,7 @@ static ytm_status launch_q4(const Q4XArgs &xa, unsigned x_blocks, const Q4Args &
 
 static ytm_status check_q4(int32_t C, int32_t K, int32_t group, int32_t scale_type) {
     if (C <= 0 || K <= 0) return fail(YTM_ERR_ARG, "q4: clauses and classes must be positive");
-    if (C > (1 << 30)) return fail(YTM_ERR_UNSUPPORTED, "q4: more than 2^30 clauses");
+    if (C > (1 << 30) || K > (1 << 30)) return fail(YTM_ERR_UNSUPPORTED, "q4: more than 2^30 clauses or classes");
     if (group != 32 && group != 64 && group != 128) return fail(YTM_ERR_ARG, "q4: group must be 32, 64 or 128");
     if (!is_float_type(scale_type)) return fail(YTM_ERR_ARG, "q4: scales must be fp32, fp16 or bf16");
     return YTM_OK;

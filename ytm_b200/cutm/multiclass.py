@@ -77,7 +77,7 @@ class MultiClassTM(BaseTM):
         assert Yd.dim() == 1 and Yd.shape[0] == X.shape[0], "X and Y must have the same number of samples."
         cs = self._score_device(self._literals_device(X, is_X_encoded), votes=votes)
         t0 = float(self.T) / 4 if temperature is None else float(temperature)
-        n = max(1, int((Yd >= 0).sum()))
+        n = max(1, int(((Yd >= 0) & (Yd < self.number_of_outputs)).sum()))
         weight = torch.full((Yd.shape[0],), 1.0 / n, device=self.device)
         theta = torch.zeros(self.number_of_outputs + 1, device=self.device)  # bias / t0, log(temperature / t0)
         m, v = torch.zeros_like(theta), torch.zeros_like(theta)

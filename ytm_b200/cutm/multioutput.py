@@ -21,11 +21,13 @@ class MultiOutputTM(BaseTM):
         encoded_X = self._literals_device(X, is_X_encoded)
         self._fit(encoded_X, encoded_Y, **opt_args)
 
-    def score(self, X, is_X_encoded: bool, block_size: int | None = None):
+    def score(self, X, is_X_encoded: bool, block_size: int | None = None, votes=None):
+        """Class sums float32 [samples, outputs]; with `votes` (pack_votes)
+        those of the weights packed to 4 bits."""
         lits = self._literals_device(X, is_X_encoded)
-        return self._score_device(lits).cpu().numpy().astype(np.float32)
+        return self._score_device(lits, votes=votes).cpu().numpy().astype(np.float32)
 
-    def predict(self, X, is_X_encoded: bool = False, block_size: int | None = None):
-        class_sums = self.score(X, is_X_encoded, block_size=block_size)
+    def predict(self, X, is_X_encoded: bool = False, block_size: int | None = None, votes=None):
+        class_sums = self.score(X, is_X_encoded, block_size=block_size, votes=votes)
         preds = (class_sums >= 0).astype(np.uint32)  # multioutput.py:56
         return preds, class_sums
