@@ -69,30 +69,6 @@ struct LossPart {
     double *dt;
 };
 
-// Two fp32 operations in one instruction, on register pairs.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 pair(float x, float y) {
-    F2 d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-    return d;
-}
-__device__ __forceinline__ void split(F2 a, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a)); }
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-    F2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-    F2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-
 // -------------------------------------------------- rows of few classes
 // TPR threads hold a row, E classes each (e TPR + lane), in pairs for the paired
 // arithmetic.  The label's class is not looked for among them: the lane that

@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "elem.cuh"
@@ -117,6 +118,7 @@ struct Q4XArgs {
     char *xs;
     int64_t xs_block;
     int C, x_type, samples, parts, cols, segs, group;
+    bool tiles;               // for k_q4_tiles
 };
 
 // Clauses c .. c + 7 of a row (0 behind the last clause) as fp32.
@@ -166,7 +168,8 @@ __global__ void __launch_bounds__(256) k_q4_x(const Q4XArgs a) {
     if (MODE >= Q4_BF16) {
         // order (0, 4, 1, 5, 2, 6, 3, 7); the four 16-byte pieces of a (group,
         // column) are exchanged by the column's bits 1 and 2, so that the eight
-        // lanes that read two columns together meet 32 different banks
+        // lanes that read two columns together meet 32 different banks; for tiles
+        // rows of 64 clauses, the eight pieces exchanged by the column's low bits
         const uint16_t *p = (const uint16_t *)a.x + row + c;
         uint32_t w[4] = {0, 0, 0, 0};
         if (c + 8 <= a.C && (uintptr_t)p % 16 == 0) {
@@ -176,7 +179,9 @@ __global__ void __launch_bounds__(256) k_q4_x(const Q4XArgs a) {
             for (int j = 0; j < 8; ++j)
                 if (c + j < a.C) w[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
         }
-        *(uint4 *)(seg + ((in_seg >> 2) * a.cols + col) * 64 + ((o & 3) ^ (col >> 1 & 3)) * 16) =
+        const int at = a.tiles ? ((in_seg >> 3) * a.cols + col) * 128 + ((o & 7) ^ (col & 7)) * 16
+                               : ((in_seg >> 2) * a.cols + col) * 64 + ((o & 3) ^ (col >> 1 & 3)) * 16;
+        *(uint4 *)(seg + at) =
             make_uint4(__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x5410),
                        __byte_perm(w[1], w[3], 0x7632));
         return;
@@ -323,6 +328,30 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
     else
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Adds the cluster's sums `mine` [samples][2^log_rows classes from row0] in
+// rank order, and the bias, and writes the votes.
+__device__ __forceinline__ void q4_join(const Q4Args &a, float *mine, int rank, int row0, int log_rows, int64_t sample0, int samples) {
+    const int outs = samples << log_rows;
+    __syncthreads();
+    if (a.cluster > 1) cg::this_cluster().sync();
+    for (int u = rank * (int)blockDim.x + (int)threadIdx.x; u < outs; u += a.cluster * (int)blockDim.x) {
+        const int i = u >> log_rows, r = u & ((1 << log_rows) - 1);
+        float v = 0.f;
+        if (a.cluster > 1) {
+            for (int k = 0; k < a.cluster; ++k) v += *cg::this_cluster().map_shared_rank(mine + u, k);
+        } else {
+            v = mine[u];
+        }
+        if (row0 + r >= a.K) continue;
+        if (a.bias) v += a.bias[row0 + r];
+        const int64_t at = (sample0 + i) * a.K + row0 + r;
+        if (a.y_type == YTM_F32) ((float *)a.y)[at] = v;
+        else if (a.y_type == YTM_F16) ((__half *)a.y)[at] = __float2half_rn(v);
+        else ((__nv_bfloat16 *)a.y)[at] = __float2bfloat16_rn(v);
+    }
+    if (a.cluster > 1) cg::this_cluster().sync();  // nobody leaves while its sums are read
 }
 
 // COLS: the columns of a block, padded to a multiple of 8.
@@ -578,24 +607,322 @@ __global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS <= 32 ? 2 : 1
             for (int p = 0; p < a.parts; ++p) v += red[((k * WM + (r >> 4)) * 16 + (r & 15)) * COLS + i * a.parts + p];
         mine[u] = v;
     }
-    __syncthreads();
-    if (a.cluster > 1) cg::this_cluster().sync();
-    for (int u = rank * Q4_THREADS + tid; u < outs; u += a.cluster * Q4_THREADS) {
-        const int i = u >> log_rows, r = u & (rows - 1);
-        float v = 0.f;
-        if (a.cluster > 1) {
-            for (int k = 0; k < a.cluster; ++k) v += *cg::this_cluster().map_shared_rank(mine + u, k);
-        } else {
-            v = mine[u];
+    q4_join(a, mine, rank, row0, log_rows, sample0, samples);
+}
+
+// ---- products of many 16-bit activations on the tensor cores' own memory
+//
+// A block takes 256 classes as two products of 128 by COLS.  Sixteen warps turn
+// words into 16-bit pairs as above, a thread a class, and store them into the
+// tensor memory as the products' first operand; the activations are the second,
+// from shared memory.  A group's sums land in one of two accumulators a
+// product, from which eight other warps add them, scaled, to theirs in
+// registers.  Every step is handed on by a barrier in shared memory, so copies,
+// conversion, products and scaling all run at once, and the hand-overs' latency
+// bounds them: leaving out three products of four saves 5%, the conversion's
+// arithmetic nothing.  That set the sizes: operands of 128 clauses (of 64: 15%
+// slower), two halves of converting warps that take turns (one: 30% slower at 64
+// samples), a warp for each product.  8192 x 16384, groups of 64, 64 samples:
+// 38 us, 445 TFLOP/s (k_q4_votes 76); groups of 128 29 us.
+
+constexpr int QT_TILES = 2;                           // products of a block
+constexpr int QT_THREADS = 32 * 27;                   // 16 warps convert, 8 scale, one copies, one issues each product
+constexpr int QT_SCALE = 16, QT_COPY = 24, QT_ISSUE = 25;  // their first
+constexpr int QT_ROWS = 128 * QT_TILES, QT_W_BYTES = QT_ROWS * 128;
+constexpr int QT_BARS = 384;
+
+__host__ __device__ constexpr int qt_stages(int cols) { return cols == 64 ? 3 : 4; }  // what shared memory holds
+
+struct QtBars {
+    uint64_t full[4], empty[4], a_full[QT_TILES][4], a_empty[QT_TILES][4], d_full[QT_TILES][2], d_empty[QT_TILES][2], done[QT_TILES];
+    uint32_t tmem;
+    int failed, copied;
+};
+static_assert(sizeof(QtBars) <= QT_BARS, "barriers");
+
+// bar_try_long and bar_wait without a call, which a kernel that deals out its
+// registers cannot make; `stop`: ends the wait at once, or NULL.
+__device__ __forceinline__ bool bar_poll(uint32_t bar, uint32_t parity, volatile int *stop) {
+    if (bar_try(bar, parity)) return true;
+    const long long start = clock64();
+    do {
+        if (bar_try(bar, parity)) return true;
+        if (stop && *stop) return false;
+    } while (clock64() - start < 4000000000ll);  // about two seconds
+    return false;
+}
+__device__ __forceinline__ bool bar_wait_inline(uint32_t bar, uint32_t parity, volatile int &failed) {
+    const bool ok = bar_poll(bar, parity, &failed);
+    if (!ok) failed = 1;
+    return ok;
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Arrives at the barrier when the products issued so far are done.
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile("{.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void tc_store16(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tc_load16(uint32_t at, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(at) : "memory");
+}
+
+// One lane of a whole warp, always the same.
+__device__ __forceinline__ bool elected() {
+    uint32_t is;
+    asm volatile("{.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;}" : "=r"(is));
+    return is;
+}
+
+// COLS: the samples of a block, padded to 32, 48 or 64.
+template <bool HALF, int COLS, int GROUP>
+__global__ void __launch_bounds__(QT_THREADS, 1) k_q4_tiles(const Q4Args a, const __grid_constant__ CUtensorMap weights) {
+    constexpr int STAGES = qt_stages(COLS), X_BYTES = COLS * 512, STAGE = QT_W_BYTES + X_BYTES, GPS = Q4_SEG / GROUP;
+    // columns of the tensor memory: accumulators [ND][tile][COLS], operands of 128
+    // clauses [NA][tile][64]; a stage has a whole number of turns of both
+    constexpr int ND = 2, NA = 2, KB = Q4_SEG / NA;
+    constexpr uint32_t A_AT = ND * QT_TILES * COLS;
+    static_assert(A_AT + NA * QT_TILES * KB / 2 <= 512 && GPS % ND == 0, "tensor memory");
+    extern __shared__ __align__(1024) char smem[];
+    QtBars &bars = *(QtBars *)(smem + a.bars_at);
+    volatile int &failed = bars.failed, &copied = bars.copied;
+    const auto bar = [](const uint64_t &b) { return (uint32_t)__cvta_generic_to_shared(&b); };
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = a.cluster > 1 ? (int)cg::this_cluster().block_rank() : 0;
+    const int row0 = (int)(blockIdx.x / a.cluster) * QT_ROWS;
+    const int per = (a.stages + a.cluster - 1) / a.cluster;
+    const int first = min(rank * per, a.stages), count = min(first + per, a.stages) - first;
+    const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem);
+    if (tid == 0) {
+        failed = 0;
+        copied = 0;
+        for (int s = 0; s < STAGES; ++s) {
+            bar_init(bar(bars.full[s]), 1);
+            bar_init(bar(bars.empty[s]), 16 + QT_TILES);  // the converting warps and the products
         }
-        if (row0 + r >= a.K) continue;
-        if (a.bias) v += a.bias[row0 + r];
-        const int64_t at = (sample0 + i) * a.K + row0 + r;
-        if (a.y_type == YTM_F32) ((float *)a.y)[at] = v;
-        else if (a.y_type == YTM_F16) ((__half *)a.y)[at] = __float2half_rn(v);
-        else ((__nv_bfloat16 *)a.y)[at] = __float2bfloat16_rn(v);
+        for (int t = 0; t < QT_TILES; ++t) {
+            for (int s = 0; s < NA; ++s) {
+                bar_init(bar(bars.a_full[t][s]), 4);
+                bar_init(bar(bars.a_empty[t][s]), 1);
+            }
+            for (int s = 0; s < ND; ++s) {
+                bar_init(bar(bars.d_full[t][s]), 1);
+                bar_init(bar(bars.d_empty[t][s]), 4);
+            }
+            bar_init(bar(bars.done[t]), 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (a.cluster > 1) cg::this_cluster().sync();  // nobody leaves while its sums are read
+    if (warp == QT_ISSUE) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"((uint32_t)__cvta_generic_to_shared(&bars.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // all 512 columns are this block's, so they start at 0: the products' addresses are constants
+    constexpr uint32_t tmem = 0;
+    if (tid == 0 && *(volatile uint32_t *)&bars.tmem != tmem) failed = 1;
+    const int part = warp >> 2 & 1;                       // product of a converting or scaling warp
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;    // its lanes of the tensor memory
+    const int row = part * 128 + (warp & 3) * 32 + lane;  // and the thread's class
+
+    const int64_t sample0 = a.n0 + (int64_t)blockIdx.z * a.samples;
+    const int samples = (int)min((int64_t)a.samples, a.n0 + a.n - sample0);
+    float *const mine = (float *)smem;  // [samples][QT_ROWS]
+
+    if (warp == QT_COPY) {
+        if (lane == 0) {
+            const char *const x0 = a.xs + blockIdx.z * a.xs_block + (int64_t)first * X_BYTES;
+            const auto copy_weights = [&](int s) {
+                const uint32_t at = smem_at + s % STAGES * STAGE, b = bar(bars.full[s % STAGES]);
+                bar_expect(b, STAGE);
+                asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                             ::"r"(at), "l"(&weights), "r"((first + s) * 128), "r"(row0), "r"(b) : "memory");
+            };
+            const auto copy_x = [&](int s) {
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                             ::"r"(smem_at + s % STAGES * STAGE + QT_W_BYTES), "l"(x0 + (int64_t)s * X_BYTES), "r"(X_BYTES),
+                               "r"(bar(bars.full[s % STAGES])) : "memory");
+            };
+            for (int s = 0; s < min(count, STAGES); ++s) copy_weights(s);  // they do not wait for k_q4_x
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            int s = 0;
+            for (; s < min(count, STAGES); ++s) copy_x(s);
+            for (; s < count; ++s) {
+                if (!bar_wait_inline(bar(bars.empty[s % STAGES]), (s / STAGES - 1) & 1, failed)) break;
+                copy_weights(s);
+                copy_x(s);
+            }
+            copied = s;
+        }
+    } else if (warp >= QT_ISSUE) {
+        // The whole warp goes along, so that addresses stay in uniform registers; one
+        // lane issues (an `if (lane == 0)` around all of this took 100 cycles a product).
+        // fp32 sums; operands fp16 or bf16, both with the clauses innermost; 128 by COLS
+        constexpr uint32_t SHAPE = 1u << 4 | (HALF ? 0u : 1u << 7 | 1u << 10) | (uint32_t)(COLS / 8) << 17 | 8u << 24;
+        const auto issue = [&](auto product, int s) {
+            constexpr int t = decltype(product)::value;
+            if (!bar_wait_inline(bar(bars.full[s % STAGES]), (s / STAGES) & 1, failed)) return false;
+            // rows of 128 bytes under the 128-byte swizzle, eight of them 1024 bytes from the next eight
+            const uint64_t x = (uint64_t)((smem_at + s % STAGES * STAGE + QT_W_BYTES) >> 4) | 1ull << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
+#pragma unroll
+            for (int j = 0; j < NA; ++j) {
+                if (!bar_wait_inline(bar(bars.a_full[t][j]), s & 1, failed)) return false;
+#pragma unroll
+                for (int k0 = 0; k0 < KB; k0 += GROUP) {  // products into one accumulator
+                    const int g = (j * KB + k0) / GROUP;  // of the stage
+                    // the accumulator's last turn: in this stage or the one before
+                    if ((s > 0 || g >= ND) && !bar_wait_inline(bar(bars.d_empty[t][g % ND]), (s * (GPS / ND) + g / ND - 1) & 1, failed))
+                        return false;
+                    tc_fence_after();
+                    if (elected()) {
+#pragma unroll
+                        for (int k = k0; k < k0 + GROUP; k += 16)
+                            tc_mma((g % ND * QT_TILES + t) * COLS, A_AT + (j * QT_TILES + t) * (KB / 2) + k / 2,
+                                   x + (uint64_t)((j * KB + k) / 64 * COLS * 8 + k % 64 / 8), SHAPE, k > k0);
+                        tc_commit(bar(bars.d_full[t][g % ND]));
+                        if (k0 + GROUP == KB) tc_commit(bar(bars.a_empty[t][j]));
+                        if (k0 + GROUP == KB && j == NA - 1) tc_commit(bar(bars.empty[s % STAGES]));
+                    }
+                    __syncwarp();
+                }
+            }
+            return true;
+        };
+        const auto run = [&](auto product) {
+            bool ok = true;
+            for (int s = 0; s < count && ok; ++s) ok = __all_sync(0xFFFFFFFFu, issue(product, s));
+            if (ok) return;
+            // the products on their way still read their operands
+            if (elected()) tc_commit(bar(bars.done[decltype(product)::value]));
+            bar_poll(bar(bars.done[decltype(product)::value]), 0, nullptr);
+        };
+        if (warp == QT_ISSUE) run(std::integral_constant<int, 0>());
+        else run(std::integral_constant<int, 1>());
+    } else if (warp < QT_SCALE) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        const char *const w_row = smem + row * 128;
+        // a half of the warps has an operand each, so that one computes while the other waits
+        const int j = warp >> 3;
+        const uint32_t at = tmem + lanes + A_AT + (j * QT_TILES + part) * (KB / 2);
+        for (int s = 0; s < count; ++s) {
+            bar_wait_inline(bar(bars.full[s % STAGES]), (s / STAGES) & 1, failed);
+            __syncwarp();
+            const char *const w_at = w_row + s % STAGES * STAGE;
+#pragma unroll
+            for (int h = 0; h < KB / 32; ++h) {
+                const uint4 q = *(const uint4 *)(w_at + ((j * (KB / 32) + h) ^ (row & 7)) * 16);
+                uint32_t v[16], p[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    unpack<HALF>(i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w, p);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[i * 4 + e] = p[e];
+                }
+                if (h == 0) {
+                    if (s > 0) bar_wait_inline(bar(bars.a_empty[part][j]), (s - 1) & 1, failed);
+                    __syncwarp();
+                    tc_fence_after();
+                }
+                tc_store16(at + h * 16, v);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                bar_arrive(bar(bars.a_full[part][j]));
+                bar_arrive(bar(bars.empty[s % STAGES]));  // its words have come: their conversion is stored
+            }
+        }
+    } else {
+        // of the block's 864 * 72 registers: 512 * 48 for conversion, 256 * 120 here, 96 * 72
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+        F2 acc[COLS / 2];
+#pragma unroll
+        for (int i = 0; i < COLS / 2; ++i) acc[i] = pair(0.f, 0.f);
+        // scales of a few groups; the next ones are on their way
+        constexpr int CH = GPS < 4 || COLS == 64 ? 2 : 4, AT_ONCE = COLS == 64 ? 32 : COLS == 48 ? 16 : COLS;
+        const int k = row0 + row, G = a.G;
+        const int64_t of = k < a.K ? (int64_t)k * G : 0;
+        const int chunks = count * (GPS / CH);
+        uint32_t next[CH];
+        const auto load_scales = [&](int c) {
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const int g = first * GPS + c * CH + j;
+                next[j] = 0u;  // behind the last group: 0
+                if (g < G) next[j] = a.scale_type == YTM_F32 ? ((const uint32_t *)a.scales)[of + g] : ((const uint16_t *)a.scales)[of + g];
+            }
+        };
+        load_scales(0);
+        for (int c = 0, g = 0; c < chunks; ++c) {
+            float sc[CH];
+#pragma unroll
+            for (int j = 0; j < CH; ++j) sc[j] = scale_value(next[j], a.scale_type);
+            if (c + 1 < chunks) load_scales(c + 1);
+#pragma unroll
+            for (int j = 0; j < CH; ++j, ++g) {
+                bar_wait_inline(bar(bars.d_full[part][g % ND]), (g / ND) & 1, failed);
+                __syncwarp();
+                tc_fence_after();
+                const F2 s2 = pair(sc[j], sc[j]);
+                const uint32_t at = tmem + lanes + (g % ND * QT_TILES + part) * COLS;
+#pragma unroll
+                for (int i0 = 0; i0 < COLS; i0 += AT_ONCE) {
+                    uint32_t d[AT_ONCE / 16][16];
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE / 16; ++i) tc_load16(at + i0 + i * 16, d[i]);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (i0 + AT_ONCE == COLS) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(bar(bars.d_empty[part][g % ND]));
+                    }
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE / 2; ++i)
+                        acc[i0 / 2 + i] = fma2(pair(__uint_as_float(d[i / 8][2 * i % 16]), __uint_as_float(d[i / 8][2 * i % 16 + 1])), s2, acc[i0 / 2 + i]);
+                }
+            }
+        }
+        // The sums go over the first stage, which the other product, up to two stages
+        // behind, may still read: first the scaling warps wait for one another.
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < COLS / 2; ++i) {
+            float v, w;
+            split(acc[i], v, w);
+            if (2 * i < samples) mine[2 * i * QT_ROWS + row] = v;
+            if (2 * i + 1 < samples) mine[(2 * i + 1) * QT_ROWS + row] = w;
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == QT_ISSUE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (failed) {  // copies may still be on their way; the sums are none
+        if (tid < STAGES && tid < copied) {
+            const int s = copied - 1 - tid;
+            bar_poll(bar(bars.full[s % STAGES]), (s / STAGES) & 1, nullptr);
+        }
+        __syncthreads();
+        for (int u = tid; u < samples * QT_ROWS; u += QT_THREADS) mine[u] = NAN;
+    }
+    q4_join(a, mine, rank, row0, 8, sample0, samples);
 }
 
 // How a call is cut.  The cost of a cut in microseconds, as measured: a stage of
@@ -610,12 +937,44 @@ struct Q4Plan {
     int wm, log_wk, cluster, stages;
     int64_t z, xs_block;       // blocks of samples of a launch, bytes of one's activations
     size_t smem;
+    bool tiles;                // k_q4_tiles
 };
+
+// A stage takes 1.4 to 1.8 us, a block 3 more to start and to end, 5 in a cluster.
+static void tiles_plan(Q4Plan &p, int64_t N, int64_t C, int64_t K) {
+    p.tiles = true;
+    p.samples = (int)cdiv(N, cdiv(N, (int64_t)64));
+    p.cols = std::max(32, (p.samples + 15) / 16 * 16);
+    p.z = std::min<int64_t>(cdiv(N, p.samples), 65535);
+    p.wm = QT_ROWS / 16;
+    p.stages = (int)cdiv(C, Q4_SEG);
+    p.xs_block = (int64_t)p.cols * 512 * p.stages;
+    p.smem = qt_stages(p.cols) * (QT_W_BYTES + (size_t)p.cols * 512) + QT_BARS;
+    const int64_t sms = sm_count(), tiles = cdiv(K, QT_ROWS) * p.z;
+    double least = 0;
+    for (int cl = 1; cl <= 16 && (cl == 1 || cl <= p.stages); cl *= 2) {
+        const int64_t place = cl == 16 ? sms * 3 / 4 : cl == 8 ? sms * 6 / 7 : sms;
+        const double cost = (double)cdiv(tiles * cl, place) * ((double)cdiv(p.stages, cl) * 1.6 + (cl > 1 ? 5 : 3));
+        if (!p.cluster || cost < least * 0.97) {
+            p.cluster = cl;
+            least = cost;
+        }
+    }
+}
 
 static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group) {
     Q4Plan p = {};
     p.mode = x_type == YTM_BITS ? Q4_BITS : x_type == YTM_F32 || (N <= 2 && K >= 1024) ? Q4_DIGITS : x_type == YTM_F16 ? Q4_FP16 : Q4_BF16;
     p.parts = p.mode == Q4_DIGITS ? 4 : 1;
+    // Tiles cost 2 us more to set up and as much for 3 samples as for 16, so they
+    // are for many samples of many classes; scaling bounds them under groups of 32.
+    // 8192 x 16384, groups of 64: 16 samples 25 us against 28 in k_q4_votes, 24 31
+    // against 37, 64 38 against 76; groups of 32: 17 44 against 39, 32 44 against 55.
+    // 16384 x 512, groups of 64: 17 13.0 against 11.9, 32 13.3 against 14.9.
+    if (p.mode >= Q4_BF16 && N > (group == 32 ? 24 : 16) && K >= 512) {
+        tiles_plan(p, N, C, K);
+        return p;
+    }
     // digits: blocks of up to 8 samples, two an SM (21 samples of 8192 x 16384: 92 us
     // against 112 with 16); else up to 64 (64 samples: 76 us against 98 with 32)
     const int64_t most = p.mode == Q4_DIGITS ? 8 : 64;
@@ -696,15 +1055,15 @@ static EncodeTiled encode_tiled() {
     return f;
 }
 
-template <Q4Mode MODE, int COLS, int GROUP>
-static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, dim3 grid, cudaStream_t st) {
-    static std::atomic<uint64_t> done{0};
-    auto *f = k_q4_votes<MODE, COLS, GROUP>;
+using Q4Kernel = void (*)(const Q4Args, const CUtensorMap);
+
+static ytm_status launch_q4(Q4Kernel f, std::atomic<uint64_t> &done, unsigned threads, const Q4Args &a, const Q4Plan &p,
+                            const CUtensorMap &map, dim3 grid, cudaStream_t st) {
     ytm_status rc = allow_smem(f, 227 * 1024, done);
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(Q4_THREADS);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = p.smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -716,6 +1075,34 @@ static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap 
     cfg.attrs = at;
     cfg.numAttrs = p.cluster > 1 ? 2 : 1;
     return cuda_check(cudaLaunchKernelEx(&cfg, f, a, map), "q4 votes");
+}
+
+template <Q4Mode MODE, int COLS, int GROUP>
+static ytm_status launch_q4(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, dim3 grid, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    return launch_q4(k_q4_votes<MODE, COLS, GROUP>, done, Q4_THREADS, a, p, map, grid, st);
+}
+
+template <bool HALF, int COLS, int GROUP>
+static ytm_status launch_tiles(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, dim3 grid, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    return launch_q4(k_q4_tiles<HALF, COLS, GROUP>, done, QT_THREADS, a, p, map, grid, st);
+}
+
+template <bool HALF, int COLS>
+static ytm_status launch_tiles(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, int group, dim3 grid, cudaStream_t st) {
+    if (group == 32) return launch_tiles<HALF, COLS, 32>(a, p, map, grid, st);
+    if (group == 64) return launch_tiles<HALF, COLS, 64>(a, p, map, grid, st);
+    return launch_tiles<HALF, COLS, 128>(a, p, map, grid, st);
+}
+
+template <bool HALF>
+static ytm_status launch_tiles(const Q4Args &a, const Q4Plan &p, const CUtensorMap &map, int group, dim3 grid, cudaStream_t st) {
+    switch (p.cols) {
+        case 32: return launch_tiles<HALF, 32>(a, p, map, group, grid, st);
+        case 48: return launch_tiles<HALF, 48>(a, p, map, group, grid, st);
+        default: return launch_tiles<HALF, 64>(a, p, map, group, grid, st);
+    }
 }
 
 template <Q4Mode MODE, int COLS>
@@ -731,6 +1118,8 @@ static ytm_status launch_q4(const Q4XArgs &xa, unsigned x_blocks, const Q4Args &
     k_q4_x<MODE><<<x_blocks, 256, 0, st>>>(xa);
     ytm_status rc = launch_check("q4 activations");
     if (rc) return rc;
+    if constexpr (MODE >= Q4_BF16)
+        if (p.tiles) return launch_tiles<MODE == Q4_FP16>(a, p, map, group, grid, st);
     switch (p.cols) {
         case 8: return launch_q4<MODE, 8>(a, p, map, group, grid, st);
         case 16: return launch_q4<MODE, 16>(a, p, map, group, grid, st);
@@ -813,11 +1202,11 @@ ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t
     const int segs = p.stages << p.log_wk;
     for (int64_t i = 0; i < N; i += most) {
         const int64_t n = std::min(N - i, most);
-        const Q4XArgs xa = {x, x_stride, i, n, (char *)workspace, p.xs_block, C, x_type, p.samples, p.parts, p.cols, segs, group};
+        const Q4XArgs xa = {x, x_stride, i, n, (char *)workspace, p.xs_block, C, x_type, p.samples, p.parts, p.cols, segs, group, p.tiles};
         const uint64_t blocks = cdiv((uint64_t)n * segs * 32, 256);
         if (blocks > INT_MAX) return fail(YTM_ERR_UNSUPPORTED, "q4 votes: too many activations for one call");
         const Q4Args a = {(const char *)workspace, scales, bias, y, i, n, p.xs_block, K, (int)cdiv(C, group), p.stages, scale_type,
-                          y_type, p.samples, p.parts, p.log_wk, p.cluster, (int)p.smem - Q4_BARS, 0u};
+                          y_type, p.samples, p.parts, p.log_wk, p.cluster, (int)p.smem - (p.tiles ? QT_BARS : Q4_BARS), 0u};
         const dim3 grid((unsigned)(cdiv(K, 16 * p.wm) * p.cluster), 1, (unsigned)cdiv(n, p.samples));
         switch (p.mode) {
             case Q4_BITS: rc = launch_q4<Q4_BITS>(xa, (unsigned)blocks, a, p, map, group, grid, st); break;
