@@ -361,8 +361,9 @@ ytm_status ytm_match_counters(uint64_t *out, void *stream);
  * the class sums (src/cutm/multiclass.py:54-59).  They take plain arrays (no
  * ytm_config); rows are strided (strides in elements), the elements of a row
  * contiguous, and a stride of 0 repeats one row.  Indices and sizes are 64-bit
- * inside.  Calls keep nothing between them and may overlap on different
- * streams. */
+ * inside; more than 2^31 - 1 rows of `n` or 2^30 clauses or classes are refused
+ * with YTM_ERR_UNSUPPORTED.  Calls keep nothing between them and may overlap on
+ * different streams, each with its own workspace. */
 #define YTM_I32 0
 #define YTM_F32 1
 #define YTM_F16 2
@@ -374,14 +375,17 @@ ytm_status ytm_match_counters(uint64_t *out, void *stream);
  * max |w|, scale = a / 7 (rounded to scale_type) and q = round-half-even(7 w /
  * a) in [-7, 7].  packed u8 [K][16 * ceil(C / 32)]: q + 8, clause c in byte c /
  * 2, low half when c is even, 8 behind the last clause.  scales [K][ceil(C /
- * group)]. */
+ * group)]; f16 scales hold weights of up to 7 * 65504. */
 ytm_status ytm_q4_pack(const void *weights, int32_t w_type, int64_t w_stride, int32_t C, int32_t K, int32_t group,
                        uint8_t *packed, void *scales, int32_t scale_type, void *stream);
 
 /* Votes y[n][k] = bias[k] + sum_g scale[k][g] * sum_{c in g} (packed[k][c] - 8)
  * * x[n][c], sums in fp32, rounded once to y_type.  x [N][C] (f32, f16, bf16)
  * or clause bits (YTM_BITS, x_stride in words); packed on a 16-byte boundary,
- * halves 0..15; bias f32 [K] or NULL; y [N][K].  workspace:
+ * halves 0..15; bias f32 [K] or NULL; y [N][K].  f32 activations, and 16-bit
+ * ones of one or two samples, are held to 2^-30 of the largest of their 128
+ * neighbouring clauses (128 i .. 128 i + 127); several infinities among those
+ * give NaN.  workspace:
  * ytm_q4_votes_workspace_bytes(...), on a 16-byte boundary. */
 ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t N, int32_t C, const uint8_t *packed,
                         const void *scales, int32_t scale_type, int32_t group, int32_t K, const float *bias, void *y,
@@ -431,7 +435,8 @@ ytm_status ytm_answer(const ytm_answer_args *args, void *stream);
 /* Cross entropy with z as above (no penalties): loss[n] = weight[n] *
  * (log sum exp z - z[target[n]]), and with d = weight (softmax z - onehot) the
  * gradients dcs = d / temperature, dbias = sum_n d / temperature and
- * dtemperature = -sum d z / temperature, summed in a fixed order.  Rows whose
+ * dtemperature = -sum d z / temperature, summed in a fixed order.  A NaN among
+ * a row's allowed class sums makes its loss and its gradients NaN.  Rows whose
  * target lies outside [0, k) or whose weight is 0 count for nothing; a target
  * that the mask forbids gives a loss of weight * inf and no gradient. */
 typedef struct ytm_loss_args {

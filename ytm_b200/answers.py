@@ -56,7 +56,8 @@ def q4_pack(weights: torch.Tensor, group: int = 64, scale_dtype: torch.dtype = t
     """Clause weights [clauses, classes] (int32 or float32, finite) -> (packed
     uint8 [classes, 16 * ceil(clauses / 32)], scales [classes, ceil(clauses /
     group)]): per class and `group` (32, 64, 128) consecutive clauses the scale
-    max|w| / 7 and the weights rounded to [-7, 7] of it (half to even)."""
+    max|w| / 7 and the weights rounded to [-7, 7] of it (half to even).  float16
+    scales hold weights of up to 7 * 65504."""
     return _bind.q4_pack(weights, group, scale_dtype)
 
 
@@ -68,7 +69,10 @@ def q4_votes(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group:
 
     x: real activations [n, clauses] (float32, float16, bfloat16), or clause
     outputs as bits, int32 [n, ceil(clauses / 32)] (`CudaEngine.infer_fired`);
-    with bits, `clauses` is needed.  bias: float32 [classes]."""
+    with bits, `clauses` is needed.  bias: float32 [classes].  float32
+    activations, and 16-bit ones of one or two samples, are held to 2^-30 of the
+    largest of their 128 neighbouring clauses; several infinities among those
+    give NaN."""
     return _bind.q4_votes(x, packed, scales, group, bias, clauses, out_dtype)
 
 
@@ -114,5 +118,6 @@ def class_loss(cs: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None
     of 0 count for nothing.  A target that its mask forbids gives weight * inf
     and no gradient.  bias: float32 [k]; allowed as for `answer`; temperature:
     a positive number or float32 [1], whose value is not checked; weight:
-    float32 [n]."""
+    float32 [n].  A NaN among a row's allowed class sums makes its loss and
+    gradients NaN."""
     return _bind.class_loss(cs, target, bias, allowed, temperature, weight)

@@ -6,6 +6,7 @@
 
 #include <atomic>
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 #include "elem.cuh"
@@ -962,22 +963,8 @@ static void tiles_plan(Q4Plan &p, int64_t N, int64_t C, int64_t K) {
     }
 }
 
-static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group) {
-    Q4Plan p = {};
-    p.mode = x_type == YTM_BITS ? Q4_BITS : x_type == YTM_F32 || (N <= 2 && K >= 1024) ? Q4_DIGITS : x_type == YTM_F16 ? Q4_FP16 : Q4_BF16;
-    p.parts = p.mode == Q4_DIGITS ? 4 : 1;
-    // Tiles cost 2 us more to set up and as much for 3 samples as for 16, so they
-    // are for many samples of many classes; scaling bounds them under groups of 32.
-    // 8192 x 16384, groups of 64: 16 samples 25 us against 28 in k_q4_votes, 24 31
-    // against 37, 64 38 against 76; groups of 32: 17 44 against 39, 32 44 against 55.
-    // 16384 x 512, groups of 64: 17 13.0 against 11.9, 32 13.3 against 14.9.
-    if (p.mode >= Q4_BF16 && N > (group == 32 ? 24 : 16) && K >= 512) {
-        tiles_plan(p, N, C, K);
-        return p;
-    }
-    // digits: blocks of up to 8 samples, two an SM (21 samples of 8192 x 16384: 92 us
-    // against 112 with 16); else up to 64 (64 samples: 76 us against 98 with 32)
-    const int64_t most = p.mode == Q4_DIGITS ? 8 : 64;
+// Blocks of k_q4_votes of up to `most` samples, and the least cost.
+static std::pair<Q4Plan, double> cut(Q4Plan p, int64_t N, int64_t C, int64_t K, int group, int64_t most) {
     p.samples = (int)cdiv(N, cdiv(N, most));
     p.z = std::min<int64_t>(cdiv(N, p.samples), 65535);
     const int used = p.samples * p.parts;
@@ -996,7 +983,7 @@ static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group)
         for (int cl = 1; cl <= 16 && (cl == 1 || cl <= stages); cl *= 2) {
             const int64_t place = cl == 16 ? sms * 3 / 4 : cl == 8 ? sms * 6 / 7 : sms;  // SMs that such clusters reach
             const int64_t rounds = tiles * cl / (place * held), rest = tiles * cl % (place * held);
-            const auto stage = [&](int64_t r) { return std::max(0.37 * r, 0.15 * nt * (1 + r)); };
+            const auto stage = [&](int64_t r) { return std::max(0.37 * r, nt > 4 ? 0.19 * nt * r : 0.15 * nt * (1 + r)); };
             const double per = (double)cdiv(stages, cl);
             const double cost = per * (rounds * stage(held) + (rest ? stage(cdiv(rest, place)) : 0)) +
                                 (rounds - (rest ? 0 : 1)) * (cl > 1 ? 6 : 3);
@@ -1011,7 +998,28 @@ static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group)
             }
         }
     }
-    return p;
+    return {p, least};
+}
+
+static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group) {
+    Q4Plan p = {};
+    p.mode = x_type == YTM_BITS ? Q4_BITS : x_type == YTM_F32 || (N <= 2 && K >= 1024) ? Q4_DIGITS : x_type == YTM_F16 ? Q4_FP16 : Q4_BF16;
+    p.parts = p.mode == Q4_DIGITS ? 4 : 1;
+    // Tiles cost 2 us more to set up and as much for 3 samples as for 16, so they
+    // are for many samples of many classes; scaling bounds them under groups of 32.
+    // 8192 x 16384, groups of 64: 16 samples 25 us against 28 in k_q4_votes, 24 31
+    // against 37, 64 38 against 76; groups of 32: 17 44 against 39, 32 44 against 55.
+    // 16384 x 512, groups of 64: 17 13.0 against 11.9, 32 13.3 against 14.9.
+    if (p.mode >= Q4_BF16 && N > (group == 32 ? 24 : 16) && K >= 512) {
+        tiles_plan(p, N, C, K);
+        return p;
+    }
+    // digits: blocks of up to 8 samples, two an SM (21 samples of 8192 x 16384: 92 us
+    // against 112 with 16); else of up to 64 or 32, whichever costs less (bits, 64
+    // samples of 8192 x 16384: 54 us against 58, 256 of 65536 x 100: 48 against 37)
+    if (p.mode == Q4_DIGITS) return cut(p, N, C, K, group, 8).first;
+    const auto wide = cut(p, N, C, K, group, 64), narrow = cut(p, N, C, K, group, 32);
+    return narrow.second < wide.second ? narrow.first : wide.first;
 }
 
 // The thread's last plan again if the sizes are the same: the workspace's size
