@@ -106,7 +106,7 @@ def test_votes(n, c, k, group, scale, out, x):
     check_votes(answers.q4_votes(xt, packed, scales, group, clauses=c), xv, q, scales, group, np.zeros(k), "f32", c)
 
 
-@pytest.mark.parametrize("x", ["f16", "bf16"])
+@pytest.mark.parametrize("x", ["bits", "f16", "bf16"])
 @pytest.mark.parametrize("n,c,k,group,scale,out", [
     (3, 64, 512, 64, "f32", "f32"), (3, 1, 513, 32, "f32", "f32"), (16, 256, 700, 32, "f16", "f32"), (17, 257, 1025, 128, "f32", "f16"),
     (33, 4000, 600, 64, "bf16", "f32"), (48, 2500, 2000, 32, "f16", "bf16"), (49, 1023, 999, 128, "f32", "f32"),
@@ -155,6 +155,7 @@ def test_votes_of_no_samples_and_infinite_activations():
 @pytest.mark.parametrize("n,c,k,x,group,scale", [(1, 16384, 32768, "bf16", 32, "f32"), (1, 16384, 20011, "f32", 128, "f16"),
                                                  (2, 8192, 30000, "f16", 64, "bf16"), (7, 8192, 20000, "bf16", 32, "f32"),
                                                  (1, 16384, 30000, "bits", 64, "f32"), (64, 16384, 8192, "bf16", 32, "f32"),
+                                                 (64, 16384, 9000, "bits", 64, "f16"),
                                                  (40, 16384, 20011, "f16", 64, "f16"), (48, 10000, 16000, "bf16", 128, "f32")])
 def test_votes_again_and_again(n, c, k, x, group, scale):
     """Streams of many stages over all SMs, call after call on two inputs: a

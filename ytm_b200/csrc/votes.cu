@@ -165,12 +165,13 @@ __global__ void __launch_bounds__(256) k_q4_x(const Q4XArgs a) {
     const int o = (int)(u - i * octets), c = o * 8, in_seg = o & 31;
     const int64_t row = (a.n0 + i) * a.x_stride;
     const int col = (int)(i % a.samples) * a.parts;
-    char *const seg = a.xs + i / a.samples * a.xs_block + (int64_t)(o >> 5) * q4_seg_bytes(MODE, a.cols, a.group);
+    char *const seg = a.xs + i / a.samples * a.xs_block + (int64_t)(o >> 5) * q4_seg_bytes(a.tiles ? Q4_FP16 : MODE, a.cols, a.group);
+    // for tiles: rows of 64 clauses, their eight 16-byte pieces exchanged by the column's low bits
+    const int tile_at = ((in_seg >> 3) * a.cols + col) * 128 + ((o & 7) ^ (col & 7)) * 16;
     if (MODE >= Q4_BF16) {
         // order (0, 4, 1, 5, 2, 6, 3, 7); the four 16-byte pieces of a (group,
         // column) are exchanged by the column's bits 1 and 2, so that the eight
-        // lanes that read two columns together meet 32 different banks; for tiles
-        // rows of 64 clauses, the eight pieces exchanged by the column's low bits
+        // lanes that read two columns together meet 32 different banks
         const uint16_t *p = (const uint16_t *)a.x + row + c;
         uint32_t w[4] = {0, 0, 0, 0};
         if (c + 8 <= a.C && (uintptr_t)p % 16 == 0) {
@@ -180,8 +181,7 @@ __global__ void __launch_bounds__(256) k_q4_x(const Q4XArgs a) {
             for (int j = 0; j < 8; ++j)
                 if (c + j < a.C) w[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
         }
-        const int at = a.tiles ? ((in_seg >> 3) * a.cols + col) * 128 + ((o & 7) ^ (col & 7)) * 16
-                               : ((in_seg >> 2) * a.cols + col) * 64 + ((o & 3) ^ (col >> 1 & 3)) * 16;
+        const int at = a.tiles ? tile_at : ((in_seg >> 2) * a.cols + col) * 64 + ((o & 3) ^ (col >> 1 & 3)) * 16;
         *(uint4 *)(seg + at) =
             make_uint4(__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x5410),
                        __byte_perm(w[1], w[3], 0x7632));
@@ -198,6 +198,11 @@ __global__ void __launch_bounds__(256) k_q4_x(const Q4XArgs a) {
     if (MODE == Q4_BITS) {
         uint32_t w = c < a.C ? ((const uint32_t *)a.x)[row + (c >> 5)] >> (c & 31) & 255u : 0u;
         if (c < a.C && c + 8 > a.C) w &= (1u << (a.C - c)) - 1u;
+        if (a.tiles) {  // fp16 ones, in the order above
+            const auto ones = [&](int j) { return (w >> j & 1u) * 0x3C00u | (w >> (j + 4) & 1u) * 0x3C000000u; };
+            *(uint4 *)(seg + tile_at) = make_uint4(ones(0), ones(1), ones(2), ones(3));
+            return;
+        }
         const auto spread = [](uint32_t v) { return (v & 1u) | (v & 4u) << 6 | (v & 16u) << 12 | (v & 64u) << 18; };
         *(uint2 *)digits = make_uint2(spread(w), spread(w >> 1));
         start(0, __popc(w));
@@ -941,8 +946,9 @@ struct Q4Plan {
     bool tiles;                // k_q4_tiles
 };
 
-// A stage takes 1.4 to 1.8 us, a block 3 more to start and to end, 5 in a cluster.
-static void tiles_plan(Q4Plan &p, int64_t N, int64_t C, int64_t K) {
+// Blocks of k_q4_tiles, and the least cost: a stage takes 1.0 to 2.8 us by the
+// number of its groups, a block 5 more to start and to end, 7 in a cluster.
+static std::pair<Q4Plan, double> cut_tiles(Q4Plan p, int64_t N, int64_t C, int64_t K, int group) {
     p.tiles = true;
     p.samples = (int)cdiv(N, cdiv(N, (int64_t)64));
     p.cols = std::max(32, (p.samples + 15) / 16 * 16);
@@ -951,16 +957,18 @@ static void tiles_plan(Q4Plan &p, int64_t N, int64_t C, int64_t K) {
     p.stages = (int)cdiv(C, Q4_SEG);
     p.xs_block = (int64_t)p.cols * 512 * p.stages;
     p.smem = qt_stages(p.cols) * (QT_W_BYTES + (size_t)p.cols * 512) + QT_BARS;
+    const double stage = (group == 32 ? 2.8 : group == 64 ? 1.7 : 1.15) * (p.cols == 32 ? 0.84 : 1.0);
     const int64_t sms = sm_count(), tiles = cdiv(K, QT_ROWS) * p.z;
     double least = 0;
     for (int cl = 1; cl <= 16 && (cl == 1 || cl <= p.stages); cl *= 2) {
         const int64_t place = cl == 16 ? sms * 3 / 4 : cl == 8 ? sms * 6 / 7 : sms;
-        const double cost = (double)cdiv(tiles * cl, place) * ((double)cdiv(p.stages, cl) * 1.6 + (cl > 1 ? 5 : 3));
+        const double cost = (double)cdiv(tiles * cl, place) * ((double)cdiv(p.stages, cl) * stage + (cl > 1 ? 7 : 5));
         if (!p.cluster || cost < least * 0.97) {
             p.cluster = cl;
             least = cost;
         }
     }
+    return {p, least};
 }
 
 // Blocks of k_q4_votes of up to `most` samples, and the least cost.
@@ -1005,21 +1013,24 @@ static Q4Plan q4_plan_of(int64_t N, int64_t C, int64_t K, int x_type, int group)
     Q4Plan p = {};
     p.mode = x_type == YTM_BITS ? Q4_BITS : x_type == YTM_F32 || (N <= 2 && K >= 1024) ? Q4_DIGITS : x_type == YTM_F16 ? Q4_FP16 : Q4_BF16;
     p.parts = p.mode == Q4_DIGITS ? 4 : 1;
-    // Tiles cost 2 us more to set up and as much for 3 samples as for 16, so they
-    // are for many samples of many classes; scaling bounds them under groups of 32.
-    // 8192 x 16384, groups of 64: 16 samples 25 us against 28 in k_q4_votes, 24 31
-    // against 37, 64 38 against 76; groups of 32: 17 44 against 39, 32 44 against 55.
-    // 16384 x 512, groups of 64: 17 13.0 against 11.9, 32 13.3 against 14.9.
-    if (p.mode >= Q4_BF16 && N > (group == 32 ? 24 : 16) && K >= 512) {
-        tiles_plan(p, N, C, K);
-        return p;
-    }
     // digits: blocks of up to 8 samples, two an SM (21 samples of 8192 x 16384: 92 us
-    // against 112 with 16); else of up to 64 or 32, whichever costs less (bits, 64
-    // samples of 8192 x 16384: 54 us against 58, 256 of 65536 x 100: 48 against 37)
+    // against 112 with 16)
     if (p.mode == Q4_DIGITS) return cut(p, N, C, K, group, 8).first;
+    // else of up to 64 or 32, whichever costs less (bits, groups of 64: 64 samples of
+    // 8192 x 16384 54 us against 58, 256 of 65536 x 100 48 against 37)
     const auto wide = cut(p, N, C, K, group, 64), narrow = cut(p, N, C, K, group, 32);
-    return narrow.second < wide.second ? narrow.first : wide.first;
+    const auto best = narrow.second < wide.second ? narrow : wide;
+    // Tiles take as long for 3 samples as for 32 and suit many classes: 8192 x 16384,
+    // groups of 64, fp16: 16 samples 25 us against 28 in k_q4_votes, 24 31 against 37,
+    // 64 38 against 76; bits: 33 34 against 39, 64 38 against 54; groups of 32, fp16:
+    // 17 44 against 39, 32 44 against 55.  16384 x 512, fp16: 17 13.0 against 11.9.
+    if (K >= 512 && N > (p.mode == Q4_BITS ? group == 32 ? 48 : 32 : group == 32 ? 24 : 16)) {
+        // cut's costs are those of bits under groups of 64, without the start
+        const double more = (p.mode == Q4_BITS ? 1.0 : 1.35) * (group == 32 ? 1.27 : group == 64 ? 1.0 : 0.85);
+        const auto tiles = cut_tiles(p, N, C, K, group);
+        if (tiles.second < best.second * more + 7) return tiles.first;
+    }
+    return best.first;
 }
 
 // The thread's last plan again if the sizes are the same: the workspace's size
@@ -1126,8 +1137,8 @@ static ytm_status launch_q4(const Q4XArgs &xa, unsigned x_blocks, const Q4Args &
     k_q4_x<MODE><<<x_blocks, 256, 0, st>>>(xa);
     ytm_status rc = launch_check("q4 activations");
     if (rc) return rc;
-    if constexpr (MODE >= Q4_BF16)
-        if (p.tiles) return launch_tiles<MODE == Q4_FP16>(a, p, map, group, grid, st);
+    if constexpr (MODE != Q4_DIGITS)
+        if (p.tiles) return launch_tiles<MODE != Q4_BF16>(a, p, map, group, grid, st);
     switch (p.cols) {
         case 8: return launch_q4<MODE, 8>(a, p, map, group, grid, st);
         case 16: return launch_q4<MODE, 16>(a, p, map, group, grid, st);
