@@ -111,7 +111,10 @@ def test_votes(n, c, k, group, scale, out, x):
     (3, 64, 512, 64, "f32", "f32"), (3, 1, 513, 32, "f32", "f32"), (16, 256, 700, 32, "f16", "f32"), (17, 257, 1025, 128, "f32", "f16"),
     (33, 4000, 600, 64, "bf16", "f32"), (48, 2500, 2000, 32, "f16", "bf16"), (49, 1023, 999, 128, "f32", "f32"),
     (64, 2048, 512, 64, "f32", "f32"), (65, 700, 777, 32, "f32", "f32"), (150, 3001, 1500, 128, "bf16", "f32"),
-    (5, 20000, 4100, 64, "f16", "f32"), (64, 5000, 9000, 32, "f32", "f32")])
+    (5, 20000, 4100, 64, "f16", "f32"), (64, 5000, 9000, 32, "f32", "f32"), (33, 1, 70001, 64, "f32", "f32"),
+    (40, 300, 40000, 128, "f16", "bf16"), (64, 1300, 3001, 128, "bf16", "f32"), (20, 1500, 20011, 64, "f32", "f16"),
+    (130, 9000, 1500, 128, "f16", "f32"), (100, 20000, 700, 64, "f32", "f32"), (70, 1000, 30000, 32, "bf16", "f32"),
+    (64, 4097, 5000, 32, "f16", "f32"), (1000, 3000, 600, 64, "f32", "bf16")])
 def test_votes_of_many_classes_and_several_samples(n, c, k, group, scale, out, x):
     test_votes(n, c, k, group, scale, out, x)
 
@@ -130,6 +133,60 @@ def test_votes_strides_and_alignment(x):
         check_votes(y, v, q, scales, group, np.zeros(k), "f32", c)
     y = answers.q4_votes(xt, packed[5:20], scales[5:20], group, bias=dev(bias)[5:20], clauses=c)
     check_votes(y, xv, q[5:20], scales[5:20], group, bias[5:20], "f32", c)
+
+
+@pytest.mark.parametrize("x", ["bits", "f16", "bf16"])
+def test_votes_of_many_classes_strides_and_infinities(x):
+    """As above for 64 samples of many classes: rows off any boundary, memory
+    full of NaN behind a block's last sample, infinities that stay in their row."""
+    n, c, k, group = 64, 1301, 3001, 128
+    xt, xv, packed, q, scales, bias = votes_inputs(n, c, k, x, group, "f32")
+    wide = torch.full((n, xt.shape[1] + 5), 7, dtype=xt.dtype, device="cuda")
+    wide[:, 3:-2] = xt
+    for view, v in ((wide[:, 3:-2], xv), (xt[2:3].expand(n, -1), np.repeat(xv[2:3], n, 0)), (xt[:50], xv[:50])):
+        trash = torch.full((1 << 22,), float("nan"), device="cuda")
+        del trash
+        check_votes(answers.q4_votes(view, packed, scales, group, clauses=c), v, q, scales, group, np.zeros(k), "f32", c)
+    part = answers.q4_votes(xt, packed[8:2905], scales[8:2905], group, bias=dev(bias)[8:2905], clauses=c)
+    check_votes(part, xv, q[8:2905], scales[8:2905], group, bias[8:2905], "f32", c)
+    if x == "bits":
+        return
+    y = answers.q4_votes(xt, packed, scales, group)
+    xt[5, 77], xt[9, 1300] = float("inf"), float("nan")
+    z = answers.q4_votes(xt, packed, scales, group)
+    w = dev(q[:, 77])
+    assert (z[5][w > 0] == float("inf")).all() and (z[5][w < 0] == -float("inf")).all() and torch.isnan(z[5][w == 0]).all()
+    assert torch.isnan(z[9]).all()
+    others = [i for i in range(n) if i not in (5, 9)]
+    assert torch.equal(z[others], y[others])
+
+
+def test_votes_of_many_classes_captured_and_on_two_streams():
+    sets = []
+    for seed, x, n in ((0, "f16", 64), (1, "bits", 40), (2, "bf16", 130)):
+        xt, _, packed, _, scales, _ = votes_inputs(n, 1500, 5000, x, 64, "f32", seed=seed)
+        sets.append((xt, packed, scales, 64, None, 1500))
+    want = [answers.q4_votes(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(60):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((i % 3, answers.q4_votes(*sets[i % 3])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [answers.q4_votes(*s) for s in sets]
+    for _ in range(3):
+        for y in outs:
+            y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, w) for y, w in zip(outs, want))
+    sets[0][0].mul_(-1)  # a replay reads what is there then
+    graph.replay()
+    assert torch.equal(outs[0], -want[0])
 
 
 def test_votes_of_more_samples_than_one_launch_takes():

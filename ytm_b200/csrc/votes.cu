@@ -71,7 +71,8 @@ __global__ void k_q4_pack(const T *__restrict__ w, int64_t w_stride, int C, int 
 //   activations from three samples on (16384 x 32768, bf16: one sample 71 us against
 //   53 in digits, three 71 against 67, five 71 against 110; 8192 x 8192: 13.6
 //   against 12.2, 13.9 against 14.5, 14.2 against 19.9), and where few classes leave
-//   the weights' stream short (65536 x 100: 7.9 against 9.4).
+//   the weights' stream short (65536 x 100: 7.9 against 9.4).  Many samples of many
+//   classes have a kernel of their own, k_q4_tiles.
 //
 // A group's sum is scaled in fp32.  k_q4_x lays the activations out before, in
 // pieces of 256 clauses, so that a stage's are one piece of memory.
@@ -616,7 +617,8 @@ __global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS <= 32 ? 2 : 1
     q4_join(a, mine, rank, row0, log_rows, sample0, samples);
 }
 
-// ---- products of many 16-bit activations on the tensor cores' own memory
+// ---- products of many samples on the tensor cores' own memory: 16-bit
+// activations, and clause bits as fp16 ones (their group sums stay exact)
 //
 // A block takes 256 classes as two products of 128 by COLS.  Sixteen warps turn
 // words into 16-bit pairs as above, a thread a class, and store them into the
