@@ -1,6 +1,6 @@
 // answers_bind.cpp — the Python entry points of ytm_b200.answers: argument
 // checks, output tensors and the calls of libytm's C ABI.  They stand here and
-// not in Python because one sample's answer takes the GPU 3 us and an
+// not in Python because one sample's answer takes the GPU 2 us and an
 // interpreter's share of a call 10.
 #include <Python.h>
 
