@@ -19,7 +19,7 @@
 //
 // Measured with a bias: 262144 x 100 int32 51 us (2.1 TB/s; bound by some 20
 // instructions a class), with row masks 64; 2047 x 32001 bf16 118 us, with row
-// masks 147 (393 MB in two streams, 3.3 and 2.7 TB/s; bound by instructions and
+// masks 145 (393 MB in two streams, 3.3 and 2.7 TB/s; bound by instructions and
 // latency in both: the first reads the bias again for every row, 15 us of it).
 // One pass with a cluster a row, the exponentials kept, took 583 us: labels and
 // clusters waited for, with half of the clusters that would fill the SMs.
@@ -436,8 +436,9 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
     __shared__ double red_dt[LB_THREADS / 32];
     cudaGridDependencySynchronize();
     const int K = a.k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int id = (int)(blockIdx.y + blockIdx.z * gridDim.y);  // of the chunk
-    if (id >= chunks) return;
+    // the last rows first: the cache still holds their class sums
+    const int id = chunks - 1 - (int)(blockIdx.y + blockIdx.z * gridDim.y);  // of the chunk
+    if (id < 0) return;
     const int64_t n0 = id % period + (int64_t)(id / period) * chunk * period;  // the chunk's rows: n0 + i * period
     const int count = n0 < a.n ? (int)min((int64_t)chunk, (a.n - n0 + period - 1) / period) : 0;
     const float rt = loss_rt(a), c = loss_c(rt);
