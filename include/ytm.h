@@ -360,7 +360,8 @@ ytm_status ytm_match_counters(uint64_t *out, void *stream);
  * gradients.  No counterpart in the reference, whose predict is the argmax of
  * the class sums (src/cutm/multiclass.py:54-59).  They take plain arrays (no
  * ytm_config); rows are strided (strides in elements), the elements of a row
- * contiguous, and a stride of 0 repeats one row.  Indices and sizes are 64-bit
+ * contiguous, a stride of 0 repeats one row, and the stride beside a NULL
+ * pointer counts for nothing.  Indices and sizes are 64-bit
  * inside; more than 2^31 - 1 rows of `n` or 2^30 clauses or classes are refused
  * with YTM_ERR_UNSUPPORTED.  Calls keep nothing between them and may overlap on
  * different streams, each with its own workspace. */

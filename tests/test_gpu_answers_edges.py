@@ -1,0 +1,55 @@
+"""GPU tests of the answer operators at their edges: C callers' arguments,
+sums that cancel, infinities and large whole numbers, large batches.
+
+Tolerances count roundings: u = 2^-24 is half a step of fp32."""
+import ctypes as ct
+
+import numpy as np
+import pytest
+import torch
+
+from ytm_b200 import _lib, answers
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "i32": torch.int32}
+CODE = {"i32": _lib.YTM_I32, "f32": _lib.YTM_F32, "f16": _lib.YTM_F16, "bf16": _lib.YTM_BF16}
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def stream():
+    return ct.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+# ------------------------------------------------------- the C ABI's arguments
+
+@pytest.mark.parametrize("dt", ["i32", "bf16"])
+@pytest.mark.parametrize("k", [10, 100, 400, 1000, 5003])
+def test_strides_beside_null_pointers_count_for_nothing(k, dt):
+    n, lib = 5, _lib.load()
+    rng = np.random.default_rng(k)
+    cs = dev(rng.integers(-20, 21, (n, k)).astype(np.int32)).to(DT[dt])
+    y = dev(rng.integers(0, k, n))
+    choice, logprob, z = answers.answer(cs)
+    c2, l2, z2 = torch.empty_like(choice), torch.empty_like(logprob), torch.empty_like(z)
+    a = _lib.AnswerArgs(cs=cs.data_ptr(), cs_stride=k, n=n, k=k, cs_type=CODE[dt], bias_stride=k, allowed_stride=(k + 31) // 32,
+                        history_stride=9, temperature_all=1.0, repetition_all=1.0, choice=c2.data_ptr(), logprob=l2.data_ptr(),
+                        adjusted=z2.data_ptr())
+    _lib.check(lib.ytm_answer(ct.byref(a), stream()))
+    assert torch.equal(c2, choice) and torch.equal(l2, logprob) and torch.equal(z2, z)
+    loss, dcs, _, dtem = answers.class_loss(cs, y)
+    loss2, dtem2 = torch.empty_like(loss), torch.empty_like(dtem)
+    dcs2 = None if dcs is None else torch.empty_like(dcs)
+    ws = torch.empty(max(16, lib.ytm_class_loss_workspace_bytes(n, k, CODE[dt], k)), dtype=torch.uint8, device="cuda")
+    a = _lib.LossArgs(cs=cs.data_ptr(), cs_stride=k, n=n, k=k, cs_type=CODE[dt], allowed_stride=(k + 31) // 32, target=y.data_ptr(),
+                      target_64=1, temperature_all=1.0, loss=loss2.data_ptr(), dcs=None if dcs is None else dcs2.data_ptr(),
+                      dtemperature=dtem2.data_ptr())
+    _lib.check(lib.ytm_class_loss(ct.byref(a), ws.data_ptr(), stream()))
+    assert torch.equal(loss2, loss) and torch.equal(dtem2, dtem) and (dcs is None or torch.equal(dcs2, dcs))

@@ -364,7 +364,7 @@ extern "C" {
 
 ytm_status ytm_answer(const ytm_answer_args *args, void *stream) {
     if (!args) return fail(YTM_ERR_ARG, "args is NULL");
-    const ytm_answer_args &a = *args;
+    ytm_answer_args a = *args;
     if (a.n < 0 || a.k <= 0) return fail(YTM_ERR_ARG, "answer: needs n >= 0 rows of k >= 1 classes");
     if (a.n > INT_MAX || a.k > (1 << 30)) return fail(YTM_ERR_UNSUPPORTED, "answer: more than 2^31 - 1 rows or 2^30 classes");
     if (!is_sum_type(a.cs_type)) return fail(YTM_ERR_ARG, "answer: class sums must be int32, fp32, fp16 or bf16");
@@ -372,6 +372,9 @@ ytm_status ytm_answer(const ytm_answer_args *args, void *stream) {
         return fail(YTM_ERR_ARG, "answer: negative stride or length");
     if (a.n == 0) return YTM_OK;
     if (!a.cs || (a.lengths && !a.history)) return fail(YTM_ERR_ARG, "null pointer");
+    // the kernels take a stride to say that there is something to read row by row
+    if (!a.bias) a.bias_stride = 0;
+    if (!a.allowed) a.allowed_stride = 0;
     cudaStream_t st = as_stream(stream);
     switch (a.cs_type) {
         case YTM_I32: return launch_answer<int32_t>(a, st);

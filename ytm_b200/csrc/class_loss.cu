@@ -746,12 +746,13 @@ uint64_t ytm_class_loss_workspace_bytes(int64_t n, int32_t k, int32_t cs_type, i
 
 ytm_status ytm_class_loss(const ytm_loss_args *args, void *workspace, void *stream) {
     if (!args) return fail(YTM_ERR_ARG, "args is NULL");
-    const ytm_loss_args &a = *args;
+    ytm_loss_args a = *args;
     if (a.n < 0 || a.k <= 0) return fail(YTM_ERR_ARG, "class loss: needs n >= 0 rows of k >= 1 classes");
     if (a.n > INT_MAX || a.k > (1 << 30)) return fail(YTM_ERR_UNSUPPORTED, "class loss: more than 2^31 - 1 rows or 2^30 classes");
     if (!is_sum_type(a.cs_type)) return fail(YTM_ERR_ARG, "class loss: class sums must be int32, fp32, fp16 or bf16");
     if (a.cs_type == YTM_I32 && a.dcs) return fail(YTM_ERR_ARG, "class loss: int32 class sums have no gradient");
     if (a.cs_stride < 0 || a.allowed_stride < 0) return fail(YTM_ERR_ARG, "class loss: negative stride");
+    if (!a.allowed) a.allowed_stride = 0;  // the kernels take a stride to say that there is something to read row by row
     cudaStream_t st = as_stream(stream);
     ytm_status rc;
     if (a.n == 0) {
