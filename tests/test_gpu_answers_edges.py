@@ -53,3 +53,31 @@ def test_strides_beside_null_pointers_count_for_nothing(k, dt):
                       dtemperature=dtem2.data_ptr())
     _lib.check(lib.ytm_class_loss(ct.byref(a), ws.data_ptr(), stream()))
     assert torch.equal(loss2, loss) and torch.equal(dtem2, dtem) and (dcs is None or torch.equal(dcs2, dcs))
+
+
+# ------------------------------------------------------------ sums that cancel
+
+@pytest.mark.parametrize("dt", ["i32", "f32", "bf16"])
+@pytest.mark.parametrize("n,k", [(4_000_000, 10), (1_000_000, 100), (300_000, 300), (100_000, 1000)])
+def test_bias_gradient_of_many_certain_rows(n, k, dt):
+    """Rows that are all right with probability 1 - (k - 1) e^-9: a label's
+    gradient is the small rest of its weight.  All terms of a class have one
+    sign, so every rounding counts relative to the sum.  A term: the exponent 13
+    off by 2 u of itself (18 u of the exponential), ex2 by 2 steps, the row's sum
+    by its chain, the quotients by 6 u, a long row's difference from its weight
+    by u of 1; the sum: at most 256 rows one after another, 64 teams of a block."""
+    cs = torch.zeros((1, k), dtype=DT[dt], device="cuda")
+    cs[0, 3] = 9
+    y = torch.full((n,), 3, device="cuda")
+    loss, _, dbias, _ = answers.class_loss(cs.expand(n, k), y, bias=torch.zeros(k, device="cuda"))
+    e = np.exp(-9.0)
+    p = np.full(k, e / (1 + (k - 1) * e))
+    p[3] = -(k - 1) * p[0]
+    chain = k / 32 + 64
+    tol = (22 + chain + 6 + 256 + 64 + 4) * U * np.abs(n * p)
+    if k > 512:
+        tol[3] += n * 2 * U
+    err = np.abs(f64(dbias) - n * p)
+    assert (err <= tol).all(), (err / tol).max()
+    want = np.log1p((k - 1) * e)
+    assert (loss - want).abs().max().item() <= (2 * chain + 64) * U

@@ -78,16 +78,17 @@ struct LossPart {
 
 // -------------------------------------------------- rows of few classes
 // TPR threads hold a row, E classes each (e TPR + lane), in pairs for the paired
-// arithmetic.  The label's class is not looked for among them: the lane that
-// holds it adds the row's weight to its own sum in shared memory and stores the
-// class's gradient once more.
+// arithmetic.  The label's class is closed there and taken apart, by every thread
+// of the row from the label's own load: its gradient is -(w / t) times the others'
+// share, without the cancellation of p_y - 1.  The lane that holds the class adds
+// that to its own sum in shared memory and stores the class's gradient once more.
 
 constexpr int LS_THREADS = 256;
 
 template <typename T, int TPR, int E>
 __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_loss_small(const ytm_loss_args a, const LossPart part) {
     constexpr int ROWS = LS_THREADS / TPR, SLOTS = TPR * E;
-    extern __shared__ float red[];  // [ROWS][SLOTS]: the labels' weights, at the end dbias of the teams
+    extern __shared__ float red[];  // [ROWS][SLOTS]: sums of the labels' gradients, at the end dbias of the teams
     __shared__ double red_dt[LS_THREADS / 32];
     const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR, K = a.k;
     float *const mine = red + team * SLOTS + lane;
@@ -155,13 +156,17 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
         }
         const bool live = n0 + team < a.n;
         const int64_t n = clamped(n0 + team);
-        float z[E], m = -INFINITY;
+        const int y = row.label.y;
+        const bool own = y >= 0 && y % TPR == lane;
+        const uint32_t open = own ? row.open & ~(1u << (y / TPR)) : row.open;  // without the label's class
+        const float uy = loss_u(to_f32(row.vy), row.by);
+        float z[E], m = row.label.open ? uy : -INFINITY;
 #pragma unroll
         for (int q = 0; q < E / 2; ++q) {
-            float x, y;
-            split(add2(pair(to_f32(row.v[2 * q]), to_f32(row.v[2 * q + 1])), b[q]), x, y);
-            z[2 * q] = row.open & (1u << (2 * q)) ? x : -INFINITY;
-            z[2 * q + 1] = row.open & (2u << (2 * q)) ? y : -INFINITY;
+            float x0, x1;
+            split(add2(pair(to_f32(row.v[2 * q]), to_f32(row.v[2 * q + 1])), b[q]), x0, x1);
+            z[2 * q] = open & (1u << (2 * q)) ? x0 : -INFINITY;
+            z[2 * q + 1] = open & (2u << (2 * q)) ? x1 : -INFINITY;
             m = fmaxf(m, fmaxf(z[2 * q], z[2 * q + 1]));
         }
 #pragma unroll
@@ -170,13 +175,13 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
         const F2 m2 = pair(-m, -m);
 #pragma unroll
         for (int q = 0; q < E / 2; ++q) {
-            float x, y;
-            split(mul2(add2(pair(z[2 * q], z[2 * q + 1]), m2), c2), x, y);
-            z[2 * q] = ex2(x);
-            z[2 * q + 1] = ex2(y);
+            float x0, x1;
+            split(mul2(add2(pair(z[2 * q], z[2 * q + 1]), m2), c2), x0, x1);
+            z[2 * q] = ex2(x0);
+            z[2 * q + 1] = ex2(x1);
             const F2 e2 = pair(z[2 * q], z[2 * q + 1]);
             s2 = add2(s2, e2);
-            h2 = fma2(e2, pair(fmaxf(x, -1024.f), fmaxf(y, -1024.f)), h2);  // 0 * -inf counts for nothing
+            h2 = fma2(e2, pair(fmaxf(x0, -1024.f), fmaxf(x1, -1024.f)), h2);  // 0 * -inf counts for nothing
         }
         float s, h, t;
         split(s2, s, t);
@@ -189,7 +194,10 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
             h += __shfl_xor_sync(0xFFFFFFFFu, h, d);
         }
         const bool use = live && row.label.open;
-        const float wt = row.label.w * rt, f = wt / s, uy = loss_u(to_f32(row.vy), row.by);
+        const float xy = loss_x(uy, m, c), ey = ex2(xy), others = s;
+        s += ey;
+        h = fmaf(ey, fmaxf(xy, -1024.f), h);
+        const float f = row.label.w * rt / s, dy = -others * f;
         if (use) {
             const F2 f2 = pair(f, f);
 #pragma unroll
@@ -210,15 +218,15 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
                     if (e * TPR + lane < K) out[e * TPR] = from_f32<T>(z[e]);
             }
         }
-        if (use && row.label.y % TPR == lane) {
-            mine[row.label.y - lane] += wt;
+        if (use && own) {
+            mine[y - lane] += dy;
             if constexpr (!std::is_integral<T>::value) {
-                if (a.dcs) ((T *)a.dcs)[n * (int64_t)K + row.label.y] = from_f32<T>(ex2(loss_x(uy, m, c)) * f - wt);
+                if (a.dcs) ((T *)a.dcs)[n * (int64_t)K + y] = from_f32<T>(dy);
             }
         }
         if (lane == 0 && live) {
             const float w = row.label.w, gap = uy - m;
-            a.loss[n] = use ? w * (logf(s) - gap * rt) : row.label.y >= 0 ? w * INFINITY : 0.f;
+            a.loss[n] = use ? w * (logf(s) - gap * rt) : y >= 0 ? w * INFINITY : 0.f;
             if (use) dt += (double)w * ((double)(h / s) - (double)gap * (double)c);
         }
     }
@@ -227,8 +235,8 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
     for (int q = 0; q < E / 2; ++q) {
         float x, y;
         split(acc[q], x, y);
-        mine[2 * q * TPR] = x - mine[2 * q * TPR];
-        mine[(2 * q + 1) * TPR] = y - mine[(2 * q + 1) * TPR];
+        mine[2 * q * TPR] += x;
+        mine[(2 * q + 1) * TPR] += y;
     }
     for (int d = 16; d; d >>= 1) dt += __shfl_xor_sync(0xFFFFFFFFu, dt, d);
     if ((threadIdx.x & 31) == 0) red_dt[threadIdx.x >> 5] = dt;
