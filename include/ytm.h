@@ -436,8 +436,8 @@ ytm_status ytm_answer(const ytm_answer_args *args, void *stream);
 /* Cross entropy with z as above (no penalties): loss[n] = weight[n] *
  * (log sum exp z - z[target[n]]), and with d = weight (softmax z - onehot) the
  * gradients dcs = d / temperature, dbias = sum_n d / temperature and
- * dtemperature = -sum d z / temperature, summed in a fixed order.  A NaN among
- * a row's allowed class sums makes its loss and its gradients NaN.  Rows whose
+ * dtemperature = -sum d z / temperature, summed in a fixed order.  A NaN or
+ * +inf among a row's allowed class sums makes its loss and its gradients NaN.  Rows whose
  * target lies outside [0, k) or whose weight is 0 count for nothing; a target
  * that the mask forbids gives a loss of weight * inf and no gradient. */
 typedef struct ytm_loss_args {

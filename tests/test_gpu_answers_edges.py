@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+from tests.test_gpu_answers import check_loss
 from ytm_b200 import _lib, answers
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +82,36 @@ def test_bias_gradient_of_many_certain_rows(n, k, dt):
     assert (err <= tol).all(), (err / tol).max()
     want = np.log1p((k - 1) * e)
     assert (loss - want).abs().max().item() <= (2 * chain + 64) * U
+
+
+# --------------------------------------------------- infinities and large sums
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shift", [0, 1, 3])
+@pytest.mark.parametrize("k", [40, 500, 1025, 5003, 40001])
+def test_class_loss_of_unusual_values_wherever_they_lie(k, shift, dt):
+    """A NaN or +inf among the allowed makes a row's loss and gradients NaN, -inf
+    is a probability of 0, and a masked value counts for nothing, at a row's
+    first, middle and last class and at any alignment of its memory."""
+    rng = np.random.default_rng(k + shift)
+    cases = [(v, at, masked) for v in (np.nan, np.inf, -np.inf) for at in (0, 5, k // 2, k - 1) for masked in (False, True)]
+    n = len(cases)
+    wide = torch.zeros((n, k + 5), dtype=DT[dt], device="cuda")
+    cs = wide[:, shift:shift + k]
+    cs.copy_(dev(rng.normal(size=(n, k)).astype(np.float32)))
+    open_ = np.ones((n, k), bool)
+    y = dev(np.full(n, 1))
+    clean = open_.copy()
+    for i, (v, at, masked) in enumerate(cases):
+        open_[i, at] = not masked
+        clean[i, at] = False
+    want = answers.class_loss(cs, y, allowed=answers.pack_allowed(clean).cuda())
+    check_loss(want, cs, y.cpu().numpy(), {"allowed": clean, "temperature": np.float32(1.0)})
+    for i, (v, at, masked) in enumerate(cases):
+        cs[i, at] = v
+    loss, dcs, _, _ = answers.class_loss(cs, y, allowed=answers.pack_allowed(open_).cuda())
+    for i, (v, at, masked) in enumerate(cases):
+        if masked or v == -np.inf:
+            assert torch.equal(loss[i], want[0][i]) and torch.equal(dcs[i], want[1][i]), cases[i]
+        else:
+            assert torch.isnan(loss[i]) and torch.isnan(dcs[i]).all(), cases[i]

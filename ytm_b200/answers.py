@@ -118,6 +118,6 @@ def class_loss(cs: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None
     of 0 count for nothing.  A target that its mask forbids gives weight * inf
     and no gradient.  bias: float32 [k]; allowed as for `answer`; temperature:
     a positive number or float32 [1], whose value is not checked; weight:
-    float32 [n].  A NaN among a row's allowed class sums makes its loss and
-    gradients NaN."""
+    float32 [n].  A NaN or +inf among a row's allowed class sums makes its loss
+    and gradients NaN."""
     return _bind.class_loss(cs, target, bias, allowed, temperature, weight)

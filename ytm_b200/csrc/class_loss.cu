@@ -402,8 +402,8 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
         const int k = (int)threadIdx.x < head ? (int)threadIdx.x : tail + ((int)threadIdx.x - head);
         if (k < K && is_allowed(allowed, k)) {
             const float u = loss_u(to_f32(row.row[k]), a.bias ? a.bias[k] : 0.f);
-            // u itself if it is no number, so that it reaches the sum
-            st = merge(st, {u, u == u ? (u == -INFINITY ? 0.f : 1.f) : u, 0.f}, c);
+            // as in the streams: e of -inf is 0, and NaN that of NaN or +inf, which u - u is
+            st = merge(st, {u, u == -INFINITY ? 0.f : 1.f + (u - u), 0.f}, c);
         }
     }
 #pragma unroll
