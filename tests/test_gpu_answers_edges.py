@@ -115,3 +115,67 @@ def test_class_loss_of_unusual_values_wherever_they_lie(k, shift, dt):
             assert torch.equal(loss[i], want[0][i]) and torch.equal(dcs[i], want[1][i]), cases[i]
         else:
             assert torch.isnan(loss[i]) and torch.isnan(dcs[i]).all(), cases[i]
+
+
+def check_whole_loss(cs, y, mask, bias, t, far=None):
+    """The loss of int32 sums (64 bits in `cs`) against 64 bits.  A row's
+    gradients and, its gradients' sum being 0, the temperature's do not change
+    when a number is taken from all of the row; less their largest, the sums
+    are as near as they lie, which is what the bounds of check_loss count."""
+    kw = {"temperature": np.float32(t)}
+    kt = {"temperature": float(t)}
+    if mask is not None:
+        kw["allowed"], kt["allowed"] = mask, answers.pack_allowed(mask).cuda()
+    if bias is not None:
+        kw["bias"], kt["bias"] = bias, dev(bias)
+    got = answers.class_loss(dev(cs.astype(np.int32)), dev(y), **kt)
+    open_ = np.ones(cs.shape, bool) if mask is None else np.broadcast_to(mask, cs.shape)
+    if far is not None:  # classes whose probability is 0 in fp32
+        open_ = open_ & ~far
+        kw["allowed"] = open_
+    top = np.where(open_, cs, np.iinfo(np.int64).min).max(1, keepdims=True)
+    # A sum v below 2^24 is not moved: with a bias, fp32 rounds v + b by up to u of
+    # |v + b|, which check_loss counts where v itself is given to it.
+    if bias is not None:
+        top[((np.abs(cs) < 2 ** 24) & open_).any(1)] = 0
+    check_loss(got, torch.from_numpy(np.where(open_, cs - top, 0)), y, kw)
+
+
+BASES = [0, 12345, 2 ** 24, -2 ** 24 - 30, 2 ** 24 - 7, -2 ** 24 - 1, 2 ** 30 + 7, 2 ** 31 - 61, -2 ** 31]
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("mask", [None, "all", "row"])
+@pytest.mark.parametrize("k", [3, 10, 100, 300, 1000, 5003])
+def test_class_loss_of_large_whole_sums(k, mask, bias):
+    """Whole numbers above 2^24 keep their differences."""
+    rng = np.random.default_rng(k)
+    n = 4 * len(BASES)
+    base = np.array(BASES)[np.arange(n) % len(BASES)][:, None]
+    y = rng.integers(0, k, n)
+    a = None
+    if mask:
+        a = rng.random((n if mask == "row" else 1, k)) < 0.7
+        a[np.arange(n) if mask == "row" else 0, y] = True
+    b = rng.normal(size=k).astype(np.float32) if bias else None
+    cs = base + rng.integers(0, 61, (n, k))
+    check_whole_loss(cs, y, a, b, 1.0)
+    check_whole_loss(cs, y, a, b, 15.5)
+    check_whole_loss(rng.integers(-2 ** 26, 2 ** 26, (n, k)), y, a, b, 2.0 ** 20)
+    check_whole_loss(rng.integers(-2 ** 31, 2 ** 31, (n, k)), y, a, b, 2.0 ** 29)
+    # some classes far below, beyond an int32 difference for the highest rows
+    far = rng.random((n, k)) < 0.4
+    far[np.arange(n), y] = False
+    rows = (base[:, 0] > 0)
+    cs = np.where(far, rng.integers(-2 ** 31, -2 ** 30, (n, k)), cs)
+    check_whole_loss(cs[rows], y[rows], a[rows] if mask == "row" else a, b, 3.0, far[rows])
+
+
+def test_class_loss_tells_neighbouring_whole_sums_apart():
+    for k in (5, 700):
+        cs = np.zeros((2, k), np.int32)
+        cs[:, 0], cs[:, 1], cs[:, 2:] = 16777217, 16777216, -2 ** 31
+        loss, _, db, _ = answers.class_loss(dev(cs), dev(np.array([0, 1])), bias=torch.zeros(k, device="cuda"))
+        q = 1 / (1 + np.exp(-1.0))
+        np.testing.assert_allclose(f64(loss), [-np.log(q), -np.log(1 - q)], rtol=16 * U)
+        np.testing.assert_allclose(f64(db)[:2], [2 * q - 1, 1 - 2 * q], rtol=32 * U)

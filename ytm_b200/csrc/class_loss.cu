@@ -10,6 +10,11 @@
 // factor comes after the difference: a row of the type's lowest value, whose
 // product with c has left the type, keeps its u - m = 0.
 //
+// fp32 rounds whole numbers above 2^24.  Where a row's largest u reaches 2^23, they
+// are taken less a whole number r near it, in 64 bits, so that their differences
+// stay: that changes neither the loss nor a gradient.  r is 0 for other rows, whose
+// rounded classes lie at least 2^23 below and so are off by 2^-23 of that at most.
+//
 // Rows of up to 512 classes stay in the registers of 4 to 32 threads between
 // the sum and the gradient (k_loss_small).  Longer rows take two streams over
 // the class sums, which need no barrier: k_loss_stat for (m, s, h), then
@@ -41,6 +46,16 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));  // within 2 steps, 2^0 = 1 exactly
     return y;
 }
+
+constexpr float WHOLE = 8388608.f;  // 2^23
+
+// Whether whole numbers with the largest u of m are to be taken less an r.
+__device__ __forceinline__ bool large_whole(float m) { return fabsf(m) >= WHOLE && m != -INFINITY; }
+
+// A class sum less the row's r.
+template <typename T>
+__device__ __forceinline__ float class_sum(T v, int) { return to_f32(v); }
+__device__ __forceinline__ float class_sum(int32_t v, int r) { return r ? (float)((int64_t)v - r) : (float)v; }
 
 // u and x, the same operations for every use of a class's, so that the largest
 // class's x is 0 exactly.
@@ -144,6 +159,7 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
         return r;
     };
     double dt = 0.0;
+    [[maybe_unused]] float top = 0.f;  // the largest |m|
     const int64_t step = (int64_t)gridDim.x * ROWS;
     int64_t n0 = (int64_t)blockIdx.x * ROWS;
     LossLabel label1 = loss_label(a, clamped(n0 + step + team));
@@ -156,11 +172,12 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
         }
         const bool live = n0 + team < a.n;
         const int64_t n = clamped(n0 + team);
-        const int y = row.label.y;
-        const bool own = y >= 0 && y % TPR == lane;
-        const uint32_t open = own ? row.open & ~(1u << (y / TPR)) : row.open;  // without the label's class
+        // (of rows without a label, or with a closed one, nothing is used)
+        const uint32_t y = (uint32_t)row.label.y;
+        const bool own = y % TPR == lane;
+        const uint32_t open = own ? row.open & ~(1u << (y / TPR % 32)) : row.open;  // without the label's class
         const float uy = loss_u(to_f32(row.vy), row.by);
-        float z[E], m = row.label.open ? uy : -INFINITY;
+        float z[E], m = uy;
 #pragma unroll
         for (int q = 0; q < E / 2; ++q) {
             float x0, x1;
@@ -194,10 +211,10 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
             h += __shfl_xor_sync(0xFFFFFFFFu, h, d);
         }
         const bool use = live && row.label.open;
+        if constexpr (std::is_integral<T>::value) top = fmaxf(top, use ? fabsf(m) : 0.f);
         const float xy = loss_x(uy, m, c), ey = ex2(xy), others = s;
         s += ey;
-        h = fmaf(ey, fmaxf(xy, -1024.f), h);
-        const float f = row.label.w * rt / s, dy = -others * f;
+        const float f = row.label.w * rt / s;
         if (use) {
             const F2 f2 = pair(f, f);
 #pragma unroll
@@ -219,15 +236,68 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
             }
         }
         if (use && own) {
-            mine[y - lane] += dy;
+            const float dy = -others * f;
+            mine[(int)y - lane] += dy;
             if constexpr (!std::is_integral<T>::value) {
                 if (a.dcs) ((T *)a.dcs)[n * (int64_t)K + y] = from_f32<T>(dy);
             }
         }
         if (lane == 0 && live) {
             const float w = row.label.w, gap = uy - m;
-            a.loss[n] = use ? w * (logf(s) - gap * rt) : y >= 0 ? w * INFINITY : 0.f;
+            a.loss[n] = use ? w * (logf(s) - gap * rt) : row.label.y >= 0 ? w * INFINITY : 0.f;
+            h = fmaf(ey, fmaxf(xy, -1024.f), h);
             if (use) dt += (double)w * ((double)(h / s) - (double)gap * (double)c);
+        }
+    }
+    if constexpr (std::is_integral<T>::value) {
+        // Large whole numbers were among the block's rows: all of them once more, from
+        // memory and class by class, as such rows are rare.
+        if (__syncthreads_or(large_whole(top))) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) mine[e * TPR] = 0.f;
+#pragma unroll
+            for (int q = 0; q < E / 2; ++q) acc[q] = pair(0.f, 0.f);
+            dt = 0.0;
+            for (n0 = (int64_t)blockIdx.x * ROWS; n0 < a.n; n0 += step) {
+                const int64_t n = clamped(n0 + team);
+                const LossLabel label = loss_label(a, n);
+                const T *cs = (const T *)a.cs + n * a.cs_stride;
+                const uint32_t *allowed = a.allowed ? a.allowed + n * a.allowed_stride : nullptr;
+                const int y = label.y, last = n0 + team < a.n && label.open ? K : 0;  // 0: the row has its loss and no gradient
+                const auto each = [&](auto f) {
+                    for (int k = lane; k < last; k += TPR)
+                        if (is_allowed(allowed, k)) f(k);
+                };
+                const auto over_team = [&](auto v, auto join) {
+#pragma unroll
+                    for (int d = TPR / 2; d; d >>= 1) v = join(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+                    return v;
+                };
+                const auto sum = [](float p, float q) { return p + q; };
+                int r = INT_MIN;
+                each([&](int k) { r = max(r, cs[k]); });
+                r = over_team(r, [](int p, int q) { return max(p, q); });
+                const auto u = [&](int k) { return loss_u(class_sum(cs[k], r), a.bias ? a.bias[k] : 0.f); };
+                float m = -INFINITY, s = 0.f, h = 0.f;
+                each([&](int k) { m = fmaxf(m, u(k)); });
+                m = over_team(m, [](float p, float q) { return fmaxf(p, q); });
+                each([&](int k) {
+                    const float x = loss_x(u(k), m, c), e = ex2(x);
+                    if (k != y) s += e, h = fmaf(e, fmaxf(x, -1024.f), h);
+                });
+                s = over_team(s, sum);
+                h = over_team(h, sum);
+                if (!last) continue;
+                const float uy = u(y), xy = loss_x(uy, m, c), ey = ex2(xy), others = s;
+                s += ey;
+                h = fmaf(ey, fmaxf(xy, -1024.f), h);
+                const float f = label.w * rt / s;
+                each([&](int k) { mine[k - lane] += k == y ? -others * f : ex2(loss_x(u(k), m, c)) * f; });
+                if (lane == 0) {
+                    a.loss[n] = label.w * (logf(s) - (uy - m) * rt);
+                    dt += (double)label.w * ((double)(h / s) - (double)(uy - m) * (double)c);
+                }
+            }
         }
     }
     // the block's sums, teams in order
@@ -257,11 +327,46 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
 
 // -------------------------------------------------- rows of many classes
 
+// m: the largest u, less r.
 struct LossStat {
     float m, s, h;
+    int r;
 };
 
-__device__ __forceinline__ LossStat merge(const LossStat &a, const LossStat &b, float c) {
+// The largest u, less another r: exact where that is near.
+__device__ __forceinline__ float largest_less(const LossStat &a, int r) {
+    return (float)((double)a.m + (double)((int64_t)a.r - r));
+}
+
+// r next to the largest u (unless that is no number, or far from any class sum).
+__device__ __forceinline__ void bring_near(LossStat &a) {
+    if (!(fabsf(a.m) < 2.f * WHOLE)) return;
+    const int64_t r = (int64_t)a.r + __float2int_rn(a.m);
+    if (r != (int)r) return;
+    a.m = largest_less(a, (int)r);
+    a.r = (int)r;
+}
+
+template <typename T>
+__device__ __forceinline__ LossStat merge(LossStat a, LossStat b, float c) {
+    if constexpr (std::is_integral<T>::value) {
+        if (a.r != b.r) {
+            if (a.m == -INFINITY) {
+                a.r = b.r;
+            } else if (b.m == -INFINITY) {
+                b.r = a.r;
+            } else {
+                bring_near(a);
+                bring_near(b);
+                const int r = max(a.r, b.r);
+                a.m = largest_less(a, r);
+                b.m = largest_less(b, r);
+                a.r = r;
+            }
+        }
+    } else {
+        a.r = 0;
+    }
     const float m = fmaxf(a.m, b.m);
     // a.m == m: the factor is 1 also where both are infinite
     const float da = a.m == m ? 0.f : loss_x(a.m, m, c), db = b.m == m ? 0.f : loss_x(b.m, m, c);
@@ -270,7 +375,15 @@ __device__ __forceinline__ LossStat merge(const LossStat &a, const LossStat &b, 
     // exchange end with the same bits
     return {m, __fadd_rn(__fmul_rn(fa, a.s), __fmul_rn(fb, b.s)),
             __fadd_rn(__fmul_rn(fa, fmaf(a.s, fmaxf(da, -1024.f), a.h)),
-                      __fmul_rn(fb, fmaf(b.s, fmaxf(db, -1024.f), b.h)))};
+                      __fmul_rn(fb, fmaf(b.s, fmaxf(db, -1024.f), b.h))), a.r};
+}
+
+// merge with the lane d away.
+template <typename T>
+__device__ __forceinline__ LossStat merge_lane(const LossStat &a, int d, float c) {
+    LossStat b = {__shfl_xor_sync(0xFFFFFFFFu, a.m, d), __shfl_xor_sync(0xFFFFFFFFu, a.s, d), __shfl_xor_sync(0xFFFFFFFFu, a.h, d), 0};
+    if constexpr (std::is_integral<T>::value) b.r = __shfl_xor_sync(0xFFFFFFFFu, a.r, d);
+    return merge<T>(a, b, c);
 }
 
 constexpr int LB_THREADS = 256;
@@ -327,6 +440,28 @@ __device__ __forceinline__ void load_bias(const float *bias, int k, F2 (&b)[V / 
     }
 }
 
+// A thread's round (vectors i0, i0 + LB_THREADS, ... below `to`) of large whole
+// numbers, from memory and class by class, as such rows are rare.
+template <int NV>
+__device__ __noinline__ LossStat large_round(const int *row, int off, const uint32_t *allowed, const float *bias, int i0, int to,
+                                             LossStat st, float c) {
+    const auto each = [&](auto f) {
+        for (int i = i0; i < to && i < i0 + NV * LB_THREADS; i += LB_THREADS)
+            for (int k = i * 4 - off; k < i * 4 - off + 4; ++k)
+                if (is_allowed(allowed, k)) f(k);
+    };
+    LossStat now = {-INFINITY, 0.f, 0.f, INT_MIN};
+    each([&](int k) { now.r = max(now.r, row[k]); });
+    const auto u = [&](int k) { return loss_u(class_sum(row[k], now.r), bias ? bias[k] : 0.f); };
+    each([&](int k) { now.m = fmaxf(now.m, u(k)); });
+    each([&](int k) {
+        const float x = now.m == -INFINITY ? u(k) : loss_x(u(k), now.m, c), e = ex2(x);
+        now.s += e;
+        now.h = fmaf(e, fmaxf(x, -1024.f), now.h);
+    });
+    return merge<int>(st, now, c);
+}
+
 // (m, s, h) of `rounds` rounds of NV * LB_THREADS vectors of one row: block
 // (part, row).
 template <typename T, int NV>
@@ -340,7 +475,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
     const F2 c2 = pair(c, c);
     const RowVecs<T> row(a.cs, n, a.cs_stride);
     const uint32_t *allowed = a.allowed ? a.allowed + n * a.allowed_stride : nullptr;
-    LossStat st = {-INFINITY, 0.f, 0.f};
+    LossStat st = {-INFINITY, 0.f, 0.f, 0};
     const int first = row.first(), below = row.off & 3, end = row.end(K, below);  // the bias is read up to the next boundary
     const auto stream = [&](auto r) {
         constexpr int R = decltype(r)::value;
@@ -369,6 +504,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
                     z[j][2 * q + 1] = open[j] & (2u << (2 * q)) ? y : -INFINITY;
                     m = fmaxf(m, fmaxf(z[j][2 * q], z[j][2 * q + 1]));
                 }
+            [[maybe_unused]] const LossStat before = st;
             const float base = m == -INFINITY ? 0.f : -m;  // nothing yet: every e is 0
             const float d = st.m == m ? 0.f : loss_x(st.m, m, c), f = ex2(d);
             F2 s = pair(f * st.s, 0.f), h = pair(f * fmaf(st.s, fmaxf(d, -1024.f), st.h), 0.f);
@@ -389,6 +525,8 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
             st.s = x + y;
             split(h, x, y);
             st.h = x + y;
+            if constexpr (std::is_integral<T>::value)
+                if (large_whole(m) || before.r) st = large_round<NV>((const int *)row.row, row.off, allowed, a.bias, i0, to, before, c);
         }
     };
     switch (below) {  // where the bias lies against the vectors: the same for the block
@@ -401,23 +539,21 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
         const int head = first * V - (first ? row.off : 0), tail = end * V - row.off;
         const int k = (int)threadIdx.x < head ? (int)threadIdx.x : tail + ((int)threadIdx.x - head);
         if (k < K && is_allowed(allowed, k)) {
-            const float u = loss_u(to_f32(row.row[k]), a.bias ? a.bias[k] : 0.f);
+            int r = 0;
+            if constexpr (std::is_integral<T>::value) r = large_whole(to_f32(row.row[k])) ? (int)row.row[k] : 0;
+            const float u = loss_u(class_sum(row.row[k], r), a.bias ? a.bias[k] : 0.f);
             // as in the streams: e of -inf is 0, and NaN that of NaN or +inf, which u - u is
-            st = merge(st, {u, u == -INFINITY ? 0.f : 1.f + (u - u), 0.f}, c);
+            st = merge<T>(st, {u, u == -INFINITY ? 0.f : 1.f + (u - u), 0.f, r}, c);
         }
     }
 #pragma unroll
-    for (int d = 16; d; d >>= 1)
-        st = merge(st, {__shfl_xor_sync(0xFFFFFFFFu, st.m, d), __shfl_xor_sync(0xFFFFFFFFu, st.s, d),
-                        __shfl_xor_sync(0xFFFFFFFFu, st.h, d)}, c);
+    for (int d = 16; d; d >>= 1) st = merge_lane<T>(st, d, c);
     if ((threadIdx.x & 31) == 0) warp_stat[threadIdx.x >> 5] = st;
     __syncthreads();
     if (threadIdx.x >= 32) return;
     st = warp_stat[threadIdx.x % (LB_THREADS / 32)];
 #pragma unroll
-    for (int d = LB_THREADS / 64; d; d >>= 1)
-        st = merge(st, {__shfl_xor_sync(0xFFFFFFFFu, st.m, d), __shfl_xor_sync(0xFFFFFFFFu, st.s, d),
-                        __shfl_xor_sync(0xFFFFFFFFu, st.h, d)}, c);
+    for (int d = LB_THREADS / 64; d; d >>= 1) st = merge_lane<T>(st, d, c);
     if (threadIdx.x == 0) stats[n * gridDim.x + blockIdx.x] = st;
 }
 
@@ -432,8 +568,8 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
 constexpr int LB_ROWS = 128;  // rows of a chunk at most
 
 struct GradRow {
-    float m, f, wt;  // u of the largest class, w / (t s), w / t
-    int y;           // -1: no gradient
+    float m, f;  // the largest u less r, w / (t s)
+    int r, y;    // y -1: no gradient
 };
 
 template <typename T>
@@ -441,6 +577,7 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
                                                              int parts, int chunks, int chunk, int period, const LossPart part) {
     constexpr int V = RowVecs<T>::V, U = 4;
     __shared__ GradRow rows[LB_ROWS];
+    __shared__ float wts[LB_ROWS];  // w / t
     __shared__ double red_dt[LB_THREADS / 32];
     cudaGridDependencySynchronize();
     const int K = a.k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -451,17 +588,20 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
     const int count = n0 < a.n ? (int)min((int64_t)chunk, (a.n - n0 + period - 1) / period) : 0;
     const float rt = loss_rt(a), c = loss_c(rt);
     double dt = 0.0;
+    [[maybe_unused]] int large = 0;  // rows with an r
     for (int i = threadIdx.x; i < count; i += LB_THREADS) {
         const int64_t n = n0 + (int64_t)i * period;
         const LossLabel label = loss_label(a, n);
-        GradRow r = {0.f, 0.f, 0.f, -1};
+        GradRow r = {0.f, 0.f, 0, -1};
         float loss = label.y >= 0 ? label.w * INFINITY : 0.f;
         if (label.open) {
             LossStat st = stats[n * parts];
-            for (int j = 1; j < parts; ++j) st = merge(st, stats[n * parts + j], c);
-            r = {st.m, label.w * rt / st.s, label.w * rt, label.y};
+            for (int j = 1; j < parts; ++j) st = merge<T>(st, stats[n * parts + j], c);
+            r = {st.m, label.w * rt / st.s, st.r, label.y};
+            wts[i] = label.w * rt;
+            large |= st.r;
             if (blockIdx.x == 0) {
-                const float gap = loss_u(to_f32(((const T *)a.cs)[n * a.cs_stride + label.y]), a.bias ? a.bias[label.y] : 0.f) - st.m;
+                const float gap = loss_u(class_sum(((const T *)a.cs)[n * a.cs_stride + label.y], st.r), a.bias ? a.bias[label.y] : 0.f) - st.m;
                 loss = label.w * (logf(st.s) - gap * rt);
                 dt += (double)label.w * ((double)(st.h / st.s) - (double)gap * (double)c);
             }
@@ -474,7 +614,8 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
         for (int d = 16; d; d >>= 1) dt += __shfl_xor_sync(0xFFFFFFFFu, dt, d);
         if (lane == 0) red_dt[warp] = dt;
     }
-    __syncthreads();
+    if constexpr (std::is_integral<T>::value) large = __syncthreads_or(large);
+    else __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         for (int i = 1; i < LB_THREADS / 32; ++i) dt += red_dt[i];
         if (chunks > 1) part.dt[id] = dt;
@@ -498,8 +639,8 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
             const GradRow r = rows[i];
             float d = 0.f;
             if (r.y >= 0) {
-                if (!mask || (*mask >> (k & 31)) & 1u) d = ex2(loss_x(loss_u(to_f32(*in), b), r.m, c)) * r.f;
-                if (r.y == k) d -= r.wt;
+                if (!mask || (*mask >> (k & 31)) & 1u) d = ex2(loss_x(loss_u(class_sum(*in, r.r), b), r.m, c)) * r.f;
+                if (r.y == k) d -= wts[i];
                 sum += d;
             }
             if (mask) mask += mask_step;
@@ -539,59 +680,73 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
     const char *in = (const char *)in0.at(vec);
     char *out = (char *)out0.at(vec);
     const uint32_t *mask = mask0 + (k0 >> 5);
-    for (int i0 = 0; i0 < count; i0 += U) {
-        uint4 raw[U];
-        uint32_t open[U], lo[U], hi[U];
+    const auto stream = [&](auto with_r) {
+        for (int i0 = 0; i0 < count; i0 += U) {
+            uint4 raw[U];
+            uint32_t open[U], lo[U], hi[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {  // loads only: a use between them would wait for each in turn
-            raw[u] = make_uint4(0, 0, 0, 0);
-            lo[u] = hi[u] = 0u;
-            if (i0 + u < count) {
-                raw[u] = *(const uint4 *)in;
-                if (masked) lo[u] = mask[0];
-                if (masked && straddle) hi[u] = mask[1];
+            for (int u = 0; u < U; ++u) {  // loads only: a use between them would wait for each in turn
+                raw[u] = make_uint4(0, 0, 0, 0);
+                lo[u] = hi[u] = 0u;
+                if (i0 + u < count) {
+                    raw[u] = *(const uint4 *)in;
+                    if (masked) lo[u] = mask[0];
+                    if (masked && straddle) hi[u] = mask[1];
+                }
+                in += in_step * (int64_t)sizeof(T);
+                mask += mask_step;
             }
-            in += in_step * (int64_t)sizeof(T);
-            mask += mask_step;
+#pragma unroll
+            for (int u = 0; u < U; ++u) open[u] = masked ? __funnelshift_r(lo[u], hi[u], k0 & 31) : shared_open;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i0 + u >= count) break;
+                const GradRow r = rows[i0 + u];
+                float d[V];
+                if (r.y >= 0) {
+                    const F2 m2 = pair(-r.m, -r.m), f2 = pair(r.f, r.f);
+#pragma unroll
+                    for (int q = 0; q < V / 2; ++q) split(class_pair<T>(raw[u], q), d[2 * q], d[2 * q + 1]);
+                    if constexpr (decltype(with_r)::value) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) d[j] = class_sum(((const T *)&raw[u])[j], r.r);
+                    }
+#pragma unroll
+                    for (int q = 0; q < V / 2; ++q) {
+                        float x, y;
+                        split(mul2(add2(add2(pair(d[2 * q], d[2 * q + 1]), b[q]), m2), c2), x, y);
+                        x = open[u] & (1u << (2 * q)) ? ex2(x) : 0.f;
+                        y = open[u] & (2u << (2 * q)) ? ex2(y) : 0.f;
+                        split(mul2(pair(x, y), f2), d[2 * q], d[2 * q + 1]);
+                    }
+                    if (r.y >= warp_k && r.y - warp_k < 32 * V) {  // the label's class is this warp's
+#pragma unroll
+                        for (int j = 0; j < V; ++j)
+                            if (r.y - k0 == j) d[j] -= wts[i0 + u];
+                    }
+#pragma unroll
+                    for (int q = 0; q < V / 2; ++q) acc[q] = add2(acc[q], pair(d[2 * q], d[2 * q + 1]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) d[j] = 0.f;
+                }
+                if constexpr (!std::is_integral<T>::value) {
+                    if (a.dcs) {
+                        alignas(16) T t[V];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) t[j] = from_f32<T>(d[j]);
+                        *(uint4 *)out = *(const uint4 *)t;
+                        out += out_step * (int64_t)sizeof(T);
+                    }
+                }
+            }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) open[u] = masked ? __funnelshift_r(lo[u], hi[u], k0 & 31) : shared_open;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i0 + u >= count) break;
-            const GradRow r = rows[i0 + u];
-            float d[V];
-            if (r.y >= 0) {
-                const F2 m2 = pair(-r.m, -r.m), f2 = pair(r.f, r.f);
-#pragma unroll
-                for (int q = 0; q < V / 2; ++q) {
-                    float x, y;
-                    split(mul2(add2(add2(class_pair<T>(raw[u], q), b[q]), m2), c2), x, y);
-                    x = open[u] & (1u << (2 * q)) ? ex2(x) : 0.f;
-                    y = open[u] & (2u << (2 * q)) ? ex2(y) : 0.f;
-                    split(mul2(pair(x, y), f2), d[2 * q], d[2 * q + 1]);
-                }
-                if (r.y >= warp_k && r.y - warp_k < 32 * V) {  // the label's class is this warp's
-#pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (r.y - k0 == j) d[j] -= r.wt;
-                }
-#pragma unroll
-                for (int q = 0; q < V / 2; ++q) acc[q] = add2(acc[q], pair(d[2 * q], d[2 * q + 1]));
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) d[j] = 0.f;
-            }
-            if constexpr (!std::is_integral<T>::value) {
-                if (a.dcs) {
-                    alignas(16) T t[V];
-#pragma unroll
-                    for (int j = 0; j < V; ++j) t[j] = from_f32<T>(d[j]);
-                    *(uint4 *)out = *(const uint4 *)t;
-                    out += out_step * (int64_t)sizeof(T);
-                }
-            }
-        }
+    };
+    if constexpr (std::is_integral<T>::value) {
+        if (large) stream(std::true_type());
+        else stream(std::false_type());
+    } else {
+        stream(std::false_type());
     }
     if (db) {
 #pragma unroll
