@@ -386,8 +386,8 @@ ytm_status ytm_q4_pack(const void *weights, int32_t w_type, int64_t w_stride, in
  * halves 0..15; bias f32 [K] or NULL; y [N][K].  f32 activations, and 16-bit
  * ones of one or two samples, are held to 2^-30 of the largest of their 128
  * neighbouring clauses (128 i .. 128 i + 127); several infinities among those
- * give NaN.  workspace:
- * ytm_q4_votes_workspace_bytes(...), on a 16-byte boundary. */
+ * give NaN.  workspace: ytm_q4_votes_workspace_bytes(...), on a 16-byte
+ * boundary; at most 1 GB, unless 64 samples' activations (in 16 bits) take more. */
 ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t N, int32_t C, const uint8_t *packed,
                         const void *scales, int32_t scale_type, int32_t group, int32_t K, const float *bias, void *y,
                         int32_t y_type, void *workspace, void *stream);

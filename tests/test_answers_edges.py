@@ -1,0 +1,15 @@
+"""CPU tests of the answer operators' argument checks and sizes at their edges."""
+import ctypes as ct
+
+import pytest
+
+from ytm_b200 import _lib
+
+
+@pytest.mark.parametrize("x", ["YTM_BITS", "YTM_F32", "YTM_F16", "YTM_BF16"])
+@pytest.mark.parametrize("c,k", [(33, 2), (2048, 1000), (10000, 10), (65536, 100), (65536, 4000), (1 << 20, 700)])
+@pytest.mark.parametrize("group", [32, 128])
+def test_votes_workspace_does_not_grow_with_the_samples(x, c, k, group):
+    size = lambda n: _lib.load().ytm_q4_votes_workspace_bytes(getattr(_lib, x), n, c, k, group)  # noqa: E731
+    sizes = [size(n) for n in (1, 64, 1000, 30000, 250000, 1 << 24, (1 << 31) - 1)]
+    assert all(0 < s <= 1 << 30 for s in sizes), sizes

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_answers import check_loss
+from tests.test_gpu_answers import check_loss, check_votes, votes_inputs
 from ytm_b200 import _lib, answers
 
 pytestmark = pytest.mark.gpu
@@ -179,3 +179,31 @@ def test_class_loss_tells_neighbouring_whole_sums_apart():
         q = 1 / (1 + np.exp(-1.0))
         np.testing.assert_allclose(f64(loss), [-np.log(q), -np.log(1 - q)], rtol=16 * U)
         np.testing.assert_allclose(f64(db)[:2], [2 * q - 1, 1 - 2 * q], rtol=32 * U)
+
+
+# ---------------------------------------------------------------- large batches
+
+@pytest.mark.parametrize("x,n,c,k", [("bits", 20001, 65536, 100), ("bits", 9001, 65536, 600), ("bf16", 9000, 65536, 520),
+                                     ("f32", 4100, 65536, 40)])
+def test_votes_of_more_activations_than_are_laid_out_at_once(x, n, c, k):
+    """Several launches of one call, against 64 bits for some of the samples and
+    against calls of 64 samples for all: two sums of the same terms, each within
+    the bound of check_votes."""
+    torch.manual_seed(n)
+    _, _, packed, q, scales, bias = votes_inputs(1, c, k, x, 64, "f32")
+    if x == "bits":
+        xt = torch.randint(-2 ** 31, 2 ** 31 - 1, (n, c // 32), dtype=torch.int32, device="cuda")
+        some = lambda r: ((xt[r].cpu().numpy().view(np.uint32)[:, np.arange(c) // 32] >> (np.arange(c) % 32)) & 1).astype(np.float64)  # noqa: E731
+        most = torch.ones((1, c), device="cuda")
+    else:
+        xt = torch.randn((n, c), device="cuda").to(DT[x])
+        some = lambda r: f64(xt[r])  # noqa: E731
+        most = xt.abs().amax(0, keepdim=True).float()
+    y = answers.q4_votes(xt, packed, scales, 64, bias=dev(bias), clauses=c)
+    rows, cols = np.r_[0:3, n // 2 - 40:n // 2 + 40, n - 3:n], np.r_[0:4, k - 4:k]
+    check_votes(y[rows][:, cols], some(rows), q[cols], scales[cols], 64, bias[cols], "f32", c)
+    parts = torch.cat([answers.q4_votes(xt[i:i + 64], packed, scales, 64, bias=dev(bias), clauses=c) for i in range(0, n, 64)])
+    w = dev(np.abs(q).astype(np.float32)) * scales.repeat_interleave(64, 1)[:, :c]
+    mag = ((most.double() @ w.double().t()) + dev(bias).abs()) * 1.001
+    depth = 64 + c // 64 + 64 + 1  # and the result's own rounding
+    assert ((y.double() - parts.double()).abs() <= 2 * depth * 2 * U * mag).all()

@@ -944,9 +944,22 @@ struct Q4Plan {
     int cols, samples, parts;  // of a block (columns padded); columns of a sample
     int wm, log_wk, cluster, stages;
     int64_t z, xs_block;       // blocks of samples of a launch, bytes of one's activations
+    int64_t launches;
     size_t smem;
     bool tiles;                // k_q4_tiles
 };
+
+// Bytes of activations laid out at once (clause bits become 8 to 16 times as large): a
+// call of more samples takes several launches (4096 bit samples of 65536 x 100 in two
+// launches: 450 us against 435).
+constexpr int64_t Q4_SCRATCH = 1 << 30;
+
+// Launches of `blocks` blocks of samples, equal but for the last.
+static void cut_launches(Q4Plan &p, int64_t blocks) {
+    const int64_t most = std::min<int64_t>(65535, std::max<int64_t>(1, Q4_SCRATCH / p.xs_block));
+    p.launches = cdiv(blocks, most);
+    p.z = cdiv(blocks, p.launches);
+}
 
 // Blocks of k_q4_tiles, and the least cost: a stage takes 1.0 to 2.8 us by the
 // number of its groups, a block 5 more to start and to end, 7 in a cluster.
@@ -954,17 +967,17 @@ static std::pair<Q4Plan, double> cut_tiles(Q4Plan p, int64_t N, int64_t C, int64
     p.tiles = true;
     p.samples = (int)cdiv(N, cdiv(N, (int64_t)64));
     p.cols = std::max(32, (p.samples + 15) / 16 * 16);
-    p.z = std::min<int64_t>(cdiv(N, p.samples), 65535);
     p.wm = QT_ROWS / 16;
     p.stages = (int)cdiv(C, Q4_SEG);
     p.xs_block = (int64_t)p.cols * 512 * p.stages;
+    cut_launches(p, cdiv(N, p.samples));
     p.smem = qt_stages(p.cols) * (QT_W_BYTES + (size_t)p.cols * 512) + QT_BARS;
     const double stage = (group == 32 ? 2.8 : group == 64 ? 1.7 : 1.15) * (p.cols == 32 ? 0.84 : 1.0);
     const int64_t sms = sm_count(), tiles = cdiv(K, QT_ROWS) * p.z;
     double least = 0;
     for (int cl = 1; cl <= 16 && (cl == 1 || cl <= p.stages); cl *= 2) {
         const int64_t place = cl == 16 ? sms * 3 / 4 : cl == 8 ? sms * 6 / 7 : sms;
-        const double cost = (double)cdiv(tiles * cl, place) * ((double)cdiv(p.stages, cl) * stage + (cl > 1 ? 7 : 5));
+        const double cost = p.launches * (double)cdiv(tiles * cl, place) * ((double)cdiv(p.stages, cl) * stage + (cl > 1 ? 7 : 5));
         if (!p.cluster || cost < least * 0.97) {
             p.cluster = cl;
             least = cost;
@@ -976,7 +989,6 @@ static std::pair<Q4Plan, double> cut_tiles(Q4Plan p, int64_t N, int64_t C, int64
 // Blocks of k_q4_votes of up to `most` samples, and the least cost.
 static std::pair<Q4Plan, double> cut(Q4Plan p, int64_t N, int64_t C, int64_t K, int group, int64_t most) {
     p.samples = (int)cdiv(N, cdiv(N, most));
-    p.z = std::min<int64_t>(cdiv(N, p.samples), 65535);
     const int used = p.samples * p.parts;
     p.cols = used <= 32 ? (used + 7) / 8 * 8 : used <= 48 ? 48 : 64;
     const int seg_bytes = q4_seg_bytes(p.mode, p.cols, group);
@@ -988,22 +1000,28 @@ static std::pair<Q4Plan, double> cut(Q4Plan p, int64_t N, int64_t C, int64_t K, 
         const size_t red = (size_t)Q4_WARPS * 16 * p.cols * 4 + (size_t)p.samples * 16 * wm * 4;
         const size_t smem = std::max<size_t>(Q4_STAGES * (Q4_STAGE_BYTES + (size_t)seg_bytes * wk), red) + Q4_BARS;
         if (smem > 227 * 1024) continue;
-        const int64_t tiles = cdiv(K, 16 * wm) * p.z, stages = cdiv(C, Q4_SEG * wk);
+        const int64_t stages = cdiv(C, Q4_SEG * wk);
+        Q4Plan q = p;
+        q.xs_block = (int64_t)seg_bytes * wk * stages;
+        cut_launches(q, cdiv(N, p.samples));
+        const int64_t tiles = cdiv(K, 16 * wm) * q.z;
         const int64_t held = std::max<int64_t>(1, std::min<int64_t>(nt == 1 ? 3 : nt <= 4 ? 2 : 1, 227 * 1024 / (smem + 1024)));  // blocks of an SM
         for (int cl = 1; cl <= 16 && (cl == 1 || cl <= stages); cl *= 2) {
             const int64_t place = cl == 16 ? sms * 3 / 4 : cl == 8 ? sms * 6 / 7 : sms;  // SMs that such clusters reach
             const int64_t rounds = tiles * cl / (place * held), rest = tiles * cl % (place * held);
             const auto stage = [&](int64_t r) { return std::max(0.37 * r, nt > 4 ? 0.19 * nt * r : 0.15 * nt * (1 + r)); };
             const double per = (double)cdiv(stages, cl);
-            const double cost = per * (rounds * stage(held) + (rest ? stage(cdiv(rest, place)) : 0)) +
-                                (rounds - (rest ? 0 : 1)) * (cl > 1 ? 6 : 3);
+            const double cost = q.launches * (per * (rounds * stage(held) + (rest ? stage(cdiv(rest, place)) : 0)) +
+                                              (rounds - (rest ? 0 : 1)) * (cl > 1 ? 6 : 3));
             if (!p.wm || cost < least * 0.97) {
                 p.wm = wm;
                 p.log_wk = log_wk;
                 p.cluster = cl;
                 p.stages = (int)stages;
                 p.smem = smem;
-                p.xs_block = (int64_t)seg_bytes * wk * stages;
+                p.xs_block = q.xs_block;
+                p.z = q.z;
+                p.launches = q.launches;
                 least = cost;
             }
         }
