@@ -782,20 +782,22 @@ __global__ void __launch_bounds__(QT_THREADS, 1) k_q4_tiles(const Q4Args a, cons
         // lane issues (an `if (lane == 0)` around all of this took 100 cycles a product).
         // fp32 sums; operands fp16 or bf16, both with the clauses innermost; 128 by COLS
         constexpr uint32_t SHAPE = 1u << 4 | (HALF ? 0u : 1u << 7 | 1u << 10) | (uint32_t)(COLS / 8) << 17 | 8u << 24;
+        // A stage's products; false if a wait gave up.  Its lanes may see that apart,
+        // so all go on to the end of the stage (the waits end at once then, and what
+        // the products find is this block's memory) and vote behind it.
         const auto issue = [&](auto product, int s) {
             constexpr int t = decltype(product)::value;
-            if (!bar_wait_inline(bar(bars.full[s % STAGES]), (s / STAGES) & 1, failed)) return false;
+            bool ok = bar_wait_inline(bar(bars.full[s % STAGES]), (s / STAGES) & 1, failed);
             // rows of 128 bytes under the 128-byte swizzle, eight of them 1024 bytes from the next eight
             const uint64_t x = (uint64_t)((smem_at + s % STAGES * STAGE + QT_W_BYTES) >> 4) | 1ull << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
 #pragma unroll
             for (int j = 0; j < NA; ++j) {
-                if (!bar_wait_inline(bar(bars.a_full[t][j]), s & 1, failed)) return false;
+                ok &= bar_wait_inline(bar(bars.a_full[t][j]), s & 1, failed);
 #pragma unroll
                 for (int k0 = 0; k0 < KB; k0 += GROUP) {  // products into one accumulator
                     const int g = (j * KB + k0) / GROUP;  // of the stage
                     // the accumulator's last turn: in this stage or the one before
-                    if ((s > 0 || g >= ND) && !bar_wait_inline(bar(bars.d_empty[t][g % ND]), (s * (GPS / ND) + g / ND - 1) & 1, failed))
-                        return false;
+                    if (s > 0 || g >= ND) ok &= bar_wait_inline(bar(bars.d_empty[t][g % ND]), (s * (GPS / ND) + g / ND - 1) & 1, failed);
                     tc_fence_after();
                     if (elected()) {
 #pragma unroll
@@ -809,7 +811,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) k_q4_tiles(const Q4Args a, cons
                     __syncwarp();
                 }
             }
-            return true;
+            return ok;
         };
         const auto run = [&](auto product) {
             bool ok = true;
