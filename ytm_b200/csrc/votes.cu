@@ -816,7 +816,10 @@ __global__ void __launch_bounds__(QT_THREADS, 1) k_q4_tiles(const Q4Args a, cons
         const auto run = [&](auto product) {
             bool ok = true;
             for (int s = 0; s < count && ok; ++s) ok = __all_sync(0xFFFFFFFFu, issue(product, s));
-            if (ok) return;
+            if (ok) {  // the last arrivals are still on their way to the barriers, whose memory goes with the block
+                if (count) bar_wait_inline(bar(bars.empty[(count - 1) % STAGES]), ((count - 1) / STAGES) & 1, failed);
+                return;
+            }
             // the products on their way still read their operands
             if (elected()) tc_commit(bar(bars.done[decltype(product)::value]));
             bar_poll(bar(bars.done[decltype(product)::value]), 0, nullptr);
