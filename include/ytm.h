@@ -393,6 +393,13 @@ ytm_status ytm_q4_votes(const void *x, int32_t x_type, int64_t x_stride, int64_t
                         int32_t y_type, void *workspace, void *stream);
 uint64_t ytm_q4_votes_workspace_bytes(int32_t x_type, int64_t N, int32_t C, int32_t K, int32_t group);
 
+/* Waits inside ytm_q4_votes end after about two seconds; a block that gave one up
+ * writes NaN votes.  *out: how many blocks did on the current device since the
+ * process began, among the calls that have ended: 0 unless the device is in
+ * trouble, so that NaN votes are those of the activations.  Synchronizes the
+ * stream. */
+ytm_status ytm_q4_votes_gave_up(uint64_t *out, void *stream);
+
 /* Fired clauses of inference as bits u32 [N][ceil(C / 32)] (bits behind the
  * last clause 0): the clauses ytm_infer counts, i.e. without those that
  * include nothing unless cfg->count_empty.  workspace:

@@ -13,3 +13,7 @@ def test_votes_workspace_does_not_grow_with_the_samples(x, c, k, group):
     size = lambda n: _lib.load().ytm_q4_votes_workspace_bytes(getattr(_lib, x), n, c, k, group)  # noqa: E731
     sizes = [size(n) for n in (1, 64, 1000, 30000, 250000, 1 << 24, (1 << 31) - 1)]
     assert all(0 < s <= 1 << 30 for s in sizes), sizes
+
+
+def test_gave_up_needs_a_place_for_the_count():
+    assert _lib.load().ytm_q4_votes_gave_up(None, None) == 1

@@ -207,3 +207,11 @@ def test_votes_of_more_activations_than_are_laid_out_at_once(x, n, c, k):
     mag = ((most.double() @ w.double().t()) + dev(bias).abs()) * 1.001
     depth = 64 + c // 64 + 64 + 1  # and the result's own rounding
     assert ((y.double() - parts.double()).abs() <= 2 * depth * 2 * U * mag).all()
+
+
+@pytest.mark.parametrize("n", [1, 3, 64])
+def test_nan_votes_of_nan_activations_are_no_wait_given_up(n):
+    xt, _, packed, _, scales, _ = votes_inputs(n, 1000, 3001, "bf16", 64, "f32")
+    xt[:, 7] = float("nan")
+    assert torch.isnan(answers.q4_votes(xt, packed, scales, 64)).all()
+    assert answers.q4_votes_gave_up() == 0 and answers.q4_votes_gave_up(xt.device) == 0

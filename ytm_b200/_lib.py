@@ -27,7 +27,7 @@ EXPORTS = (
     "ytm_encode_thermometer", "ytm_nccl_unique_id", "ytm_nccl_comm_init", "ytm_nccl_comm_destroy",
     "ytm_train_fit_batches", "ytm_peer_ar_create", "ytm_peer_ar_open", "ytm_peer_allreduce_i32",
     "ytm_peer_ar_status", "ytm_peer_ar_destroy", "ytm_config_size", "ytm_match_counters",
-    "ytm_q4_pack", "ytm_q4_votes", "ytm_q4_votes_workspace_bytes", "ytm_infer_fired", "ytm_answer", "ytm_class_loss", "ytm_class_loss_workspace_bytes",
+    "ytm_q4_pack", "ytm_q4_votes", "ytm_q4_votes_workspace_bytes", "ytm_q4_votes_gave_up", "ytm_infer_fired", "ytm_answer", "ytm_class_loss", "ytm_class_loss_workspace_bytes",
 )
 
 
@@ -125,6 +125,7 @@ _SIGS = {
     "ytm_q4_pack": ([_P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I32, _P], ct.c_int),
     "ytm_q4_votes": ([_P, _I32, _I64, _I64, _I32, _P, _P, _I32, _I32, _I32, _P, _P, _I32, _P, _P], ct.c_int),
     "ytm_q4_votes_workspace_bytes": ([_I32, _I64, _I32, _I32, _I32], _U64),
+    "ytm_q4_votes_gave_up": ([ct.POINTER(_U64), _P], ct.c_int),
     "ytm_infer_fired": ([_CFG, _P, _P, _I64, _P, _P, _P], ct.c_int),
     "ytm_answer": ([ct.POINTER(AnswerArgs), _P], ct.c_int),
     "ytm_class_loss": ([ct.POINTER(LossArgs), _P, _P], ct.c_int),

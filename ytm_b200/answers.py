@@ -17,6 +17,8 @@ autograd, and a tensor that requires grad is refused while grad mode is on.
 """
 from __future__ import annotations
 
+import ctypes as ct
+
 import numpy as np
 import torch
 
@@ -74,6 +76,17 @@ def q4_votes(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, group:
     largest of their 128 neighbouring clauses; several infinities among those
     give NaN."""
     return _bind.q4_votes(x, packed, scales, group, bias, clauses, out_dtype)
+
+
+def q4_votes_gave_up(device=None) -> int:
+    """How many blocks of q4_votes calls that have ended on the device (default:
+    the current one) gave up a wait, since the process began.  Their votes are
+    NaN; 0 unless the device is in trouble.  Waits for the current stream."""
+    out = ct.c_uint64()
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().ytm_q4_votes_gave_up(ct.byref(out), ct.c_void_p(torch.cuda.current_stream().cuda_stream)),
+                   "ytm_q4_votes_gave_up")
+    return out.value
 
 
 # -------------------------------------------------------------- adjusted class sums

@@ -291,6 +291,9 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     return bar_try(bar, parity) || bar_wait_long(bar, parity, failed);
 }
 
+// Blocks whose votes are NaN because a wait gave up (ytm_q4_votes_gave_up).
+__device__ unsigned long long g_gave_up;
+
 __device__ __forceinline__ float scale_value(uint32_t raw, int type) {
     if (type == YTM_F32) return __uint_as_float(raw);
     if (type == YTM_F16) return __half2float(__ushort_as_half((unsigned short)raw));
@@ -592,6 +595,7 @@ __global__ void __launch_bounds__(Q4_THREADS, COLS == 8 ? 3 : COLS <= 32 ? 2 : 1
             const int s = copied - 1 - tid;
             bar_try_long(full + 8 * (s % Q4_STAGES), (s / Q4_STAGES) & 1);
         }
+        if (tid == 0) atomicAdd(&g_gave_up, 1ull);
         __syncthreads();
     }
     // sums of the warps along the clauses and of the parts of an activation
@@ -932,6 +936,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1) k_q4_tiles(const Q4Args a, cons
             const int s = copied - 1 - tid;
             bar_poll(bar(bars.full[s % STAGES]), (s / STAGES) & 1, nullptr);
         }
+        if (tid == 0) atomicAdd(&g_gave_up, 1ull);
         __syncthreads();
         for (int u = tid; u < samples * QT_ROWS; u += QT_THREADS) mine[u] = NAN;
     }
@@ -1210,6 +1215,16 @@ ytm_status ytm_q4_pack(const void *weights, int32_t w_type, int64_t w_stride, in
         else k_q4_pack<<<grid, 128, 0, st>>>(w, w_stride, C, K, group, packed, (__nv_bfloat16 *)scales);
     }
     return launch_check("q4 pack");
+}
+
+ytm_status ytm_q4_votes_gave_up(uint64_t *out, void *stream) {
+    if (!out) return fail(YTM_ERR_ARG, "null pointer");
+    unsigned long long n = 0;
+    cudaStream_t st = as_stream(stream);
+    ytm_status rc = cuda_check(cudaMemcpyFromSymbolAsync(&n, g_gave_up, sizeof n, 0, cudaMemcpyDeviceToHost, st), "q4 votes given up");
+    if (!rc) rc = cuda_check(cudaStreamSynchronize(st), "q4 votes given up");
+    if (!rc) *out = n;
+    return rc;
 }
 
 uint64_t ytm_q4_votes_workspace_bytes(int32_t x_type, int64_t N, int32_t C, int32_t K, int32_t group) {
