@@ -2,8 +2,10 @@
 import ctypes as ct
 
 import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
-from ytm_b200 import _lib
+from ytm_b200 import _lib, answers
 
 
 @pytest.mark.parametrize("x", ["YTM_BITS", "YTM_F32", "YTM_F16", "YTM_BF16"])
@@ -17,3 +19,14 @@ def test_votes_workspace_does_not_grow_with_the_samples(x, c, k, group):
 
 def test_gave_up_needs_a_place_for_the_count():
     assert _lib.load().ytm_q4_votes_gave_up(None, None) == 1
+
+
+def test_tensors_without_memory_of_their_own_are_refused():
+    with FakeTensorMode():
+        cs, i = torch.empty((3, 8), device="cuda"), torch.empty(3, dtype=torch.int64, device="cuda")
+    for f in (lambda: answers.answer(cs), lambda: answers.class_loss(cs, i), lambda: answers.q4_pack(cs),
+              lambda: answers.q4_votes(cs, cs.byte(), cs, 32)):
+        with pytest.raises(ValueError, match="memory"):
+            f()
+    with pytest.raises(TypeError, match="strided"):
+        answers.answer(torch.zeros((3, 8)).to_sparse())

@@ -7,6 +7,8 @@ import ctypes as ct
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from tests.test_gpu_answers import check_loss, check_votes, votes_inputs
 from ytm_b200 import _lib, answers
@@ -215,3 +217,50 @@ def test_nan_votes_of_nan_activations_are_no_wait_given_up(n):
     xt[:, 7] = float("nan")
     assert torch.isnan(answers.q4_votes(xt, packed, scales, 64)).all()
     assert answers.q4_votes_gave_up() == 0 and answers.q4_votes_gave_up(xt.device) == 0
+
+
+# ------------------------------------------------------------- unusual tensors
+
+def test_forward_mode_tangents_are_refused():
+    z, i = torch.randn((3, 40), device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    p, s = answers.q4_pack(torch.ones((40, 8), device="cuda"), 32)
+    b = torch.zeros(40, device="cuda")
+    want = answers.answer(z)
+    with fwad.dual_level():
+        d, db = fwad.make_dual(z, torch.ones_like(z)), fwad.make_dual(b, torch.ones_like(b))
+        for f in (lambda: answers.answer(d), lambda: answers.answer(z, bias=db), lambda: answers.class_loss(d, i),
+                  lambda: answers.class_loss(z, i, bias=db), lambda: answers.q4_pack(d), lambda: answers.q4_votes(d, p, s, 32)):
+            with pytest.raises(ValueError, match="tangent"):
+                f()
+        with torch.no_grad(), fwad._set_fwd_grad_enabled(False):
+            got = answers.answer(d)
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+        assert torch.equal(answers.answer(fwad.unpack_dual(d).primal.detach())[1], want[1])
+
+
+def test_negated_views_are_read_with_their_sign():
+    z, i = torch.randn((3, 40), device="cuda"), torch.tensor([1, 2, 3], device="cuda")
+    b = torch.randn(40, device="cuda")
+    n, nb = torch._neg_view(z), torch._neg_view(b)
+    assert n.is_neg() and nb.is_neg()
+    p, s = answers.q4_pack(-z.t(), 32)
+    p2, s2 = answers.q4_pack(n.t(), 32)
+    assert torch.equal(p, p2) and torch.equal(s, s2)
+    p, s = answers.q4_pack(torch.randn((40, 5), device="cuda"), 32)
+    for got, want in ((answers.answer(n, bias=nb), answers.answer(-z, bias=-b)),
+                      (answers.class_loss(n, i, bias=nb), answers.class_loss(-z, i, bias=-b)),
+                      ((answers.q4_votes(n, p, s, 32),), (answers.q4_votes(-z, p, s, 32),))):
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_arguments_without_memory_of_their_own_are_refused():
+    """Such a bias or mask would have been no bias and no mask."""
+    z, i = torch.randn((3, 40), device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    with FakeTensorMode():
+        b, a = torch.empty(40, device="cuda"), torch.empty((3, 2), dtype=torch.int32, device="cuda")
+    for f in (lambda: answers.answer(z, bias=b), lambda: answers.answer(z, allowed=a), lambda: answers.class_loss(z, i, bias=b),
+              lambda: answers.class_loss(z, i, allowed=a), lambda: answers.answer(z, temperature=b[:3])):
+        with pytest.raises(ValueError, match="memory"):
+            f()
+    with pytest.raises(TypeError, match="strided"):
+        answers.answer(z.to_sparse())

@@ -13,7 +13,8 @@ tensors; they keep nothing between calls.  Rows may be strided or repeated
 (`expand`); a tensor whose rows are not contiguous inside is copied.  Wrong
 types, shapes or devices raise TypeError or ValueError before anything is
 launched.  The gradients come with the loss; none of the calls records into
-autograd, and a tensor that requires grad is refused while grad mode is on.
+autograd, and a tensor that requires grad is refused while grad mode is on, as
+is one with a forward-mode tangent.
 """
 from __future__ import annotations
 

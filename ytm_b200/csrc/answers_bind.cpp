@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -71,6 +72,7 @@ int ytm_type(ScalarType t) {
 Tensor need(PyObject *o, const char *name, int dim, unsigned types, const Tensor *with = nullptr) {
     if (!THPVariable_Check(o)) type_error(std::string(name) + " must be a torch tensor, got " + Py_TYPE(o)->tp_name);
     const Tensor &t = THPVariable_Unpack(o);
+    if (t.layout() != at::kStrided) type_error(std::string(name) + " must be strided, got " + c10::str(t.layout()));
     if (!(bit_of(t.scalar_type()) & types)) type_error(std::string(name) + " must be " + names(types) + ", got " + c10::toString(t.scalar_type()));
     if (t.dim() != dim) value_error(std::string(name) + " must have " + num(dim) + " dimension" + (dim > 1 ? "s" : "") + ", got " + num(t.dim()));
     if (!t.is_cuda()) value_error(std::string(name) + " must be on a CUDA device, got " + t.device().str());
@@ -78,6 +80,10 @@ Tensor need(PyObject *o, const char *name, int dim, unsigned types, const Tensor
         value_error(std::string(name) + " is on " + t.device().str() + ", the other tensors on " + with->device().str());
     if (t.requires_grad() && c10::GradMode::is_enabled())
         value_error(std::string(name) + " requires grad: these operators do not record into autograd (detach it)");
+    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        value_error(std::string(name) + " carries a forward-mode tangent: these operators do not compute one (detach it)");
+    if (t.numel() && !t.const_data_ptr()) value_error(std::string(name) + " has no memory of its own");
+    if (t.is_neg()) return t.resolve_neg().contiguous();
     return t.stride(-1) != 1 && t.size(-1) > 1 ? t.contiguous() : t;
 }
 
