@@ -12,6 +12,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 from tests.test_gpu_answers import check_loss, check_votes, votes_inputs
 from ytm_b200 import _lib, answers
+from ytm_b200.cutm import MultiClassTM
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -264,3 +265,29 @@ def test_arguments_without_memory_of_their_own_are_refused():
             f()
     with pytest.raises(TypeError, match="strided"):
         answers.answer(z.to_sparse())
+
+
+def test_knobs_without_dimensions():
+    """A tensor [] counts for all rows, on the device or, as a number, on the CPU."""
+    torch.manual_seed(0)
+    z, h = torch.randn((5, 40), device="cuda") * 4, torch.randint(0, 40, (5, 9), device="cuda")
+    kw = {"repetition": 1.25, "frequency": 0.5, "presence": 0.75, "temperature": 1.5}
+    want = answers.answer(z, history=h, **kw)
+    y = torch.tensor([0, 1, 2, 3, 39], device="cuda")
+    want_loss = answers.class_loss(z, y, temperature=1.5)
+    for make in (lambda v: torch.tensor(v, device="cuda"), torch.tensor, lambda v: torch.tensor(v, dtype=torch.float64), np.float32, np.array):
+        got = answers.answer(z, history=h, **{k: make(v) for k, v in kw.items()})
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        got = answers.class_loss(z, y, temperature=make(1.5))
+        assert all(a is b is None or torch.equal(a, b) for a, b in zip(got, want_loss))
+    with pytest.raises(TypeError, match="temperature"):
+        answers.answer(z, temperature=torch.tensor(1.5, device="cuda", dtype=torch.float64))
+    with pytest.raises(ValueError, match="positive"):
+        answers.answer(z, temperature=torch.tensor(-1.0))
+    tm = MultiClassTM(number_of_clauses_per_class=20, T=15, s=4.0, dim=(8, 8, 1), n_classes=3, seed=2)
+    X = (np.random.default_rng(0).random((6, 64)) < 0.4).astype(np.uint32)
+    tm.fit(X, np.arange(6) % 3)
+    want = tm.answer(X, temperature=2.5)
+    for t in (torch.tensor(2.5), torch.tensor(2.5, device="cuda"), torch.tensor(2.5, device="cuda", dtype=torch.float64), np.float64(2.5),
+              np.full(6, 2.5), torch.full((6,), 2.5)):
+        assert all(np.array_equal(a, b) for a, b in zip(tm.answer(X, temperature=t), want))

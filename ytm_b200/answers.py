@@ -109,7 +109,7 @@ def answer(cs: torch.Tensor, bias: torch.Tensor | None = None, allowed: torch.Te
     in 64 bits, rounded once to float32.  bias: float32 [k] or [n, k];
     allowed: bit words, int32 [n or 1, ceil(k / 32)] (`pack_allowed`);
     repetition, frequency, presence, temperature: numbers (used as float32), or
-    float32 [n], whose values are not checked.  choice is the lowest class of
+    float32 [n] or [], whose values are not checked.  choice is the lowest class of
     the largest z (NaN above all, as numpy's argmax), -1 where no class is
     allowed; logprob is log softmax(z) at the choice, -inf where no class is
     allowed."""
@@ -131,7 +131,7 @@ def class_loss(cs: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None
     target: int32 or int64 [n]; rows with a target outside [0, k) or a weight
     of 0 count for nothing.  A target that its mask forbids gives weight * inf
     and no gradient.  bias: float32 [k]; allowed as for `answer`; temperature:
-    a positive number or float32 [1], whose value is not checked; weight:
+    a positive number or float32 [1] or [], whose value is not checked; weight:
     float32 [n].  A NaN or +inf among a row's allowed class sums makes its loss
     and gradients NaN."""
     return _bind.class_loss(cs, target, bias, allowed, temperature, weight)

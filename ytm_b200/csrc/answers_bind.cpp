@@ -74,7 +74,7 @@ Tensor need(PyObject *o, const char *name, int dim, unsigned types, const Tensor
     const Tensor &t = THPVariable_Unpack(o);
     if (t.layout() != at::kStrided) type_error(std::string(name) + " must be strided, got " + c10::str(t.layout()));
     if (!(bit_of(t.scalar_type()) & types)) type_error(std::string(name) + " must be " + names(types) + ", got " + c10::toString(t.scalar_type()));
-    if (t.dim() != dim) value_error(std::string(name) + " must have " + num(dim) + " dimension" + (dim > 1 ? "s" : "") + ", got " + num(t.dim()));
+    if (t.dim() != dim) value_error(std::string(name) + " must have " + num(dim) + " dimension" + (dim != 1 ? "s" : "") + ", got " + num(t.dim()));
     if (!t.is_cuda()) value_error(std::string(name) + " must be on a CUDA device, got " + t.device().str());
     if (with && t.device() != with->device())
         value_error(std::string(name) + " is on " + t.device().str() + ", the other tensors on " + with->device().str());
@@ -84,7 +84,7 @@ Tensor need(PyObject *o, const char *name, int dim, unsigned types, const Tensor
         value_error(std::string(name) + " carries a forward-mode tangent: these operators do not compute one (detach it)");
     if (t.numel() && !t.const_data_ptr()) value_error(std::string(name) + " has no memory of its own");
     if (t.is_neg()) return t.resolve_neg().contiguous();
-    return t.stride(-1) != 1 && t.size(-1) > 1 ? t.contiguous() : t;
+    return dim && t.stride(-1) != 1 && t.size(-1) > 1 ? t.contiguous() : t;
 }
 
 Tensor vector(PyObject *o, const char *name, int64_t n, unsigned types, const Tensor &with) {
@@ -102,7 +102,8 @@ Tensor allowed_words(PyObject *o, int64_t n, int64_t k, const Tensor &with) {
 
 int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : 0; }
 
-// A number for all rows, or float32 [n].
+// A number for all rows (a tensor without dimensions on the CPU is one), or float32
+// [n], or [] for all rows.
 struct Knob {
     Tensor rows;
     float all = 0.f;
@@ -112,8 +113,11 @@ struct Knob {
 Knob knob(PyObject *o, const char *name, int64_t n, const Tensor &with, bool positive) {
     Knob k;
     if (THPVariable_Check(o)) {
-        k.rows = vector(o, name, n, F32, with);
-        return k;
+        const Tensor &t = THPVariable_Unpack(o);
+        if (t.dim() || t.is_cuda()) {
+            k.rows = t.dim() ? vector(o, name, n, F32, with) : need(o, name, 0, F32, &with).expand({n}).contiguous();
+            return k;
+        }
     }
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw Error{nullptr, ""};

@@ -57,7 +57,7 @@ class MultiClassTM(BaseTM):
         cs = self._score_device(self._literals_device(X, is_X_encoded), votes=votes)
         if allowed is not None:
             allowed = answers.pack_allowed(allowed, self.number_of_outputs).to(self.device)
-        knobs = {name: v if np.ndim(v) == 0 else self._on_device(v, torch.float32)
+        knobs = {name: v if np.ndim(v) == 0 and not isinstance(v, torch.Tensor) else self._on_device(v, torch.float32)
                  for name, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence),
                                  ("temperature", temperature))}
         choice, logprob, z = answers.answer(cs, bias=self._on_device(bias, torch.float32), allowed=allowed,
