@@ -467,6 +467,8 @@ typedef struct ytm_loss_args {
     float *dtemperature;      /* one value, or NULL                            */
 } ytm_loss_args;
 
+/* workspace: ytm_class_loss_workspace_bytes(...), on a 16-byte boundary (NULL if
+ * that is 0). */
 uint64_t ytm_class_loss_workspace_bytes(int64_t n, int32_t k, int32_t cs_type, int64_t cs_stride);
 ytm_status ytm_class_loss(const ytm_loss_args *args, void *workspace, void *stream);
 

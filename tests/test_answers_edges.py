@@ -30,3 +30,11 @@ def test_tensors_without_memory_of_their_own_are_refused():
             f()
     with pytest.raises(TypeError, match="strided"):
         answers.answer(torch.zeros((3, 8)).to_sparse())
+
+
+@pytest.mark.parametrize("k", [4, 1000])
+def test_loss_workspaces_off_a_boundary_are_refused(k):
+    """Sums of 8 bytes lie at its start."""
+    a = _lib.LossArgs(cs=16, cs_stride=k, n=100000, k=k, cs_type=_lib.YTM_I32, target=16, loss=16, temperature_all=1.0)
+    for at in (4, 8, 20):
+        assert _lib.load().ytm_class_loss(ct.byref(a), ct.c_void_p(at), None) == 1

@@ -926,6 +926,7 @@ ytm_status ytm_class_loss(const ytm_loss_args *args, void *workspace, void *stre
     const LossPlan p = loss_plan(a.n, a.k, type_bytes(a.cs_type), a.cs_stride);
     const LossWs ws = loss_ws(p, a.n, a.k);
     if (!a.cs || !a.target || !a.loss || (ws.total && !workspace)) return fail(YTM_ERR_ARG, "null pointer");
+    if ((uintptr_t)workspace % 16) return fail(YTM_ERR_ARG, "class loss: workspace must start on a 16-byte boundary");
     const LossPart part = {(float *)((char *)workspace + ws.db), (double *)workspace};
     LossStat *stats = (LossStat *)((char *)workspace + ws.stats);
     switch (a.cs_type) {
