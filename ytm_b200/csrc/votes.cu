@@ -1174,9 +1174,14 @@ static ytm_status launch_q4(const Q4XArgs &xa, unsigned x_blocks, const Q4Args &
         case 16: return launch_q4<MODE, 16>(a, p, map, group, grid, st);
         case 24: return launch_q4<MODE, 24>(a, p, map, group, grid, st);
         case 32: return launch_q4<MODE, 32>(a, p, map, group, grid, st);
-        case 48: return launch_q4<MODE, 48>(a, p, map, group, grid, st);
-        default: return launch_q4<MODE, 64>(a, p, map, group, grid, st);
+        default: break;
     }
+    // digits have up to 8 samples, 32 columns, a block
+    if constexpr (MODE != Q4_DIGITS) {
+        if (p.cols == 48) return launch_q4<MODE, 48>(a, p, map, group, grid, st);
+        if (p.cols == 64) return launch_q4<MODE, 64>(a, p, map, group, grid, st);
+    }
+    return fail(YTM_ERR_ARG, "q4 votes: no kernel of these columns");
 }
 
 static ytm_status check_q4(int32_t C, int32_t K, int32_t group, int32_t scale_type) {
