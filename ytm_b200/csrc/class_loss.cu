@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
         if constexpr (std::is_integral<T>::value) top = fmaxf(top, use ? fabsf(m) : 0.f);
         const float xy = loss_x(uy, m, c), ey = ex2(xy), others = s;
         s += ey;
-        const float f = row.label.w * rt / s;
+        const float rs = 1.f / s, f = row.label.w * rt * rs;
         if (use) {
             const F2 f2 = pair(f, f);
 #pragma unroll
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(LS_THREADS, E == 16 ? 2 : E == 8 ? 3 : 4) k_lo
             const float w = row.label.w, gap = uy - m;
             a.loss[n] = use ? w * (logf(s) - gap * rt) : row.label.y >= 0 ? w * INFINITY : 0.f;
             h = fmaf(ey, fmaxf(xy, -1024.f), h);
-            if (use) dt += (double)w * ((double)(h / s) - (double)gap * (double)c);
+            if (use) dt += (double)w * ((double)(h * rs) - (double)gap * (double)c);
         }
     }
     if constexpr (std::is_integral<T>::value) {
