@@ -347,26 +347,7 @@ __device__ __forceinline__ void bring_near(LossStat &a) {
     a.r = (int)r;
 }
 
-template <typename T>
-__device__ __forceinline__ LossStat merge(LossStat a, LossStat b, float c) {
-    if constexpr (std::is_integral<T>::value) {
-        if (a.r != b.r) {
-            if (a.m == -INFINITY) {
-                a.r = b.r;
-            } else if (b.m == -INFINITY) {
-                b.r = a.r;
-            } else {
-                bring_near(a);
-                bring_near(b);
-                const int r = max(a.r, b.r);
-                a.m = largest_less(a, r);
-                b.m = largest_less(b, r);
-                a.r = r;
-            }
-        }
-    } else {
-        a.r = 0;
-    }
+__device__ __forceinline__ LossStat merge_alike(const LossStat &a, const LossStat &b, float c) {
     const float m = fmaxf(a.m, b.m);
     // a.m == m: the factor is 1 also where both are infinite
     const float da = a.m == m ? 0.f : loss_x(a.m, m, c), db = b.m == m ? 0.f : loss_x(b.m, m, c);
@@ -378,12 +359,46 @@ __device__ __forceinline__ LossStat merge(LossStat a, LossStat b, float c) {
                       __fmul_rn(fb, fmaf(b.s, fmaxf(db, -1024.f), b.h))), a.r};
 }
 
-// merge with the lane d away.
+// Of statistics less different r.  A call, as such rows are rare and this would be
+// in the way of others.
+__device__ __noinline__ LossStat merge_apart(LossStat a, LossStat b, float c) {
+    if (a.m == -INFINITY) {
+        a.r = b.r;
+    } else if (b.m == -INFINITY) {
+        b.r = a.r;
+    } else {
+        bring_near(a);
+        bring_near(b);
+        const int r = max(a.r, b.r);
+        a.m = largest_less(a, r);
+        b.m = largest_less(b, r);
+        a.r = r;
+    }
+    return merge_alike(a, b, c);
+}
+
 template <typename T>
-__device__ __forceinline__ LossStat merge_lane(const LossStat &a, int d, float c) {
-    LossStat b = {__shfl_xor_sync(0xFFFFFFFFu, a.m, d), __shfl_xor_sync(0xFFFFFFFFu, a.s, d), __shfl_xor_sync(0xFFFFFFFFu, a.h, d), 0};
-    if constexpr (std::is_integral<T>::value) b.r = __shfl_xor_sync(0xFFFFFFFFu, a.r, d);
-    return merge<T>(a, b, c);
+__device__ __forceinline__ LossStat merge(const LossStat &a, const LossStat &b, float c) {
+    if (std::is_integral<T>::value && a.r != b.r) return merge_apart(a, b, c);
+    return merge_alike(a, b, c);
+}
+
+// Over `lanes` neighbouring lanes of a whole warp.
+template <typename T>
+__device__ __forceinline__ LossStat merge_lanes(LossStat a, int lanes, float c) {
+    if constexpr (std::is_integral<T>::value) {
+        if (__any_sync(0xFFFFFFFFu, a.r != 0)) {
+            for (int d = lanes / 2; d; d >>= 1)
+                a = merge<T>(a, {__shfl_xor_sync(0xFFFFFFFFu, a.m, d), __shfl_xor_sync(0xFFFFFFFFu, a.s, d),
+                                 __shfl_xor_sync(0xFFFFFFFFu, a.h, d), __shfl_xor_sync(0xFFFFFFFFu, a.r, d)}, c);
+            return a;
+        }
+    }
+#pragma unroll
+    for (int d = lanes / 2; d; d >>= 1)
+        a = merge_alike(a, {__shfl_xor_sync(0xFFFFFFFFu, a.m, d), __shfl_xor_sync(0xFFFFFFFFu, a.s, d),
+                            __shfl_xor_sync(0xFFFFFFFFu, a.h, d), 0}, c);
+    return a;
 }
 
 constexpr int LB_THREADS = 256;
@@ -546,14 +561,12 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_stat(const ytm_loss_args
             st = merge<T>(st, {u, u == -INFINITY ? 0.f : 1.f + (u - u), 0.f, r}, c);
         }
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) st = merge_lane<T>(st, d, c);
+    st = merge_lanes<T>(st, 32, c);
     if ((threadIdx.x & 31) == 0) warp_stat[threadIdx.x >> 5] = st;
     __syncthreads();
     if (threadIdx.x >= 32) return;
     st = warp_stat[threadIdx.x % (LB_THREADS / 32)];
-#pragma unroll
-    for (int d = LB_THREADS / 64; d; d >>= 1) st = merge_lane<T>(st, d, c);
+    st = merge_lanes<T>(st, LB_THREADS / 32, c);
     if (threadIdx.x == 0) stats[n * gridDim.x + blockIdx.x] = st;
 }
 
@@ -596,7 +609,18 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
         float loss = label.y >= 0 ? label.w * INFINITY : 0.f;
         if (label.open) {
             LossStat st = stats[n * parts];
-            for (int j = 1; j < parts; ++j) st = merge<T>(st, stats[n * parts + j], c);
+            for (int j0 = 1; j0 < parts; j0 += 4) {  // four loads at once
+                LossStat next[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) next[j] = stats[n * parts + min(j0 + j, parts - 1)];
+                if (std::is_integral<T>::value && (st.r | next[0].r | next[1].r | next[2].r | next[3].r)) {
+                    for (int j = 0; j < 4 && j0 + j < parts; ++j) st = merge<T>(st, stats[n * parts + j0 + j], c);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j0 + j < parts) st = merge_alike(st, next[j], c);
+                }
+            }
             r = {st.m, label.w * rt / st.s, st.r, label.y};
             wts[i] = label.w * rt;
             large |= st.r;
@@ -706,15 +730,12 @@ __global__ void __launch_bounds__(LB_THREADS, 4) k_loss_grad(const ytm_loss_args
                 if (r.y >= 0) {
                     const F2 m2 = pair(-r.m, -r.m), f2 = pair(r.f, r.f);
 #pragma unroll
-                    for (int q = 0; q < V / 2; ++q) split(class_pair<T>(raw[u], q), d[2 * q], d[2 * q + 1]);
-                    if constexpr (decltype(with_r)::value) {
-#pragma unroll
-                        for (int j = 0; j < V; ++j) d[j] = class_sum(((const T *)&raw[u])[j], r.r);
-                    }
-#pragma unroll
                     for (int q = 0; q < V / 2; ++q) {
                         float x, y;
-                        split(mul2(add2(add2(pair(d[2 * q], d[2 * q + 1]), b[q]), m2), c2), x, y);
+                        F2 v = class_pair<T>(raw[u], q);
+                        if constexpr (decltype(with_r)::value)
+                            v = pair(class_sum(((const T *)&raw[u])[2 * q], r.r), class_sum(((const T *)&raw[u])[2 * q + 1], r.r));
+                        split(mul2(add2(add2(v, b[q]), m2), c2), x, y);
                         x = open[u] & (1u << (2 * q)) ? ex2(x) : 0.f;
                         y = open[u] & (2u << (2 * q)) ? ex2(y) : 0.f;
                         split(mul2(pair(x, y), f2), d[2 * q], d[2 * q + 1]);
