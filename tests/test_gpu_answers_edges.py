@@ -174,6 +174,22 @@ def test_class_loss_of_large_whole_sums(k, mask, bias):
     check_whole_loss(cs[rows], y[rows], a[rows] if mask == "row" else a, b, 3.0, far[rows])
 
 
+@pytest.mark.parametrize("n,k", [(250, 10), (120, 100), (20000, 40), (3000, 257), (603, 9001), (1300, 600)])
+def test_class_loss_of_large_whole_sums_in_many_rows(n, k):
+    """Large sums and others in turn, in one thread's rows and in one row's rounds."""
+    rng = np.random.default_rng(n)
+    base = rng.choice(np.array(BASES), (n, 1))
+    y = rng.integers(0, k, n)
+    b = rng.normal(size=k).astype(np.float32)
+    check_whole_loss(base + rng.integers(0, 61, (n, k)), y, None, None, 7.5)
+    check_whole_loss(base + rng.integers(0, 61, (n, k)), y, None, b, 7.5)
+    # a row's classes in runs of different magnitude, the largest anywhere
+    runs = np.repeat(rng.integers(0, 32, (n, -(-k // 37))), 37, 1)[:, :k]
+    cs = np.where(rng.random((n, 1)) < 0.5, 1, -1) * (2 ** runs.astype(np.int64) - 1) + rng.integers(0, 2, (n, k))
+    cs = np.clip(cs, -2 ** 31, 2 ** 31 - 1)
+    check_whole_loss(cs, y, None, b, 2.0 ** 26)
+
+
 def test_class_loss_tells_neighbouring_whole_sums_apart():
     for k in (5, 700):
         cs = np.zeros((2, k), np.int32)
