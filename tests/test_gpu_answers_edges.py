@@ -10,6 +10,7 @@ import torch
 import torch.autograd.forward_ad as fwad
 from torch._subclasses.fake_tensor import FakeTensorMode
 
+from tests.answers_ref import nibbles
 from tests.test_gpu_answers import check_loss, check_votes, votes_inputs
 from ytm_b200 import _lib, answers
 from ytm_b200.cutm import MultiClassTM
@@ -307,3 +308,49 @@ def test_knobs_without_dimensions():
     for t in (torch.tensor(2.5), torch.tensor(2.5, device="cuda"), torch.tensor(2.5, device="cuda", dtype=torch.float64), np.float64(2.5),
               np.full(6, 2.5), torch.full((6,), 2.5)):
         assert all(np.array_equal(a, b) for a, b in zip(tm.answer(X, temperature=t), want))
+
+
+# ------------------------------------------------------- offsets past 32 bits
+
+def test_loss_and_answer_of_more_than_2_to_the_32_bytes_and_2_to_the_31_classes():
+    """The last rows of 2.2e9 class sums against the same rows alone: two sums of
+    the same k exponentials, each within (108 + 4 (k / 32 + 64)) u."""
+    n, k = 68000, 32001
+    cs = torch.empty((n, k), dtype=torch.bfloat16, device="cuda")
+    for i in range(0, n, 4000):
+        cs[i:i + 4000] = torch.randn((min(4000, n - i), k), device="cuda") * 4
+    y = torch.arange(n, device="cuda") % k
+    rel = 2 * (108 + 4 * (k / 32 + 64)) * U
+    loss, dcs, _, _ = answers.class_loss(cs, y)
+    some = [0, n // 2, n - 2, n - 1]
+    want = answers.class_loss(cs[some], y[some])
+    assert ((loss[some] - want[0]).abs() <= rel * (1 + want[0].abs())).all()
+    err = (dcs[some].double() - want[1].double()).abs()
+    assert (err <= 2.0 ** -7 * want[1].double().abs() + rel).all()  # a rounding each to bf16
+    del dcs
+    choice, logprob, z = answers.answer(cs, temperature=0.5)
+    c, lp, zz = answers.answer(cs[some], temperature=0.5)
+    assert torch.equal(choice[some], c) and torch.equal(z[some], zz)
+    assert ((logprob[some] - lp).abs() <= rel * (1 + lp.abs())).all()
+
+
+def test_votes_of_activations_and_weights_past_32_bits():
+    n, c, k = 66000, 33000, 5
+    _, _, packed, _, scales, bias = votes_inputs(1, c, k, "f32", 64, "f32")
+    x = torch.empty((n, c), dtype=torch.float16, device="cuda")
+    for i in range(0, n, 4000):
+        x[i:i + 4000] = torch.randn((min(4000, n - i), c), device="cuda")
+    y = answers.q4_votes(x, packed, scales, 64)
+    some = [0, n // 2, n - 2, n - 1]
+    q = nibbles(packed.cpu().numpy(), c).astype(np.int64) - 8
+    check_votes(y[some], f64(x[some]), q, scales, 64, np.zeros(k), "f32", c)
+    del x, y
+    torch.cuda.empty_cache()
+    c, k = 32768, 140001
+    packed = torch.randint(0, 256, (k, c // 2), dtype=torch.uint8, device="cuda")
+    scales = torch.rand((k, c // 64), device="cuda") + 0.1
+    for xs in (torch.randn((1, c), device="cuda"), torch.randn((64, c), device="cuda").half()):
+        y = answers.q4_votes(xs, packed, scales, 64)
+        some = [0, 70000, k - 2, k - 1]
+        q = nibbles(packed[some].cpu().numpy(), c).astype(np.int64) - 8
+        check_votes(y[:, some], f64(xs), q, scales[some], 64, np.zeros(4), "f32", c)
