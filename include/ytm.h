@@ -411,9 +411,11 @@ ytm_status ytm_infer_fired(const ytm_config *cfg, const uint32_t *state, const u
  * times k occurs in the first lengths[n] entries of history[n]:
  *   if c > 0: v = (v > 0 ? v / repetition : v * repetition) - frequency * c - presence
  *   z = allowed ? (v + bias) / temperature : -inf
- * in 64 bits, rounded once to fp32.  choice = the lowest class of the largest
- * z (NaN above all numbers), -1 if no class is allowed; logprob =
- * log softmax(z)[choice], -inf if no class is allowed. */
+ * in 64 bits (divisions as products with reciprocals), rounded once to fp32.
+ * choice = the lowest class of the largest z (NaN above all numbers), -1 if no
+ * class is allowed; logprob = log softmax(z)[choice], as -log1p of the sum of the
+ * other allowed classes' exp(z - z[choice]) (so 0 for an infinite z alone at the
+ * top), -inf if no class is allowed. */
 typedef struct ytm_answer_args {
     const void *cs;          /* [n][k], cs_type i32, f32, f16 or bf16          */
     int64_t cs_stride;
@@ -446,7 +448,8 @@ ytm_status ytm_answer(const ytm_answer_args *args, void *stream);
  * dtemperature = -sum d z / temperature, summed in a fixed order.  A NaN or
  * +inf among a row's allowed class sums makes its loss and its gradients NaN.  Rows whose
  * target lies outside [0, k) or whose weight is 0 count for nothing; a target
- * that the mask forbids gives a loss of weight * inf and no gradient. */
+ * that the mask forbids gives a loss of weight * inf and no gradient.  cs + bias
+ * is an fp32 sum; int32 class sums keep their differences at any size. */
 typedef struct ytm_loss_args {
     const void *cs;           /* [n][k], cs_type i32, f32, f16 or bf16         */
     int64_t cs_stride;

@@ -106,7 +106,8 @@ def answer(cs: torch.Tensor, bias: torch.Tensor | None = None, allowed: torch.Te
         if c > 0: v = (v > 0 ? v / repetition : v * repetition) - frequency * c - presence
         z = (v + bias) / temperature if allowed else -inf
 
-    in 64 bits, rounded once to float32.  bias: float32 [k] or [n, k];
+    in 64 bits (divisions as products with reciprocals), rounded once to
+    float32.  bias: float32 [k] or [n, k];
     allowed: bit words, int32 [n or 1, ceil(k / 32)] (`pack_allowed`);
     repetition, frequency, presence, temperature: numbers (used as float32), or
     float32 [n] or [], whose values are not checked.  choice is the lowest class of
@@ -132,6 +133,7 @@ def class_loss(cs: torch.Tensor, target: torch.Tensor, bias: torch.Tensor | None
     of 0 count for nothing.  A target that its mask forbids gives weight * inf
     and no gradient.  bias: float32 [k]; allowed as for `answer`; temperature:
     a positive number or float32 [1] or [], whose value is not checked; weight:
-    float32 [n].  A NaN or +inf among a row's allowed class sums makes its loss
+    float32 [n].  cs + bias is a float32 sum; int32 class sums keep their
+    differences at any size.  A NaN or +inf among a row's allowed class sums makes its loss
     and gradients NaN."""
     return _bind.class_loss(cs, target, bias, allowed, temperature, weight)

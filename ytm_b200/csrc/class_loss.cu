@@ -22,10 +22,13 @@
 // kernels sum dbias in registers and leave one part per team or chunk, which
 // k_loss_join adds in a fixed order.
 //
-// Measured with a bias: 262144 x 100 int32 51 us (2.1 TB/s; bound by some 20
-// instructions a class), with row masks 64; 2047 x 32001 bf16 118 us, with row
-// masks 145 (393 MB in two streams, 3.3 and 2.7 TB/s; bound by instructions and
-// latency in both: the first reads the bias again for every row, 15 us of it).
+// Measured with a bias, calls back to back: 262144 x 100 int32 53 us (the first
+// kernel 50, 2.1 TB/s: 37 instructions a class, 27 us of issue, which the 16 warps
+// of an SM, with 122 registers a thread, fill to 57%: they wait for their loads and
+// for the row's sums), fp32 62, bf16 56, bf16 with row masks 72; 2047 x 32001 bf16
+// 119 us, with row masks 145 (393 MB in two streams, 3.3 and 2.7 TB/s; both issue
+// 57% of the time, 60 and 64 registers: instructions, and loads waited for; the
+// first reads the bias again for every row, 15 us of it).
 // One pass with a cluster a row, the exponentials kept, took 583 us: labels and
 // clusters waited for, with half of the clusters that would fill the SMs.
 #include <float.h>
